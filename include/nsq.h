@@ -299,6 +299,75 @@ typedef struct nsq_xsegment {
 int nsq_gemv_multi_xchg(const nsq_xsegment *segs, int nseg, const float *x, int64_t M, int64_t K,
                         nsq_comm *comm, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- Linear operator: bias, activation and residual in the epilogue ----
+ *
+ * y[M x N] = act(x[M x K] . W^T + bias) + residual, one product and its
+ * epilogue instead of the reference's matmul, add, silu and add dispatches
+ * (crates/nodestor-vulkan/src/transformer.rs:241-321).
+ *   dtype     element type of x, residual and y: NSQ_OUT_F32 or NSQ_OUT_BF16
+ *   bias      N f32, or NULL;  act: NSQ_ACT_*
+ *   residual  [M x N] of dtype, or NULL; may be y itself
+ * M = 1..16: fp16 hi + lo activations, exact products, f32 sums; about 3e-7
+ * relative for f32 (bf16 results are rounded once).  K is a multiple of the
+ * type's block.  `workspace` (nsq_linear_workspace_size(M, K) bytes, 16-byte
+ * aligned) holds the prepared activations; one call at a time uses it. */
+#define NSQ_ACT_NONE 0
+#define NSQ_ACT_SILU 1      /* v / (1 + e^-v) */
+#define NSQ_ACT_GELU 2      /* v (1 + erf(v / sqrt 2)) / 2 */
+#define NSQ_ACT_GELU_TANH 3 /* v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2 */
+#define NSQ_ACT_RELU 4
+size_t nsq_linear_workspace_size(int64_t M, int64_t K);
+int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, const float* bias, int act,
+               const void* residual, void* y, int dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+               size_t workspace_bytes, void* stream);
+
+/* ---- Mixture-of-experts feed-forward layer for a few tokens ----
+ *
+ * The experts' matrices are GGUF tensors [E x rows x K] as they lie in the
+ * file (ffn_gate_exps, ffn_up_exps, ffn_down_exps):
+ *   h_j  = act(x . W_gate[e_j]^T) * (x . W_up[e_j]^T)        [n_ff]
+ *   y[m] = residual[m] + sum_j weight[m, j] * (h_j . W_down[e_j]^T)
+ * over the top_k picks e_j = ids[m, j] of token m.  All tensors but the
+ * experts are f32; residual may be NULL or y itself.  Accuracy as
+ * nsq_linear's f32.  A reference routing shader exists but is never built
+ * (crates/nodestor-vulkan/build.rs:24, moe_routing). */
+typedef struct nsq_moe {
+  const void *w_gate; /* [E x n_ff rows of n_embd], type_in, 16-byte aligned */
+  const void *w_up;   /* the same */
+  const void *w_down; /* [E x n_embd rows of n_ff], type_down */
+  int type_in, layout_in, type_down, layout_down;
+  int act;            /* NSQ_ACT_*: SILU for SwiGLU experts */
+  int64_t n_expert, n_embd, n_ff;
+} nsq_moe;
+
+#define NSQ_MOE_MAX_TOKENS 64
+#define NSQ_MOE_MAX_EXPERTS 512
+#define NSQ_MOE_MAX_TOP_K 16
+
+size_t nsq_moe_workspace_size(const nsq_moe* moe, int64_t M, int64_t top_k);
+
+/* The experts' products for given picks: ids [M x top_k], weights [M x
+ * top_k].  An id outside 0..E-1 (for instance -1) marks an unused slot: it
+ * adds nothing, and a token without picks gets its residual (or zero).  An
+ * expert named twice by a token counts once with the sum of the weights. */
+int nsq_moe_ffn(const nsq_moe* moe, const float* x, const int32_t* ids, const float* weights, const float* residual,
+                float* y, int64_t M, int64_t top_k, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The whole layer: router, picks and experts.  logits = x . w_router^T
+ * (w_router [E x n_embd] f32, sums in f64).
+ *   NSQ_SCORE_SOFTMAX       s = softmax(logits); weight = scale * s
+ *   NSQ_SCORE_SOFTMAX_NORM  the same, divided by the sum over the picks
+ *   NSQ_SCORE_SIGMOID_NORM  s = sigmoid(logits), divided likewise
+ * The picks are the top_k largest of s (+ sel_bias[E], which may be NULL and
+ * does not enter the weights), largest first, of equal ones the lowest id;
+ * a NaN score comes last.  ids and weights [M x top_k] are written. */
+#define NSQ_SCORE_SOFTMAX 0
+#define NSQ_SCORE_SOFTMAX_NORM 1
+#define NSQ_SCORE_SIGMOID_NORM 2
+int nsq_moe_layer(const nsq_moe* moe, const float* w_router, int score, const float* sel_bias, float scale,
+                  const float* x, const float* residual, float* y, int32_t* ids, float* weights, int64_t M,
+                  int64_t top_k, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- NSZ (NodeStor Zip) lossless tensors and ZipGEMM ----
  *
  * An NSZ tensor is the tile stream one index entry of an .nsz file points at

@@ -28,6 +28,17 @@ pub const NSQ_OUT_BF16: c_int = 1;
 pub const NSQ_GEMV_MAX_M: i64 = 16;
 pub const NSQ_NOALLOC_MAX_ELEMS: i64 = 262144;
 pub const NSQ_NSZ_FP32: c_int = 0;
+pub const NSQ_ACT_NONE: c_int = 0;
+pub const NSQ_ACT_SILU: c_int = 1;
+pub const NSQ_ACT_GELU: c_int = 2;
+pub const NSQ_ACT_GELU_TANH: c_int = 3;
+pub const NSQ_ACT_RELU: c_int = 4;
+pub const NSQ_SCORE_SOFTMAX: c_int = 0;
+pub const NSQ_SCORE_SOFTMAX_NORM: c_int = 1;
+pub const NSQ_SCORE_SIGMOID_NORM: c_int = 2;
+pub const NSQ_MOE_MAX_TOKENS: i64 = 64;
+pub const NSQ_MOE_MAX_EXPERTS: i64 = 512;
+pub const NSQ_MOE_MAX_TOP_K: i64 = 16;
 
 #[repr(C)]
 #[derive(Clone, Copy)]
@@ -49,6 +60,22 @@ pub struct NsqXSegment {
     pub row0: i64,
     pub n_full: i64,
     pub y_off: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct NsqMoe {
+    pub w_gate: *const c_void,
+    pub w_up: *const c_void,
+    pub w_down: *const c_void,
+    pub type_in: c_int,
+    pub layout_in: c_int,
+    pub type_down: c_int,
+    pub layout_down: c_int,
+    pub act: c_int,
+    pub n_expert: i64,
+    pub n_embd: i64,
+    pub n_ff: i64,
 }
 
 #[repr(C)]
@@ -87,6 +114,19 @@ extern "C" {
                          y_bf16: *mut c_void, m: i64, n: i64, k: i64, stream: *mut c_void) -> c_int;
     pub fn nsq_matmul_f32(a: *const f32, b: *const f32, c: *mut f32, m: i64, k: i64, n: i64,
                           stream: *mut c_void) -> c_int;
+    // bias, activation and residual in the epilogue; mixture-of-experts layers
+    pub fn nsq_linear_workspace_size(m: i64, k: i64) -> usize;
+    pub fn nsq_linear(w: *const c_void, ggml_type: c_int, q6k_layout: c_int, x: *const c_void, bias: *const f32,
+                      act: c_int, residual: *const c_void, y: *mut c_void, dtype: c_int, m: i64, n: i64, k: i64,
+                      workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn nsq_moe_workspace_size(moe: *const NsqMoe, m: i64, top_k: i64) -> usize;
+    pub fn nsq_moe_ffn(moe: *const NsqMoe, x: *const f32, ids: *const i32, weights: *const f32,
+                       residual: *const f32, y: *mut f32, m: i64, top_k: i64, workspace: *mut c_void,
+                       workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn nsq_moe_layer(moe: *const NsqMoe, w_router: *const f32, score: c_int, sel_bias: *const f32, scale: f32,
+                         x: *const f32, residual: *const f32, y: *mut f32, ids: *mut i32, weights: *mut f32,
+                         m: i64, top_k: i64, workspace: *mut c_void, workspace_bytes: usize,
+                         stream: *mut c_void) -> c_int;
     // row-sharded decode over the GPUs of a node (one process per GPU)
     pub fn nsq_comm_handle_bytes() -> usize;
     pub fn nsq_comm_create(world: c_int, rank: c_int, bytes: usize, comm: *mut *mut NsqComm,

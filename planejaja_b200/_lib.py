@@ -30,6 +30,12 @@ NSZ_TILE_WEIGHTS = 512
 
 OUT_F32 = 0
 OUT_BF16 = 1
+
+ACTS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
+SCORES = {"softmax": 0, "softmax_norm": 1, "sigmoid_norm": 2}
+MOE_MAX_TOKENS = 64
+MOE_MAX_EXPERTS = 512
+MOE_MAX_TOP_K = 16
 GEMV_MAX_M = 16
 
 # (name, restype, argtypes) for every symbol declared in include/nsq.h
@@ -60,6 +66,12 @@ SIGNATURES = [
     ("nsq_comm_wait", _int, [_vp, _vp]),
     ("nsq_comm_destroy", _int, [_vp]),
     ("nsq_gemv_multi_xchg", _int, [ctypes.c_void_p, _int, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    ("nsq_linear_workspace_size", _sz, [_i64, _i64]),
+    ("nsq_linear", _int, [_vp, _int, _int, _vp, _vp, _int, _vp, _vp, _int, _i64, _i64, _i64, _vp, _sz, _vp]),
+    ("nsq_moe_workspace_size", _sz, [_vp, _i64, _i64]),
+    ("nsq_moe_ffn", _int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp]),
+    ("nsq_moe_layer", _int, [_vp, _vp, _int, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz,
+                             _vp]),
     ("nsq_nsz_num_tiles", _i64, [_i64]),
     ("nsq_nsz_index", _int, [_vp, _i64, _i64, _int, _vp]),
     ("nsq_nsz_decode", _int, [_vp, _vp, _i64, _int, _vp, _vp]),
@@ -78,6 +90,14 @@ class XSegment(ctypes.Structure):
     _fields_ = [("w", ctypes.c_void_p), ("ggml_type", ctypes.c_int), ("q6k_layout", ctypes.c_int),
                 ("N", ctypes.c_int64), ("row0", ctypes.c_int64), ("n_full", ctypes.c_int64),
                 ("y_off", ctypes.c_int64)]
+
+
+class Moe(ctypes.Structure):
+    """struct nsq_moe (include/nsq.h): the experts of a mixture-of-experts layer."""
+    _fields_ = [("w_gate", ctypes.c_void_p), ("w_up", ctypes.c_void_p), ("w_down", ctypes.c_void_p),
+                ("type_in", ctypes.c_int), ("layout_in", ctypes.c_int), ("type_down", ctypes.c_int),
+                ("layout_down", ctypes.c_int), ("act", ctypes.c_int), ("n_expert", ctypes.c_int64),
+                ("n_embd", ctypes.c_int64), ("n_ff", ctypes.c_int64)]
 
 
 MAX_SEGMENTS = 4

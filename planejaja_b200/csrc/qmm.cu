@@ -1,0 +1,349 @@
+// qmm.cu -- the linear operator (nsq_linear) and the mixture-of-experts layer
+// (nsq_moe_ffn, nsq_moe_layer): preparation kernel, launch planning, checks.
+#include "qmm.cuh"
+
+namespace nsq {
+
+int launch_qmm_q4k(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q5k(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q6k(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q40(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q80(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
+int check_weights(const void* w, int type, int layout, int64_t K);
+int device_check(int* num_sms);
+
+constexpr int kRouteTok = 8;  // tokens of one CTA's logits
+
+// Activation records of rows x nsb units (one warp each) and, in the first
+// nlog CTAs, the router's logits.  Two experts' logits may lie arbitrarily
+// close, and a pick that flips changes the output by whole experts: products
+// of f32 are exact in f64, and the sums are f64.  The f64 units do 64 FMA per
+// SM and cycle; 16 tokens, 128 experts and K = 2048 take under half a
+// microsecond of them.
+template <typename T>
+__global__ void __launch_bounds__(kQmmThreads) qmm_prep_kernel(const T* __restrict__ x, int rows, int64_t K, int nsb,
+                                                               int order, uint8_t* __restrict__ recs,
+                                                               const float* __restrict__ router, int E,
+                                                               double* __restrict__ logits, int nlog) {
+  qmm_dep_wait();
+  qmm_dep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (sizeof(T) == 4) {
+    if ((int)blockIdx.x < nlog) {
+      __shared__ double part[kQmmWarps][kRouteTok];
+      const int e = blockIdx.x % E, m0 = (blockIdx.x / E) * kRouteTok;
+      const int mc = min(kRouteTok, rows - m0);
+      double acc[kRouteTok] = {};
+      const float* w = router + (int64_t)e * K;
+      const bool wide = ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(x)) & 15) == 0;  // K % 32 == 0
+      for (int64_t k = 4 * threadIdx.x; k < K; k += 4 * kQmmThreads) {
+        float4 a;
+        if (wide) {
+          a = *reinterpret_cast<const float4*>(w + k);
+        } else {
+          a = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+        }
+        const double a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w;
+#pragma unroll
+        for (int t = 0; t < kRouteTok; ++t) {
+          if (t < mc) {
+            const T* xr = x + (int64_t)(m0 + t) * K + k;
+            float4 b;
+            if (wide) {
+              b = *reinterpret_cast<const float4*>(xr);
+            } else {
+              b = make_float4(xr[0], xr[1], xr[2], xr[3]);
+            }
+            acc[t] = fma(a0, (double)b.x, fma(a1, (double)b.y, fma(a2, (double)b.z, fma(a3, (double)b.w, acc[t]))));
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < kRouteTok; ++t) {
+        if (t < mc) {
+          double v = acc[t];
+#pragma unroll
+          for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          if (lane == 0) part[warp][t] = v;
+        }
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < mc) {
+        double v = 0.0;
+        for (int i = 0; i < kQmmWarps; ++i) v += part[i][threadIdx.x];
+        logits[(int64_t)(m0 + threadIdx.x) * E + e] = v;
+      }
+      return;
+    }
+  }
+  const int64_t job = (int64_t)(blockIdx.x - nlog) * kQmmWarps + warp;
+  if (job >= (int64_t)rows * nsb) return;
+  const int64_t row = job / nsb;
+  const int sb = (int)(job - row * nsb);
+  qmm_make_record(x + row * K + 256 * sb, (int)min((int64_t)256, K - 256 * sb), order, recs + job * kQmmRec, lane);
+}
+
+template <typename T>
+static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* recs, const float* router, int E,
+                       double* logits, cudaStream_t st) {
+  const int nsb = (int)((K + 255) / 256);
+  const int nlog = router ? E * (int)((rows + kRouteTok - 1) / kRouteTok) : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(nlog + (rows * nsb + kQmmWarps - 1) / kQmmWarps));
+  cfg.blockDim = dim3(kQmmThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  note_launch();
+  return cudaLaunchKernelEx(&cfg, qmm_prep_kernel<T>, x, (int)rows, K, nsb, order, recs, router, E, logits, nlog) ==
+                 cudaSuccess
+             ? NSQ_OK
+             : NSQ_ERR_CUDA;
+}
+
+static int qmm_pitch(int type) {
+  switch (type) {
+    case NSQ_TYPE_Q4_K: return QmmFmt<NSQ_TYPE_Q4_K>::PITCH;
+    case NSQ_TYPE_Q5_K: return QmmFmt<NSQ_TYPE_Q5_K>::PITCH;
+    case NSQ_TYPE_Q6_K: return QmmFmt<NSQ_TYPE_Q6_K>::PITCH;
+    case NSQ_TYPE_Q4_0: return QmmFmt<NSQ_TYPE_Q4_0>::PITCH;
+    default: return QmmFmt<NSQ_TYPE_Q8_0>::PITCH;
+  }
+}
+
+// Plans and launches one product.  groups: the most groups there can be.
+static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream_t st, int num_sms) {
+  // columns of K per CTA: the records of a unit are read by the RW = 8 / KW
+  // warps that share it, so more tokens want more rows per unit
+  int KW = p.TS <= 1 ? 8 : p.TS <= 4 ? 4 : p.TS <= 8 ? 2 : 1;
+  const int64_t most_units = p.mode == kQmmDown ? groups * p.nsb : p.nsb;
+  while (KW > 1 && KW / 2 >= most_units) KW /= 2;
+  p.KW = KW;
+  p.RW = kQmmWarps / KW;
+  const int64_t tile_rows = (p.mode == kQmmUp ? 8 : 16) * p.RW;
+  const int64_t tiles = (p.n + tile_rows - 1) / tile_rows;
+  const int64_t slots = 2 * (int64_t)num_sms;
+  p.split = 1;
+  if (p.mode != kQmmUp) {
+    // a K split over a cluster while the tiles leave half of the CTA slots
+    // empty and every CTA keeps a step of units
+    while (p.split < 8 && tiles * p.split * 2 <= slots && most_units >= (int64_t)p.split * 2 * KW) p.split *= 2;
+  }
+  const int pitch = qmm_pitch(type);
+  const int P = p.mode == kQmmLinear ? 0 : p.M * p.top_k;
+  const size_t fixed = (size_t)kQmmWarps * p.YC * 16 * 4 + (p.split > 1 ? (size_t)p.YC * 16 * p.RW * 4 : 0) + qmm_lists_bytes(P);
+  const size_t stage = qmm_stage_bytes(pitch, p.KW, p.TS);
+  p.stages = 4;
+  while (p.stages > 2 && fixed + p.stages * stage > (size_t)kQmmSmemHalf) --p.stages;
+  size_t smem = fixed + p.stages * stage;
+  if (smem < (size_t)P * 8) smem = (size_t)P * 8;
+  if (smem > (size_t)kQmmSmemMax) return NSQ_ERR_SHAPE;
+  const int64_t tasks = tiles * (p.mode == kQmmUp ? groups : 1);
+  int64_t grid = (tasks < slots / p.split ? tasks : slots / p.split) * p.split;
+  if (grid < p.split) grid = p.split;
+  switch (type) {
+    case NSQ_TYPE_Q4_K: return launch_qmm_q4k(layout, p, (int)grid, smem, st);
+    case NSQ_TYPE_Q5_K: return launch_qmm_q5k(layout, p, (int)grid, smem, st);
+    case NSQ_TYPE_Q6_K: return launch_qmm_q6k(layout, p, (int)grid, smem, st);
+    case NSQ_TYPE_Q4_0: return launch_qmm_q40(layout, p, (int)grid, smem, st);
+    case NSQ_TYPE_Q8_0: return launch_qmm_q80(layout, p, (int)grid, smem, st);
+    default: return NSQ_ERR_TYPE;
+  }
+}
+
+static int64_t units_of(int64_t K) { return (K + 255) / 256; }
+static bool act_ok(int act) { return act >= NSQ_ACT_NONE && act <= NSQ_ACT_RELU; }
+
+// Workspace of a mixture-of-experts call, in this order.
+struct MoeSpace {
+  size_t logits, recs_x, h, recs_h, groups, plist, pwts, ngroups, total;
+};
+static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t top_k) {
+  MoeSpace s{};
+  const int64_t P = M * top_k;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) & ~size_t(255);
+    return here;
+  };
+  s.logits = take((size_t)(M * E) * 8);
+  s.recs_x = take((size_t)(M * units_of(D)) * kQmmRec);
+  s.h = take((size_t)(P * F) * 4);
+  s.recs_h = take((size_t)(P * units_of(F)) * kQmmRec);
+  s.groups = take((size_t)P * sizeof(QmmGroup));
+  s.plist = take((size_t)P * 4);
+  s.pwts = take((size_t)P * 4);
+  s.ngroups = take(4);
+  s.total = at;
+  return s;
+}
+
+static int check_moe(const nsq_moe* moe, int64_t M, int64_t top_k) {
+  if (!moe) return NSQ_ERR_NULL;
+  if (moe->n_expert < 1 || moe->n_expert > NSQ_MOE_MAX_EXPERTS || moe->n_embd < 1 || moe->n_ff < 1) return NSQ_ERR_SHAPE;
+  if (moe->n_embd > (1 << 20) || moe->n_ff > (1 << 20)) return NSQ_ERR_SHAPE;
+  if (M < 1 || M > NSQ_MOE_MAX_TOKENS || top_k < 1 || top_k > NSQ_MOE_MAX_TOP_K || top_k > moe->n_expert)
+    return NSQ_ERR_SHAPE;
+  if (!act_ok(moe->act)) return NSQ_ERR_TYPE;
+  int rc;
+  if ((rc = check_weights(moe->w_gate, moe->type_in, moe->layout_in, moe->n_embd))) return rc;
+  if ((rc = check_weights(moe->w_up, moe->type_in, moe->layout_in, moe->n_embd))) return rc;
+  return check_weights(moe->w_down, moe->type_down, moe->layout_down, moe->n_ff);
+}
+
+// Both entry points: the router's part is left out when w_router is NULL.
+static int run_moe(const nsq_moe* moe, const float* w_router, int score, const float* sel_bias, float scale,
+                   const float* x, const float* residual, float* y, int32_t* ids, float* weights, int64_t M,
+                   int64_t top_k, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_moe(moe, M, top_k);
+  if (rc) return rc;
+  if (!x || !y || !ids || !weights) return NSQ_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual) |
+       reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights) |
+       reinterpret_cast<uintptr_t>(w_router) | reinterpret_cast<uintptr_t>(sel_bias)) & 3)
+    return NSQ_ERR_ALIGN;
+  const int64_t E = moe->n_expert, D = moe->n_embd, F = moe->n_ff;
+  const MoeSpace s = moe_space(E, D, F, M, top_k);
+  if (!workspace || workspace_bytes < s.total) return NSQ_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return NSQ_ERR_ALIGN;
+  int num_sms = 0;
+  if ((rc = device_check(&num_sms))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  double* logits = reinterpret_cast<double*>(ws + s.logits);
+  if ((rc = launch_prep(x, M, D, qmm_order(moe->type_in, moe->layout_in), ws + s.recs_x, w_router, (int)E, logits, st)))
+    return rc;
+  QmmParams p{};
+  p.M = (int)M;
+  p.top_k = (int)top_k;
+  p.TS = (int)(M < kQmmMaxTok ? M : kQmmMaxTok);
+  p.E = (int)E;
+  p.score = w_router ? score : -1;
+  p.logits = logits;
+  p.sel_bias = sel_bias;
+  p.scale = scale;
+  p.ids = ids;
+  p.wts = weights;
+  p.groups = reinterpret_cast<QmmGroup*>(ws + s.groups);
+  p.plist = reinterpret_cast<int32_t*>(ws + s.plist);
+  p.pwts = reinterpret_cast<float*>(ws + s.pwts);
+  p.ngroups = reinterpret_cast<int32_t*>(ws + s.ngroups);
+  p.act = moe->act;
+  p.dtype = NSQ_OUT_F32;
+  p.h = reinterpret_cast<float*>(ws + s.h);
+  const int64_t P = M * top_k;
+
+  p.mode = kQmmUp;
+  p.YC = p.TS;
+  p.n = F;
+  p.K = D;
+  p.nsb = (int)units_of(D);
+  p.nblk = (int)(D / 32);
+  p.rb = D / nsq_block_weights(moe->type_in) * nsq_block_bytes(moe->type_in);
+  p.w0 = static_cast<const uint8_t*>(moe->w_gate);
+  p.w1 = static_cast<const uint8_t*>(moe->w_up);
+  p.wbytes = E * F * p.rb;
+  p.recs = ws + s.recs_x;
+  if ((rc = run_qmm(p, moe->type_in, moe->layout_in, P, st, num_sms))) return rc;
+
+  if ((rc = launch_prep(static_cast<const float*>(p.h), P, F, qmm_order(moe->type_down, moe->layout_down), ws + s.recs_h,
+                        nullptr, 0, nullptr, st)))
+    return rc;
+
+  p.mode = kQmmDown;
+  p.YC = p.M;
+  p.n = D;
+  p.K = F;
+  p.nsb = (int)units_of(F);
+  p.nblk = (int)(F / 32);
+  p.rb = F / nsq_block_weights(moe->type_down) * nsq_block_bytes(moe->type_down);
+  p.w0 = static_cast<const uint8_t*>(moe->w_down);
+  p.w1 = nullptr;
+  p.wbytes = E * D * p.rb;
+  p.recs = ws + s.recs_h;
+  p.residual = residual;
+  p.y = y;
+  return run_qmm(p, moe->type_down, moe->layout_down, P, st, num_sms);
+}
+
+}  // namespace nsq
+
+using namespace nsq;
+
+extern "C" {
+
+size_t nsq_linear_workspace_size(int64_t M, int64_t K) {
+  if (M < 1 || M > NSQ_GEMV_MAX_M || K < 1) return 0;
+  return (size_t)(M * units_of(K)) * kQmmRec;
+}
+
+int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, const float* bias, int act,
+               const void* residual, void* y, int dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  int rc = check_weights(w, ggml_type, q6k_layout, K);
+  if (rc) return rc;
+  if (!act_ok(act) || (dtype != NSQ_OUT_F32 && dtype != NSQ_OUT_BF16)) return NSQ_ERR_TYPE;
+  if (M < 1 || M > NSQ_GEMV_MAX_M || N < 1 || N > (int64_t)1 << 24 || K > (int64_t)1 << 24) return NSQ_ERR_SHAPE;
+  if (!x || !y) return NSQ_ERR_NULL;
+  const uintptr_t mask = dtype == NSQ_OUT_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & mask)
+    return NSQ_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(bias) & 3) return NSQ_ERR_ALIGN;
+  if (!workspace || workspace_bytes < nsq_linear_workspace_size(M, K)) return NSQ_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return NSQ_ERR_ALIGN;
+  int num_sms = 0;
+  if ((rc = device_check(&num_sms))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* recs = static_cast<uint8_t*>(workspace);
+  const int order = qmm_order(ggml_type, q6k_layout);
+  rc = dtype == NSQ_OUT_F32
+           ? launch_prep(static_cast<const float*>(x), M, K, order, recs, nullptr, 0, nullptr, st)
+           : launch_prep(static_cast<const __nv_bfloat16*>(x), M, K, order, recs, nullptr, 0, nullptr, st);
+  if (rc) return rc;
+  QmmParams p{};
+  p.mode = kQmmLinear;
+  p.M = p.TS = p.YC = (int)M;
+  p.top_k = 1;
+  p.act = act;
+  p.dtype = dtype;
+  p.n = N;
+  p.K = K;
+  p.nsb = (int)units_of(K);
+  p.nblk = (int)(K / 32);
+  p.rb = K / nsq_block_weights(ggml_type) * nsq_block_bytes(ggml_type);
+  p.w0 = static_cast<const uint8_t*>(w);
+  p.wbytes = N * p.rb;
+  p.recs = recs;
+  p.bias = bias;
+  p.residual = residual;
+  p.y = y;
+  return run_qmm(p, ggml_type, q6k_layout, 1, st, num_sms);
+}
+
+size_t nsq_moe_workspace_size(const nsq_moe* moe, int64_t M, int64_t top_k) {
+  if (!moe || moe->n_expert < 1 || moe->n_embd < 1 || moe->n_ff < 1 || M < 1 || M > NSQ_MOE_MAX_TOKENS || top_k < 1 ||
+      top_k > NSQ_MOE_MAX_TOP_K)
+    return 0;
+  return moe_space(moe->n_expert, moe->n_embd, moe->n_ff, M, top_k).total;
+}
+
+int nsq_moe_ffn(const nsq_moe* moe, const float* x, const int32_t* ids, const float* weights, const float* residual,
+                float* y, int64_t M, int64_t top_k, void* workspace, size_t workspace_bytes, void* stream) {
+  return run_moe(moe, nullptr, 0, nullptr, 1.0f, x, residual, y, const_cast<int32_t*>(ids), const_cast<float*>(weights),
+                 M, top_k, workspace, workspace_bytes, stream);
+}
+
+int nsq_moe_layer(const nsq_moe* moe, const float* w_router, int score, const float* sel_bias, float scale,
+                  const float* x, const float* residual, float* y, int32_t* ids, float* weights, int64_t M,
+                  int64_t top_k, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!w_router) return NSQ_ERR_NULL;
+  if (score < NSQ_SCORE_SOFTMAX || score > NSQ_SCORE_SIGMOID_NORM) return NSQ_ERR_TYPE;
+  return run_moe(moe, w_router, score, sel_bias, scale, x, residual, y, ids, weights, M, top_k, workspace,
+                 workspace_bytes, stream);
+}
+
+}  // extern "C"

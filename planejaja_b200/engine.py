@@ -11,6 +11,11 @@
                                    src/operator_registry.rs:43-49, 246-259)
   dequant(w, t, n)              -> f32 / bf16 weights (DequantDispatcher::dequantize,
                                    crates/nodestor-inference/src/dequant/mod.rs:142-191)
+  linear(x, w, t, n, k, ...)    -> y = act(x . W^T + bias) + residual, the
+                                   matmul, add and activation calls of a
+                                   projection (transformer.rs:241-321) as one
+  moe_layer / moe_ffn           -> a mixture-of-experts feed-forward layer over
+                                   GGUF experts, with or without its router
   zipgemm(w, x, m, k, n)        -> y = x . W^T from an NSZ (TCA-TBE) tensor,
                                    decompressed in registers (lib.rs:124-151)
   nsz_decode(w)                 -> the NSZ tensor's original weights, bit-exact
@@ -48,6 +53,38 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class MoeExperts:
+    """The experts of a mixture-of-experts layer: three GGUF tensors on the
+    device, as they lie in the file (ffn_gate_exps and ffn_up_exps
+    [n_expert x n_ff rows of n_embd], ffn_down_exps [n_expert x n_embd rows of
+    n_ff])."""
+
+    def __init__(self, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, n_expert: int, n_embd: int,
+                 n_ff: int, type_in: int, type_down: int, layout_in: int = Q6K_GGML, layout_down: int = Q6K_GGML,
+                 act: str = "silu"):
+        for name, w, t, n, k in (("w_gate", w_gate, type_in, n_ff, n_embd), ("w_up", w_up, type_in, n_ff, n_embd),
+                                 ("w_down", w_down, type_down, n_embd, n_ff)):
+            if t not in FORMATS:
+                raise NsqError(_lib.ERR_TYPE, f"MoeExperts: {name} has ggml type {t}")
+            if min(n_expert, n, k) < 1 or k % FORMATS[t].block_weights:
+                raise NsqError(_lib.ERR_SHAPE, f"MoeExperts: {name} [{n_expert} x {n} x {k}]")
+            _check_bytes(w, n_expert * FORMATS[t].tensor_bytes(n, k), f"MoeExperts: {name}")
+        if act not in _lib.ACTS:
+            raise NsqError(_lib.ERR_TYPE, f"MoeExperts: activation {act!r}")
+        self.w_gate, self.w_up, self.w_down = w_gate, w_up, w_down
+        self.n_expert, self.n_embd, self.n_ff = n_expert, n_embd, n_ff
+        self._c = _lib.Moe(_ptr(w_gate), _ptr(w_up), _ptr(w_down), type_in, layout_in, type_down, layout_down,
+                           _lib.ACTS[act], n_expert, n_embd, n_ff)
+        self._ref = ctypes.addressof(self._c)
+
+
+def _check_bytes(w: torch.Tensor, nbytes: int, what: str) -> None:
+    if w.dtype != torch.uint8 or not w.is_cuda or not w.is_contiguous():
+        raise NsqError(_lib.ERR_TYPE, f"{what}: GGUF bytes are a contiguous uint8 CUDA tensor")
+    if w.numel() < nbytes:
+        raise NsqError(_lib.ERR_SHAPE, f"{what}: {w.numel()} bytes, {nbytes} needed")
 
 
 class CudaEngine:
@@ -206,6 +243,120 @@ class CudaEngine:
             return self.gemv(w, ggml_type, x.reshape(m, k).float().contiguous(), n, k, q6k_layout, sync=sync)
         xb = x.reshape(m, k).to(torch.bfloat16).contiguous()
         return self.gemm_bf16(w, ggml_type, xb, n, k, q6k_layout, sync=sync).float()
+
+    # ---- products with an epilogue, and mixture-of-experts layers -----------
+    def _tensor(self, t: Optional[torch.Tensor], numel: int, dtype: torch.dtype, what: str) -> Optional[torch.Tensor]:
+        """`t` as the library reads it: contiguous, of this dtype and size, on the engine's device."""
+        if t is None:
+            return None
+        if t.dtype != dtype or not t.is_cuda:
+            raise NsqError(_lib.ERR_TYPE, f"{what}: a {dtype} CUDA tensor is wanted, not {t.dtype} on {t.device}")
+        if self.device.index is not None and t.device.index != self.device.index:
+            raise NsqError(_lib.ERR_DEVICE, f"{what}: on {t.device}, the engine is on {self.device}")
+        if t.numel() != numel:
+            raise NsqError(_lib.ERR_SHAPE, f"{what}: {t.numel()} elements, not {numel}")
+        return t if t.is_contiguous() else t.contiguous()
+
+    def _out(self, out: Optional[torch.Tensor], shape, dtype: torch.dtype, what: str) -> torch.Tensor:
+        if out is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        if not out.is_contiguous():
+            raise NsqError(_lib.ERR_SHAPE, f"{what}: the output has to be contiguous")
+        return self._tensor(out, shape[0] * shape[1], dtype, what)
+
+    def _call(self, fn, what: str, nbytes: int, workspace: Optional[torch.Tensor], args, sync: bool) -> None:
+        """fn(*args, workspace, bytes, stream) with the engine's device current.  Without a workspace of the
+        caller's, the call takes one from PyTorch's allocator, which keeps it from other streams and graphs."""
+        if workspace is None:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        index = self.device.index
+        if index is None or index == torch.cuda.current_device():
+            rc = fn(*args, workspace.data_ptr(), workspace.numel(), _stream_handle(self.device))
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, workspace.data_ptr(), workspace.numel(), _stream_handle(self.device))
+        if rc:
+            raise NsqError(rc, what)
+        self._sync(sync)
+
+    def linear_workspace(self, m: int, n: int, k: int) -> torch.Tensor:
+        """Workspace of `linear` calls of up to this size; one call at a time may use it."""
+        return torch.empty(self.lib.nsq_linear_workspace_size(m, k) or 16, dtype=torch.uint8, device=self.device)
+
+    def linear(self, x: torch.Tensor, w: torch.Tensor, ggml_type: int, n: int, k: int,
+               bias: Optional[torch.Tensor] = None, act: str = "none", residual: Optional[torch.Tensor] = None,
+               q6k_layout: int = Q6K_GGML, out: Optional[torch.Tensor] = None,
+               workspace: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
+        """y[m, n] = act(x . W^T + bias) + residual in one product (nsq_linear).
+
+        x [m, k], residual and y are f32 (m <= 16) or bf16; bias [n] f32; act one of "none", "silu", "gelu",
+        "gelu_tanh", "relu".  `out` may be `residual`."""
+        if x.dtype not in (torch.float32, torch.bfloat16):
+            raise NsqError(_lib.ERR_TYPE, f"linear: activations are f32 or bf16, not {x.dtype}")
+        if ggml_type not in FORMATS or act not in _lib.ACTS:
+            raise NsqError(_lib.ERR_TYPE, f"linear: ggml type {ggml_type}, activation {act!r}")
+        if k < 1 or n < 1 or x.numel() % k or k % FORMATS[ggml_type].block_weights:
+            raise NsqError(_lib.ERR_SHAPE, f"linear: {x.numel()} activations, n = {n}, k = {k}")
+        m = x.numel() // k
+        _check_bytes(w, FORMATS[ggml_type].tensor_bytes(n, k), "linear: w")
+        x = self._tensor(x, m * k, x.dtype, "linear: x")
+        bias = self._tensor(bias, n, torch.float32, "linear: bias")
+        residual = self._tensor(residual, m * n, x.dtype, "linear: residual")
+        y = self._out(out, (m, n), x.dtype, "linear: out")
+        self._call(self.lib.nsq_linear, "nsq_linear", self.lib.nsq_linear_workspace_size(m, k) or 16, workspace,
+                   (_ptr(w), ggml_type, q6k_layout, _ptr(x), _ptr(bias), _lib.ACTS[act], _ptr(residual), _ptr(y),
+                    _lib.OUT_F32 if x.dtype == torch.float32 else _lib.OUT_BF16, m, n, k), sync)
+        return y
+
+    def moe_workspace(self, moe: MoeExperts, m: int, top_k: int) -> torch.Tensor:
+        """Workspace of `moe_ffn` / `moe_layer` calls of this size; one call at a time may use it."""
+        return torch.empty(self.lib.nsq_moe_workspace_size(moe._ref, m, top_k) or 16, dtype=torch.uint8,
+                           device=self.device)
+
+    def moe_ffn(self, moe: MoeExperts, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
+                residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                workspace: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
+        """y[m] = residual[m] + sum_j weights[m, j] * expert ids[m, j] of x[m] (nsq_moe_ffn).
+
+        x [m, n_embd] f32; ids [m, top_k] int32, -1 for an unused slot; weights [m, top_k] f32.  `out` may be
+        `residual`."""
+        if ids.dim() != 2:
+            raise NsqError(_lib.ERR_SHAPE, "moe_ffn: ids are [tokens, top_k]")
+        m, top_k = ids.shape
+        x = self._tensor(x, m * moe.n_embd, torch.float32, "moe_ffn: x")
+        ids = self._tensor(ids, m * top_k, torch.int32, "moe_ffn: ids")
+        weights = self._tensor(weights, m * top_k, torch.float32, "moe_ffn: weights")
+        residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_ffn: residual")
+        y = self._out(out, (m, moe.n_embd), torch.float32, "moe_ffn: out")
+        self._call(self.lib.nsq_moe_ffn, "nsq_moe_ffn", self.lib.nsq_moe_workspace_size(moe._ref, m, top_k) or 16,
+                   workspace, (moe._ref, _ptr(x), _ptr(ids), _ptr(weights), _ptr(residual), _ptr(y), m, top_k), sync)
+        return y
+
+    def moe_layer(self, moe: MoeExperts, w_router: torch.Tensor, x: torch.Tensor, top_k: int,
+                  score: str = "softmax_norm", sel_bias: Optional[torch.Tensor] = None, scale: float = 1.0,
+                  residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None, sync: bool = True):
+        """Router, picks and experts (nsq_moe_layer): (y [m, n_embd], ids [m, top_k] int32, weights [m, top_k]).
+
+        w_router [n_expert, n_embd] f32 (GGUF ffn_gate_inp); score one of "softmax", "softmax_norm",
+        "sigmoid_norm"; sel_bias [n_expert] enters the choice alone."""
+        if score not in _lib.SCORES:
+            raise NsqError(_lib.ERR_TYPE, f"moe_layer: score {score!r}")
+        if x.numel() % moe.n_embd:
+            raise NsqError(_lib.ERR_SHAPE, f"moe_layer: {x.numel()} activations, n_embd = {moe.n_embd}")
+        m = x.numel() // moe.n_embd
+        x = self._tensor(x, m * moe.n_embd, torch.float32, "moe_layer: x")
+        w_router = self._tensor(w_router, moe.n_expert * moe.n_embd, torch.float32, "moe_layer: w_router")
+        sel_bias = self._tensor(sel_bias, moe.n_expert, torch.float32, "moe_layer: sel_bias")
+        residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_layer: residual")
+        y = self._out(out, (m, moe.n_embd), torch.float32, "moe_layer: out")
+        ids = torch.empty((m, max(top_k, 0)), dtype=torch.int32, device=self.device)
+        weights = torch.empty((m, max(top_k, 0)), dtype=torch.float32, device=self.device)
+        self._call(self.lib.nsq_moe_layer, "nsq_moe_layer",
+                   self.lib.nsq_moe_workspace_size(moe._ref, m, top_k) or 16, workspace,
+                   (moe._ref, _ptr(w_router), _lib.SCORES[score], _ptr(sel_bias), scale, _ptr(x), _ptr(residual),
+                    _ptr(y), _ptr(ids), _ptr(weights), m, top_k), sync)
+        return y, ids, weights
 
     # ---- NSZ (TCA-TBE) tensors and ZipGEMM --------------------------------
     def nsz_upload(self, stream, num_weights: int, dtype: int = _lib.NSZ_FP32, shape=()) -> "NszTensor":
