@@ -1,17 +1,22 @@
 // qmm.cu -- the linear operator (nsq_linear) and the mixture-of-experts layer
 // (nsq_moe_ffn, nsq_moe_layer): preparation kernel, launch planning, checks.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "qmm.cuh"
 
 namespace nsq {
 
-int launch_qmm_q4k(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
-int launch_qmm_q5k(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
-int launch_qmm_q6k(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
-int launch_qmm_q40(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
-int launch_qmm_q80(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q4k(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q5k(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q6k(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q40(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st);
+int launch_qmm_q80(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st);
 int check_weights(const void* w, int type, int layout, int64_t K);
 int device_check(int* num_sms);
 
+constexpr int kPrepThreads = 32 * kQmmWarps;
 constexpr int kRouteTok = 8;  // tokens of one CTA's logits
 
 // Activation records of rows x nsb units (one warp each) and, in the first
@@ -21,7 +26,7 @@ constexpr int kRouteTok = 8;  // tokens of one CTA's logits
 // SM and cycle; 16 tokens, 128 experts and K = 2048 take under half a
 // microsecond of them.
 template <typename T>
-__global__ void __launch_bounds__(kQmmThreads) qmm_prep_kernel(const T* __restrict__ x, int rows, int64_t K, int nsb,
+__global__ void __launch_bounds__(kPrepThreads) qmm_prep_kernel(const T* __restrict__ x, int rows, int64_t K, int nsb,
                                                                int order, uint8_t* __restrict__ recs,
                                                                const float* __restrict__ router, int E,
                                                                double* __restrict__ logits, int nlog) {
@@ -36,7 +41,7 @@ __global__ void __launch_bounds__(kQmmThreads) qmm_prep_kernel(const T* __restri
       double acc[kRouteTok] = {};
       const float* w = router + (int64_t)e * K;
       const bool wide = ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(x)) & 15) == 0;  // K % 32 == 0
-      for (int64_t k = 4 * threadIdx.x; k < K; k += 4 * kQmmThreads) {
+      for (int64_t k = 4 * threadIdx.x; k < K; k += 4 * kPrepThreads) {
         float4 a;
         if (wide) {
           a = *reinterpret_cast<const float4*>(w + k);
@@ -90,7 +95,7 @@ static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* 
   const int nlog = router ? E * (int)((rows + kRouteTok - 1) / kRouteTok) : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(nlog + (rows * nsb + kQmmWarps - 1) / kQmmWarps));
-  cfg.blockDim = dim3(kQmmThreads);
+  cfg.blockDim = dim3(kPrepThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -104,52 +109,101 @@ static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* 
              : NSQ_ERR_CUDA;
 }
 
-static int qmm_pitch(int type) {
+struct QmmShape {
+  int CB, PA, PG, MT;
+};
+template <int TYPE>
+static constexpr QmmShape shape_t() {
+  return {QmmFmt<TYPE>::CB, QmmFmt<TYPE>::PA, QmmFmt<TYPE>::PG, QmmFmt<TYPE>::MT};
+}
+static QmmShape qmm_shape(int type) {
   switch (type) {
-    case NSQ_TYPE_Q4_K: return QmmFmt<NSQ_TYPE_Q4_K>::PITCH;
-    case NSQ_TYPE_Q5_K: return QmmFmt<NSQ_TYPE_Q5_K>::PITCH;
-    case NSQ_TYPE_Q6_K: return QmmFmt<NSQ_TYPE_Q6_K>::PITCH;
-    case NSQ_TYPE_Q4_0: return QmmFmt<NSQ_TYPE_Q4_0>::PITCH;
-    default: return QmmFmt<NSQ_TYPE_Q8_0>::PITCH;
+    case NSQ_TYPE_Q4_K: return shape_t<NSQ_TYPE_Q4_K>();
+    case NSQ_TYPE_Q5_K: return shape_t<NSQ_TYPE_Q5_K>();
+    case NSQ_TYPE_Q6_K: return shape_t<NSQ_TYPE_Q6_K>();
+    case NSQ_TYPE_Q4_0: return shape_t<NSQ_TYPE_Q4_0>();
+    default: return shape_t<NSQ_TYPE_Q8_0>();
   }
+}
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// Rows of weights as [rows x rb / 2] 16-bit elements, boxes of box_rows x pitch bytes.
+static bool encode_rows(CUtensorMap* map, const uint8_t* w, int64_t rows, int64_t rb, int box_rows, int pitch) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)(rb / 2), (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)rb};
+  cuuint32_t box[2] = {(cuuint32_t)(pitch / 2), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<uint8_t*>(w), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Plans and launches one product.  groups: the most groups there can be.
 static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream_t st, int num_sms) {
+  const QmmShape f = qmm_shape(type);
   // columns of K per CTA: the records of a unit are read by the RW = 8 / KW
   // warps that share it, so more tokens want more rows per unit
-  int KW = p.TS <= 1 ? 8 : p.TS <= 4 ? 4 : p.TS <= 8 ? 2 : 1;
+  int KW = p.TS <= 2 ? 8 : p.TS <= 4 ? 4 : p.TS <= 8 ? 2 : 1;
   const int64_t most_units = p.mode == kQmmDown ? groups * p.nsb : p.nsb;
   while (KW > 1 && KW / 2 >= most_units) KW /= 2;
   p.KW = KW;
   p.RW = kQmmWarps / KW;
-  const int64_t tile_rows = (p.mode == kQmmUp ? 8 : 16) * p.RW;
+  const int64_t tile_rows = (p.mode == kQmmUp ? 8 : 16) * f.MT * p.RW;
   const int64_t tiles = (p.n + tile_rows - 1) / tile_rows;
   const int64_t slots = 2 * (int64_t)num_sms;
   p.split = 1;
   if (p.mode != kQmmUp) {
     // a K split over a cluster while the tiles leave half of the CTA slots
-    // empty and every CTA keeps a step of units
+    // empty and every CTA keeps a unit per column
     while (p.split < 8 && tiles * p.split * 2 <= slots && most_units >= (int64_t)p.split * 2 * KW) p.split *= 2;
   }
-  const int pitch = qmm_pitch(type);
+  // TMA boxes where every row starts 16-byte aligned (experts and tensors then do too)
+  alignas(64) CUtensorMap maps[2] = {};
+  const int64_t rows = p.wbytes / p.rb;
+  p.rows_aligned = p.rb % 16 == 0 && rows <= 0x7FFFFFFF;
+  if (p.rows_aligned) {
+    const int box_rows = p.RW * f.MT * (p.mode == kQmmUp ? 8 : 16);
+    if (!encode_rows(&maps[0], p.w0, rows, p.rb, box_rows, f.PA)) p.rows_aligned = 0;
+    if (p.mode == kQmmUp && !encode_rows(&maps[1], p.w1, rows, p.rb, box_rows, f.PA)) p.rows_aligned = 0;
+  }
   const int P = p.mode == kQmmLinear ? 0 : p.M * p.top_k;
-  const size_t fixed = (size_t)kQmmWarps * p.YC * 16 * 4 + (p.split > 1 ? (size_t)p.YC * 16 * p.RW * 4 : 0) + qmm_lists_bytes(P);
-  const size_t stage = qmm_stage_bytes(pitch, p.KW, p.TS);
-  p.stages = 4;
-  while (p.stages > 2 && fixed + p.stages * stage > (size_t)kQmmSmemHalf) --p.stages;
-  size_t smem = fixed + p.stages * stage;
-  if (smem < (size_t)P * 8) smem = (size_t)P * 8;
-  if (smem > (size_t)kQmmSmemMax) return NSQ_ERR_SHAPE;
+  const size_t slot = qmm_slot_bytes(p.RW * f.MT, p.rows_aligned ? f.PA : f.PG, p.TS);
+  const size_t ys = (size_t)kQmmWarps * p.YC * 16 * f.MT * 4;
+  const bool in_ring = p.mode != kQmmDown && p.split > 1;
+  // buffers of partial sums: none where one column holds the whole K, two so
+  // that a task's are joined while the next one runs
+  p.PB = p.mode != kQmmDown && p.split == 1 && KW == 1 ? 0 : p.split > 1 ? 1 : 2;
+  const size_t fixed = kQmmCtl + kQmmRec + qmm_lists_bytes(P);
+  if (p.mode == kQmmDown && p.PB == 2 && fixed + 2 * ys + 2 * p.KW * slot > (size_t)kQmmSmemHalf) p.PB = 1;
+  const size_t sums = in_ring ? 0 : p.PB * ys;
+  p.stages = kQmmMaxStages;
+  while (p.stages > 2 && fixed + sums + p.stages * p.KW * slot > (size_t)kQmmSmemHalf) --p.stages;
+  const size_t ring = p.stages * p.KW * slot;
+  if (in_ring && ys > ring) return NSQ_ERR_SHAPE;
+  const size_t smem = fixed + sums + ring;
+  if (smem > (size_t)kQmmSmemMax || ring < (size_t)P * 8) return NSQ_ERR_SHAPE;
   const int64_t tasks = tiles * (p.mode == kQmmUp ? groups : 1);
-  int64_t grid = (tasks < slots / p.split ? tasks : slots / p.split) * p.split;
-  if (grid < p.split) grid = p.split;
+  const int64_t grid = (p.split > 1 || tasks < slots ? tasks : slots) * p.split;
   switch (type) {
-    case NSQ_TYPE_Q4_K: return launch_qmm_q4k(layout, p, (int)grid, smem, st);
-    case NSQ_TYPE_Q5_K: return launch_qmm_q5k(layout, p, (int)grid, smem, st);
-    case NSQ_TYPE_Q6_K: return launch_qmm_q6k(layout, p, (int)grid, smem, st);
-    case NSQ_TYPE_Q4_0: return launch_qmm_q40(layout, p, (int)grid, smem, st);
-    case NSQ_TYPE_Q8_0: return launch_qmm_q80(layout, p, (int)grid, smem, st);
+    case NSQ_TYPE_Q4_K: return launch_qmm_q4k(layout, p, maps, (int)grid, smem, st);
+    case NSQ_TYPE_Q5_K: return launch_qmm_q5k(layout, p, maps, (int)grid, smem, st);
+    case NSQ_TYPE_Q6_K: return launch_qmm_q6k(layout, p, maps, (int)grid, smem, st);
+    case NSQ_TYPE_Q4_0: return launch_qmm_q40(layout, p, maps, (int)grid, smem, st);
+    case NSQ_TYPE_Q8_0: return launch_qmm_q80(layout, p, maps, (int)grid, smem, st);
     default: return NSQ_ERR_TYPE;
   }
 }

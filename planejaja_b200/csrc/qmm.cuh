@@ -25,13 +25,20 @@
 // slots per weight (Q4_K), half of an SM's issue rate at HBM speed, so the
 // matrix instructions leave room for 4 tokens at the price of one.
 //
-// Layout.  A CTA is 8 warps = RW row tiles of 16 weight rows x KW columns of
-// 256 weights ("units").  Per step every warp computes one unit; raw weight
-// bytes and the prepared activation records of the step arrive by cp.async in
-// a ring of shared-memory stages.  Partial sums of the KW warps meet in
-// shared memory, those of a K split over a cluster through distributed
-// shared memory, always in the same order.
+// Layout.  A CTA is 8 consumer warps = RW row tiles of 16 MT weight rows x KW
+// columns, and one producer warp.  A task is a tile of 16 MT RW rows; its
+// units of 256 weights of K are dealt to the columns in turn.  A column has
+// its own ring of shared-memory slots (the weight bytes of its RW tiles and
+// the activation records of the unit) behind full / empty mbarriers, filled by
+// TMA: one 2-D box of rows where rows start 16-byte aligned, else one bulk
+// copy per row.  The partial sums of the KW columns meet in shared memory,
+// those of a K split over a cluster through distributed shared memory, always
+// in the same order.  Every wait is bounded.
 #pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
 
 #include "nsq_common.cuh"
 
@@ -49,10 +56,12 @@ namespace nsq {
 // Which k a place holds goes by the format of the weights (QmmOrder).
 constexpr int kQmmRec = 1104;
 constexpr int kQmmWarps = 8;
-constexpr int kQmmThreads = 32 * kQmmWarps;
+constexpr int kQmmThreads = 32 * (kQmmWarps + 1);  // and the producer warp
+constexpr int kQmmMaxStages = 4;
+constexpr int kQmmCtl = 1024;  // barriers and counters at the start of the shared memory
 constexpr int kQmmMaxTok = 16;  // tokens of a group
-constexpr int kQmmSmemMax = 227 * 1024 - 64;   // dynamic shared memory of a CTA alone on its SM
-constexpr int kQmmSmemHalf = 113 * 1024 - 64;  // of one of two CTAs
+constexpr int kQmmSmemMax = 227 * 1024 - 1024;   // dynamic shared memory of a CTA alone on its SM
+constexpr int kQmmSmemHalf = 113 * 1024 - 1024;  // of one of two CTAs
 
 enum QmmOrder : int { kOrdK45 = 0, kOrd32 = 1, kOrdQ6 = 2 };
 
@@ -166,6 +175,8 @@ struct QmmParams {
   int act, dtype;
   int nsb;       // units of a weight row: ceil(K / 256)
   int nblk;      // K / 32
+  int rows_aligned;  // every row starts 16-byte aligned: TMA boxes
+  int PB;            // buffers of partial sums (0: outputs straight from registers)
   int64_t n, K, rb;          // rows of one expert, K, bytes of a row
   const uint8_t* w0;         // weights (kQmmUp: gate)
   const uint8_t* w1;         // kQmmUp: up
@@ -193,24 +204,14 @@ struct QmmParams {
 __device__ __forceinline__ void qmm_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void qmm_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ void qmm_cp16(uint32_t dst, const void* src, int bytes, uint64_t pol) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
-               "l"(pol)
-               : "memory");
+__device__ __forceinline__ void qmm_tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar, uint64_t pol) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, "
+      "%3}], [%4], %5;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar)), "l"(pol)
+      : "memory");
 }
-__device__ __forceinline__ void qmm_cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void qmm_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// The oldest of the `stages` - 1 groups in flight has landed.
-__device__ __forceinline__ void qmm_wait(int stages) {
-  if (stages == 2) {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-  } else if (stages == 3) {
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-  } else {
-    asm volatile("cp.async.wait_group 2;" ::: "memory");
-  }
+__device__ __forceinline__ void qmm_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void qmm_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -237,35 +238,77 @@ __device__ __forceinline__ float qmm_act(float v, int act) {
 }
 
 // ---------------------------------------------------------------------------
-// Per format: bytes and weights of a unit of one row, its copies of 16 bytes
-// and the pitch of its shared-memory row.  Rows of Q4_0, Q8_0 and Q6_K start
-// at any even address, so their copies carry up to 14 bytes before the unit.
-// The pitches put the reads of 8 rows x 4 lanes on distinct banks.
+// Per format: bytes of a unit of one row (CB), row tiles per warp (MT) and the
+// pitches of a slot's rows: with 16-byte aligned rows (PA, the TMA box) and
+// without (PG: the copies then carry up to 14 bytes before and 15 after the
+// unit).  The pitches put the reads of 8 rows x 4 lanes on distinct banks.
+// Two row tiles share their B operands and bookkeeping; the wider formats
+// have one, for the depth of the ring.
 template <int TYPE> struct QmmFmt;
-template <> struct QmmFmt<NSQ_TYPE_Q4_K> { static constexpr int CB = 144, NCH = 9, PITCH = 144; static constexpr bool aligned = true; };
-template <> struct QmmFmt<NSQ_TYPE_Q5_K> { static constexpr int CB = 176, NCH = 11, PITCH = 176; static constexpr bool aligned = true; };
-template <> struct QmmFmt<NSQ_TYPE_Q6_K> { static constexpr int CB = 210, NCH = 14, PITCH = 240; static constexpr bool aligned = false; };
-template <> struct QmmFmt<NSQ_TYPE_Q4_0> { static constexpr int CB = 144, NCH = 10, PITCH = 176; static constexpr bool aligned = false; };
-template <> struct QmmFmt<NSQ_TYPE_Q8_0> { static constexpr int CB = 272, NCH = 18, PITCH = 304; static constexpr bool aligned = false; };
+template <> struct QmmFmt<NSQ_TYPE_Q4_K> { static constexpr int CB = 144, PA = 144, PG = 144, MT = 2; };
+template <> struct QmmFmt<NSQ_TYPE_Q5_K> { static constexpr int CB = 176, PA = 176, PG = 176, MT = 2; };
+template <> struct QmmFmt<NSQ_TYPE_Q6_K> { static constexpr int CB = 210, PA = 240, PG = 240, MT = 1; };
+template <> struct QmmFmt<NSQ_TYPE_Q4_0> { static constexpr int CB = 144, PA = 144, PG = 176, MT = 2; };
+template <> struct QmmFmt<NSQ_TYPE_Q8_0> { static constexpr int CB = 272, PA = 272, PG = 304, MT = 1; };
 
-// B operands of MMA steps 2i and 2i+1 for n-tile j (0 for absent tokens).
+// All shared memory is addressed as an offset from this array, so that loads
+// stay shared-memory loads with immediate offsets.  TMA boxes land on 128-byte
+// boundaries: slots are multiples of 128 bytes from its start.  Static shared
+// memory would come before it and leave it only 16-byte aligned, whatever is
+// declared here, so the kernel has none: the barriers take the first bytes.
+extern __shared__ __align__(128) uint8_t qmm_smem[];
+template <typename T>
+__device__ __forceinline__ T qmm_lds(uint32_t off) {
+  return *reinterpret_cast<const T*>(qmm_smem + off);
+}
+
+// Where this lane reads the B operands of NT n-tiles: its token and part in
+// each (a record of zeros for absent tokens).
+template <int NT>
 struct QmmB {
-  const uint8_t* rec;  // this lane's token and part of n-tile 0
-  int c, flip, count, tok;
+  uint32_t even[NT], odd[NT];  // units 4i + c of even and odd i, less 64 i
+  uint32_t t[NT];              // the T sums
+  __device__ __forceinline__ QmmB(uint32_t recs, uint32_t zeros, int count, int lr, int c) {
+    const int tok = lr >> 1, flip = (lr & 1) * 64;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const uint32_t r = 4 * j + tok < count ? recs + (4 * j + tok) * kQmmRec : zeros;
+      even[j] = r + (flip << 3) + 16 * c + flip;  // lo parts at + 512, units ^ 4
+      odd[j] = r + (flip << 3) + 16 * c - flip;
+      t[j] = r + 1024 + (flip >> 1) + 8 * c;
+    }
+  }
   __device__ __forceinline__ uint4 steps(int j, int i) const {
-    uint4 b = make_uint4(0, 0, 0, 0);
-    if (4 * j + tok < count)
-      b = *reinterpret_cast<const uint4*>(rec + 4 * j * kQmmRec + ((((4 * i + c) ^ flip)) << 4));
-    return b;
+    return qmm_lds<uint4>(((i & 1) ? odd[j] : even[j]) + 64 * i);
   }
 };
 
-// 32-bit word at an even shared-memory address.
-__device__ __forceinline__ uint32_t qmm_ld2(const uint8_t* p) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-  const uint32_t* b = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
-  return __funnelshift_r(b[0], b[1], (uint32_t)(a & 3) * 8);
+// A weight row whose first byte lies at an even offset: words at even
+// offsets as two aligned words and a funnel shift.
+struct QmmRow {
+  uint32_t at, a0, a2, s0, s2;
+  __device__ __forceinline__ explicit QmmRow(uint32_t off)
+      : at(off), a0(off & ~3u), a2((off + 2) & ~3u), s0((off & 2) * 8), s2(((off + 2) & 2) * 8) {}
+  template <int OFF>
+  __device__ __forceinline__ uint32_t word(uint32_t more) const {  // more: a multiple of 4
+    if constexpr (OFF % 4 == 0) {
+      return __funnelshift_r(qmm_lds<uint32_t>(a0 + more + OFF), qmm_lds<uint32_t>(a0 + more + OFF + 4), s0);
+    } else {
+      return __funnelshift_r(qmm_lds<uint32_t>(a2 + more + OFF - 2), qmm_lds<uint32_t>(a2 + more + OFF + 2), s2);
+    }
+  }
+  __device__ __forceinline__ uint32_t u16(int off) const { return qmm_lds<uint16_t>(at + off); }
+  __device__ __forceinline__ uint32_t u8(int off) const { return qmm_lds<uint8_t>(at + off); }
+};
+// Calls f(integral_constant 0), ..., f(N - 1), so that offsets are constants.
+template <int N, int I = 0, typename Fn>
+__device__ __forceinline__ void qmm_for(Fn&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    qmm_for<N, I + 1>(f);
+  }
 }
+
 // Byte b (a runtime number) of w as two equal fp16: 1024 + byte.
 __device__ __forceinline__ __half2 qmm_dup1024(uint32_t w, int b) {
   return qmm_u2h(__byte_perm(w, 0x64646464u, 0x4040u | (uint32_t)(b | (b << 8))));
@@ -279,171 +322,182 @@ __device__ __forceinline__ uint32_t qmm_off16(uint32_t v, float off) {
   return qmm_h2u(__hfma2(qmm_u2h(v), __float2half2_rn(0.0625f), __float2half2_rn(off)));
 }
 
-// Adds one unit's products to u[j][row half] (without the token scale s).
-// r0, r1: this lane's weight rows lane / 4 and lane / 4 + 8; T: the lane's
-// token sums of n-tile 0; nv: valid 32-weight blocks (Q4_0, Q8_0).
-template <int TYPE, int LAYOUT, int NT>
-__device__ __forceinline__ void qmm_unit(const uint8_t* r0, const uint8_t* r1, const QmmB& B, int nv, float (&u)[NT][2]) {
-  const int c = B.c;
-  const uint8_t* rows[2] = {r0, r1};
-
+// One unit's products u[tile][j][row half], without the token scale s.  o: the
+// shared-memory offsets of this lane's weight rows lane / 4 and lane / 4 + 8
+// of each row tile; c = lane % 4; nv: valid 32-weight blocks (Q4_0, Q8_0).
+template <int TYPE, int LAYOUT, int MT, int NT>
+__device__ __forceinline__ void qmm_unit(const uint32_t (&o)[MT][2], int c, const QmmB<NT>& B, int nv,
+                                         float (&u)[MT][NT][2]) {
   if constexpr (TYPE == NSQ_TYPE_Q4_K || TYPE == NSQ_TYPE_Q5_K) {
-    __half2 sa[2], sb[2];  // scales of sub-blocks 2c and 2c+1, times 2^10 and 2^6
-    uint32_t ma[2], mb[2];
-    float d[2], dm[2];
+    __half2 sa[MT][2], sb[MT][2];  // scales of sub-blocks 2c and 2c+1, times 2^10 and 2^6
+    const __half2 k1024 = __float2half2_rn(1024.0f), k64 = __float2half2_rn(64.0f);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint4 h = *reinterpret_cast<const uint4*>(rows[r]);
-      d[r] = h2f((uint16_t)(h.x & 0xFFFF));
-      dm[r] = h2f((uint16_t)(h.x >> 16));
-      const uint32_t s_lo = h.y & 0x3F3F3F3Fu, m_lo = h.z & 0x3F3F3F3Fu;
-      const uint32_t s_hi = (h.w & 0x0F0F0F0Fu) | ((h.y >> 2) & 0x30303030u);
-      const uint32_t m_hi = ((h.w >> 4) & 0x0F0F0F0Fu) | ((h.z >> 2) & 0x30303030u);
-      const uint32_t s = c < 2 ? s_lo : s_hi;
-      const __half2 k1024 = __float2half2_rn(1024.0f), k64 = __float2half2_rn(64.0f);
-      sa[r] = __hmul2(__hsub2(qmm_dup1024(s, (2 * c) & 3), k1024), k1024);
-      sb[r] = __hmul2(__hsub2(qmm_dup1024(s, (2 * c + 1) & 3), k1024), k64);
-      ma[r] = qmm_h2u(__hsub2(qmm_dup1024(m_lo, c), k1024));
-      mb[r] = qmm_h2u(__hsub2(qmm_dup1024(m_hi, c), k1024));
-    }
-    constexpr int QS = TYPE == NSQ_TYPE_Q4_K ? 16 : 48;
-    uint32_t q[2][8];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint4 lo = *reinterpret_cast<const uint4*>(rows[r] + QS + 32 * c);
-      const uint4 hi = *reinterpret_cast<const uint4*>(rows[r] + QS + 32 * c + 16);
-      q[r][0] = lo.x; q[r][1] = lo.y; q[r][2] = lo.z; q[r][3] = lo.w;
-      q[r][4] = hi.x; q[r][5] = hi.y; q[r][6] = hi.z; q[r][7] = hi.w;
-    }
-    [[maybe_unused]] uint32_t qh[2][8];
-    if constexpr (TYPE == NSQ_TYPE_Q5_K && LAYOUT == NSQ_Q6K_GGML) {
-      // bit 2c (2c+1) of byte l is the fifth bit of weight l of sub-block 2c (2c+1)
+    for (int t = 0; t < MT; ++t) {
+      uint32_t ma[2], mb[2];
+      float dm[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint4 lo = *reinterpret_cast<const uint4*>(rows[r] + 16);
-        const uint4 hi = *reinterpret_cast<const uint4*>(rows[r] + 32);
-        qh[r][0] = lo.x >> (2 * c); qh[r][1] = lo.y >> (2 * c); qh[r][2] = lo.z >> (2 * c); qh[r][3] = lo.w >> (2 * c);
-        qh[r][4] = hi.x >> (2 * c); qh[r][5] = hi.y >> (2 * c); qh[r][6] = hi.z >> (2 * c); qh[r][7] = hi.w >> (2 * c);
-      }
-    } else if constexpr (TYPE == NSQ_TYPE_Q5_K) {
-      // NodeStor: bit l of word 2c (2c+1) of qh
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint2 v = *reinterpret_cast<const uint2*>(rows[r] + 16 + 8 * c);
-        qh[r][0] = v.x;
-        qh[r][1] = v.y;
-      }
-    }
-    float acc[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t a[2][4];  // [row]: sub-block 2c (values 0,2 | 1,3), sub-block 2c+1 (the same)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t w = q[r][i], w8 = w >> 8;
-        uint32_t v0 = w & 0x000F000Fu, v1 = w8 & 0x000F000Fu, v2 = w & 0x00F000F0u, v3 = w8 & 0x00F000F0u;
-        if constexpr (TYPE == NSQ_TYPE_Q5_K && LAYOUT == NSQ_Q6K_GGML) {
-          const uint32_t g = qh[r][i];
-          v0 |= (g << 4) & 0x00100010u;
-          v1 |= (g >> 4) & 0x00100010u;
-          v2 |= (g << 7) & 0x01000100u;
-          v3 |= (g >> 1) & 0x01000100u;
-        } else if constexpr (TYPE == NSQ_TYPE_Q5_K) {
-          const uint32_t g = (qh[r][0] >> (4 * i)) & 15u, f = (qh[r][1] >> (4 * i)) & 15u;
-          v0 |= (g * 0x00040010u) & 0x00100010u;  // bits 0, 2 -> 4, 20
-          v1 |= (g * 0x00020008u) & 0x00100010u;  // bits 1, 3 -> 4, 20
-          v2 |= (f * 0x00400100u) & 0x01000100u;
-          v3 |= (f * 0x00200080u) & 0x01000100u;
-        }
-        a[r][0] = qmm_mul2(v0, sa[r]);
-        a[r][1] = qmm_mul2(v1, sa[r]);
-        a[r][2] = qmm_mul2(v2, sb[r]);
-        a[r][3] = qmm_mul2(v3, sb[r]);
+        const uint4 h = qmm_lds<uint4>(o[t][r]);
+        dm[r] = h2f((uint16_t)(h.x >> 16)) * -32.0f;
+        // 6-bit scales of sub-blocks 2c, 2c+1: bytes of y (c < 2), or of w and y's upper bits
+        const uint32_t s = c < 2 ? h.y & 0x3F3F3F3Fu : (h.w & 0x0F0F0F0Fu) | ((h.y >> 2) & 0x30303030u);
+        const uint32_t m_lo = h.z & 0x3F3F3F3Fu, m_hi = ((h.w >> 4) & 0x0F0F0F0Fu) | ((h.z >> 2) & 0x30303030u);
+        sa[t][r] = __hmul2(__hsub2(qmm_dup1024(s, (2 * c) & 3), k1024), k1024);
+        sb[t][r] = __hmul2(__hsub2(qmm_dup1024(s, (2 * c + 1) & 3), k1024), k64);
+        ma[r] = qmm_h2u(__hsub2(qmm_dup1024(m_lo, c), k1024));
+        mb[r] = qmm_h2u(__hsub2(qmm_dup1024(m_hi, c), k1024));
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        if (j == 0 || 4 * j < B.count) {
-          const uint4 b = B.steps(j, i);
-          qmm_mma(acc[j], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-          qmm_mma(acc[j], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
+        const uint2 b = qmm_lds<uint2>(B.t[j]);
+        float am[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // the mins against T
+        qmm_mma(am, ma[0], ma[1], mb[0], mb[1], b.x, b.y);
+        u[t][j][0] = dm[0] * (am[0] + am[1]);
+        u[t][j][1] = dm[1] * (am[2] + am[3]);
+      }
+    }
+    constexpr int QS = TYPE == NSQ_TYPE_Q4_K ? 16 : 48;
+    [[maybe_unused]] uint2 hn[MT][2];
+    if constexpr (TYPE == NSQ_TYPE_Q5_K && LAYOUT == NSQ_Q6K_NODESTOR) {
+      // bit l of word 2c (2c+1) of qh is the fifth bit of weight l of sub-block 2c (2c+1)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) hn[t][r] = qmm_lds<uint2>(o[t][r] + 16 + 8 * c);
+      }
+    }
+    float acc[MT][NT][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[t][j][0] = acc[t][j][1] = acc[t][j][2] = acc[t][j][3] = 0.0f;
+    }
+#pragma unroll
+    for (int i4 = 0; i4 < 2; ++i4) {
+      uint4 q[MT][2];
+      [[maybe_unused]] uint4 hg[MT][2];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          q[t][r] = qmm_lds<uint4>(o[t][r] + QS + 32 * c + 16 * i4);
+          // ggml: bit 2c (2c+1) of byte l is the fifth bit of weight l of sub-block 2c (2c+1)
+          if constexpr (TYPE == NSQ_TYPE_Q5_K && LAYOUT == NSQ_Q6K_GGML) hg[t][r] = qmm_lds<uint4>(o[t][r] + 16 + 16 * i4);
+        }
+      }
+#pragma unroll
+      for (int ii = 0; ii < 4; ++ii) {
+        const int i = 4 * i4 + ii;
+        uint4 b[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) b[j] = B.steps(j, i);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          uint32_t a[2][4];  // [row]: sub-block 2c (values 0,2 | 1,3), sub-block 2c+1 (the same)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t w = ii == 0 ? q[t][r].x : ii == 1 ? q[t][r].y : ii == 2 ? q[t][r].z : q[t][r].w;
+            const uint32_t w8 = w >> 8;
+            uint32_t v0 = w & 0x000F000Fu, v1 = w8 & 0x000F000Fu, v2 = w & 0x00F000F0u, v3 = w8 & 0x00F000F0u;
+            if constexpr (TYPE == NSQ_TYPE_Q5_K && LAYOUT == NSQ_Q6K_GGML) {
+              const uint32_t g =
+                  (ii == 0 ? hg[t][r].x : ii == 1 ? hg[t][r].y : ii == 2 ? hg[t][r].z : hg[t][r].w) >> (2 * c);
+              v0 |= (g << 4) & 0x00100010u;
+              v1 |= (g >> 4) & 0x00100010u;
+              v2 |= (g << 7) & 0x01000100u;
+              v3 |= (g >> 1) & 0x01000100u;
+            } else if constexpr (TYPE == NSQ_TYPE_Q5_K) {
+              const uint32_t g = (hn[t][r].x >> (4 * i)) & 15u, f = (hn[t][r].y >> (4 * i)) & 15u;
+              v0 |= (g * 0x00040010u) & 0x00100010u;  // bits 0, 2 -> 4, 20
+              v1 |= (g * 0x00020008u) & 0x00100010u;  // bits 1, 3 -> 4, 20
+              v2 |= (f * 0x00400100u) & 0x01000100u;
+              v3 |= (f * 0x00200080u) & 0x01000100u;
+            }
+            a[r][0] = qmm_mul2(v0, sa[t][r]);
+            a[r][1] = qmm_mul2(v1, sa[t][r]);
+            a[r][2] = qmm_mul2(v2, sb[t][r]);
+            a[r][3] = qmm_mul2(v3, sb[t][r]);
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            qmm_mma(acc[t][j], a[0][0], a[1][0], a[0][1], a[1][1], b[j].x, b[j].y);
+            qmm_mma(acc[t][j], a[0][2], a[1][2], a[0][3], a[1][3], b[j].z, b[j].w);
+          }
         }
       }
     }
-    float am[NT][4];  // the mins against T
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      am[j][0] = am[j][1] = am[j][2] = am[j][3] = 0.0f;
-      if (j == 0 || 4 * j < B.count) {
-        uint2 t = make_uint2(0, 0);
-        // rec points at the part's operands (0 or 512): hi T at 1024, lo T at 1056
-        if (4 * j + B.tok < B.count)
-          t = *reinterpret_cast<const uint2*>(B.rec + 4 * j * kQmmRec + (B.flip ? 1056 - 512 : 1024) + 8 * c);
-        qmm_mma(am[j], ma[0], ma[1], mb[0], mb[1], t.x, t.y);
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float d = h2f((uint16_t)qmm_lds<uint16_t>(o[t][r])) * 16384.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) u[t][j][r] += d * (acc[t][j][2 * r] + acc[t][j][2 * r + 1]);
       }
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        u[j][r] = (d[r] * 16384.0f) * (acc[j][2 * r] + acc[j][2 * r + 1]) -
-                  (dm[r] * 32.0f) * (am[j][2 * r] + am[j][2 * r + 1]);
     }
   } else if constexpr (TYPE == NSQ_TYPE_Q4_0 || TYPE == NSQ_TYPE_Q8_0) {
     constexpr int BB = TYPE == NSQ_TYPE_Q4_0 ? 18 : 34;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) u[j][0] = u[j][1] = 0.0f;
+    for (int t = 0; t < MT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t a[2][4];
-      float d[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint8_t* blk = rows[r] + BB * i;
-        d[r] = i < nv ? h2f((uint16_t)ld_u16(blk)) : 0.0f;
-        const uint32_t w = qmm_ld2(blk + 2 + 4 * c);
-        if constexpr (TYPE == NSQ_TYPE_Q4_0) {
-          // 1024 + q and 1024 + 16 q
-          const uint32_t w8 = w >> 8;
-          a[r][0] = qmm_off((w & 0x000F000Fu) | 0x64006400u, -1032.0f);
-          a[r][1] = qmm_off((w8 & 0x000F000Fu) | 0x64006400u, -1032.0f);
-          a[r][2] = qmm_off16((w & 0x00F000F0u) | 0x64006400u, -72.0f);
-          a[r][3] = qmm_off16((w8 & 0x00F000F0u) | 0x64006400u, -72.0f);
-        } else {
-          const uint32_t x = w ^ 0x80808080u, y = qmm_ld2(blk + 18 + 4 * c) ^ 0x80808080u;
-          a[r][0] = qmm_off(__byte_perm(x, 0x64646464u, 0x4240), -1152.0f);
-          a[r][1] = qmm_off(__byte_perm(x, 0x64646464u, 0x4341), -1152.0f);
-          a[r][2] = qmm_off(__byte_perm(y, 0x64646464u, 0x4240), -1152.0f);
-          a[r][3] = qmm_off(__byte_perm(y, 0x64646464u, 0x4341), -1152.0f);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if (j == 0 || 4 * j < B.count) {
-          const uint4 b = B.steps(j, i);
-          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          qmm_mma(acc, a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-          qmm_mma(acc, a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
-          u[j][0] += d[0] * (acc[0] + acc[1]);
-          u[j][1] += d[1] * (acc[2] + acc[3]);
-        }
-      }
+      for (int j = 0; j < NT; ++j) u[t][j][0] = u[t][j][1] = 0.0f;
     }
-  } else {  // Q6_K
+    qmm_for<8>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      uint4 b[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) u[j][0] = u[j][1] = 0.0f;
+      for (int j = 0; j < NT; ++j) b[j] = B.steps(j, i);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        uint32_t a[2][4];
+        float d[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const QmmRow row(o[t][r]);
+          d[r] = i < nv ? h2f((uint16_t)row.u16(BB * i)) : 0.0f;
+          const uint32_t w = row.template word<BB * i + 2>(4 * c);
+          if constexpr (TYPE == NSQ_TYPE_Q4_0) {
+            // 1024 + q and 1024 + 16 q
+            const uint32_t w8 = w >> 8;
+            a[r][0] = qmm_off((w & 0x000F000Fu) | 0x64006400u, -1032.0f);
+            a[r][1] = qmm_off((w8 & 0x000F000Fu) | 0x64006400u, -1032.0f);
+            a[r][2] = qmm_off16((w & 0x00F000F0u) | 0x64006400u, -72.0f);
+            a[r][3] = qmm_off16((w8 & 0x00F000F0u) | 0x64006400u, -72.0f);
+          } else {
+            const uint32_t x = w ^ 0x80808080u, y = row.template word<BB * i + 18>(4 * c) ^ 0x80808080u;
+            a[r][0] = qmm_off(__byte_perm(x, 0x64646464u, 0x4240), -1152.0f);
+            a[r][1] = qmm_off(__byte_perm(x, 0x64646464u, 0x4341), -1152.0f);
+            a[r][2] = qmm_off(__byte_perm(y, 0x64646464u, 0x4240), -1152.0f);
+            a[r][3] = qmm_off(__byte_perm(y, 0x64646464u, 0x4341), -1152.0f);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          qmm_mma(acc, a[0][0], a[1][0], a[0][1], a[1][1], b[j].x, b[j].y);
+          qmm_mma(acc, a[0][2], a[1][2], a[0][3], a[1][3], b[j].z, b[j].w);
+          u[t][j][0] += d[0] * (acc[0] + acc[1]);
+          u[t][j][1] += d[1] * (acc[2] + acc[3]);
+        }
+      }
+    });
+  } else {  // Q6_K
+    static_assert(MT == 1, "one row tile");
+    const QmmRow rows[2] = {QmmRow(o[0][0]), QmmRow(o[0][1])};
+    auto& v = u[0];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) v[j][0] = v[j][1] = 0.0f;
     float d[2];
     uint32_t sw[2][4];  // the 16 scale bytes, + 128
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      d[r] = h2f((uint16_t)ld_u16(rows[r] + 208));
+      d[r] = h2f((uint16_t)rows[r].u16(208));
       if constexpr (LAYOUT == NSQ_Q6K_NODESTOR) d[r] *= 0.015625f;  // scale (b - 128) / 64
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sw[r][i] = qmm_ld2(rows[r] + 192 + 4 * i);
+      qmm_for<4>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        sw[r][i] = rows[r].template word<192 + 4 * i>(0);
         if constexpr (LAYOUT == NSQ_Q6K_GGML) sw[r][i] ^= 0x80808080u;
-      }
+      });
     }
     // scale byte g of row r as f32
     auto scale = [&](int r, int g) {
@@ -452,21 +506,20 @@ __device__ __forceinline__ void qmm_unit(const uint8_t* r0, const uint8_t* r1, c
     auto group = [&](int j, const uint32_t (&a)[2][2], uint32_t b0, uint32_t b1, float s0, float s1) {
       float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       qmm_mma(acc, a[0][0], a[1][0], a[0][1], a[1][1], b0, b1);
-      u[j][0] += s0 * (acc[0] + acc[1]);
-      u[j][1] += s1 * (acc[2] + acc[3]);
+      v[j][0] += s0 * (acc[0] + acc[1]);
+      v[j][1] += s1 * (acc[2] + acc[3]);
     };
+    constexpr uint32_t kL = 0x000F000Fu, kH = 0x00F000F0u, kB = 0x64006400u;
     if constexpr (LAYOUT == NSQ_Q6K_GGML) {
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {  // (half n, 16-group of its runs of 32)
-        const int n = p >> 1, g = p & 1;
+      qmm_for<4>([&](auto P) {  // (half n, 16-group of its runs of 32)
+        constexpr int pp = decltype(P)::value, n = pp >> 1, g = pp & 1;
         uint32_t a[4][2][2];  // [run t][row][values 0,2 | 1,3]
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t A = qmm_ld2(rows[r] + 64 * n + 16 * g + 4 * c);
-          const uint32_t Bw = qmm_ld2(rows[r] + 64 * n + 32 + 16 * g + 4 * c);
-          const uint32_t H = qmm_ld2(rows[r] + 128 + 32 * n + 16 * g + 4 * c);
+          const uint32_t A = rows[r].template word<64 * n + 16 * g>(4 * c);
+          const uint32_t Bw = rows[r].template word<64 * n + 32 + 16 * g>(4 * c);
+          const uint32_t H = rows[r].template word<128 + 32 * n + 16 * g>(4 * c);
           const uint32_t A8 = A >> 8, B8 = Bw >> 8, Hl4 = H << 4, Hl2 = H << 2, Hr4 = H >> 4, Hr6 = H >> 6;
-          constexpr uint32_t kL = 0x000F000Fu, kH = 0x00F000F0u, kB = 0x64006400u;
           a[0][r][0] = qmm_off((A & kL) | ((Hl4 & 0x00300030u) | kB), -1056.0f);
           a[0][r][1] = qmm_off((A8 & kL) | ((Hr4 & 0x00300030u) | kB), -1056.0f);
           a[1][r][0] = qmm_off((Bw & kL) | ((Hl2 & 0x00300030u) | kB), -1056.0f);
@@ -484,15 +537,13 @@ __device__ __forceinline__ void qmm_unit(const uint8_t* r0, const uint8_t* r1, c
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          if (j == 0 || 4 * j < B.count) {
-            const uint4 b0 = B.steps(j, 2 * p), b1 = B.steps(j, 2 * p + 1);
-            group(j, a[0], b0.x, b0.y, s[0][0], s[0][1]);
-            group(j, a[1], b0.z, b0.w, s[1][0], s[1][1]);
-            group(j, a[2], b1.x, b1.y, s[2][0], s[2][1]);
-            group(j, a[3], b1.z, b1.w, s[3][0], s[3][1]);
-          }
+          const uint4 b0 = B.steps(j, 2 * pp), b1 = B.steps(j, 2 * pp + 1);
+          group(j, a[0], b0.x, b0.y, s[0][0], s[0][1]);
+          group(j, a[1], b0.z, b0.w, s[1][0], s[1][1]);
+          group(j, a[2], b1.x, b1.y, s[2][0], s[2][1]);
+          group(j, a[3], b1.z, b1.w, s[3][0], s[3][1]);
         }
-      }
+      });
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -504,28 +555,26 @@ __device__ __forceinline__ void qmm_unit(const uint8_t* r0, const uint8_t* r1, c
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             // values 4c .. 4c+3 of the group: ql bytes 8g + 2c, + 1; qh byte 4g + c
-            const uint32_t lo = __byte_perm(ld_u16(rows[r] + 8 * g + 2 * c), 0, 0x4140);
-            const uint32_t hb = ld_u8(rows[r] + 128 + 4 * g + c);
+            const uint32_t lo = __byte_perm(rows[r].u16(8 * g + 2 * c), 0, 0x4140);
+            const uint32_t hb = rows[r].u8(128 + 4 * g + c);
             // bits 0-1, 4-5 and 2-3, 6-7 of hb
-            a[t][r][0] = qmm_off((lo & 0x000F000Fu) | (((hb * 0x00010010u) & 0x00300030u) | 0x64006400u), -1056.0f);
-            a[t][r][1] = qmm_off(((lo >> 4) & 0x000F000Fu) | (((hb * 0x00004004u) & 0x00300030u) | 0x64006400u), -1056.0f);
+            a[t][r][0] = qmm_off((lo & kL) | (((hb * 0x00010010u) & 0x00300030u) | kB), -1056.0f);
+            a[t][r][1] = qmm_off(((lo >> 4) & kL) | (((hb * 0x00004004u) & 0x00300030u) | kB), -1056.0f);
             s[t][r] = scale(r, g);
           }
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          if (j == 0 || 4 * j < B.count) {
-            const uint4 b = B.steps(j, i);
-            group(j, a[0], b.x, b.y, s[0][0], s[0][1]);
-            group(j, a[1], b.z, b.w, s[1][0], s[1][1]);
-          }
+          const uint4 b = B.steps(j, i);
+          group(j, a[0], b.x, b.y, s[0][0], s[0][1]);
+          group(j, a[1], b.z, b.w, s[1][0], s[1][1]);
         }
       }
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      u[j][0] *= d[0];
-      u[j][1] *= d[1];
+      v[j][0] *= d[0];
+      v[j][1] *= d[1];
     }
   }
 }
@@ -538,6 +587,7 @@ struct QmmLists {
   QmmGroup* groups;
   int32_t* plist;  // picks sorted by (expert, pick)
   float* pwts;     // their weights
+  int32_t* ptok;   // their tokens
   int ngroups;
 };
 
@@ -614,12 +664,13 @@ __device__ __forceinline__ QmmLists qmm_build_lists(const QmmParams& p, uint8_t*
   L.groups = reinterpret_cast<QmmGroup*>(mem);
   L.plist = reinterpret_cast<int32_t*>(L.groups + P);
   L.pwts = reinterpret_cast<float*>(L.plist + P);
+  L.ptok = reinterpret_cast<int32_t*>(L.pwts + P);
   int32_t* ids = scratch;
   float* wts = reinterpret_cast<float*>(scratch + P);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool first = blockIdx.x == 0;
   if (p.score >= 0) {
-    for (int m = warp; m < p.M; m += kQmmWarps) {
+    for (int m = warp; m < p.M; m += kQmmWarps + 1) {
       qmm_route(p, m, lane, ids + m * p.top_k, wts + m * p.top_k);
       __syncwarp();
       if (first && lane < p.top_k) {
@@ -658,6 +709,7 @@ __device__ __forceinline__ QmmLists qmm_build_lists(const QmmParams& p, uint8_t*
     }
     L.plist[pos] = q;
     L.pwts[pos] = wts[q];
+    L.ptok[pos] = q / p.top_k;
     // groups of this expert start at every TS-th of its picks; their number
     // so far is filled in below
     L.groups[pos].expert = e;
@@ -700,10 +752,13 @@ __device__ __forceinline__ QmmLists qmm_load_lists(const QmmParams& p, uint8_t* 
   L.groups = reinterpret_cast<QmmGroup*>(mem);
   L.plist = reinterpret_cast<int32_t*>(L.groups + P);
   L.pwts = reinterpret_cast<float*>(L.plist + P);
+  L.ptok = reinterpret_cast<int32_t*>(L.pwts + P);
   L.ngroups = *p.ngroups;
   for (int q = threadIdx.x; q < P; q += kQmmThreads) {
     if (q < L.ngroups) L.groups[q] = p.groups[q];
-    L.plist[q] = p.plist[q];
+    const int pick = p.plist[q];
+    L.plist[q] = pick;
+    L.ptok[q] = (int)((uint32_t)pick / (uint32_t)p.top_k);
     L.pwts[q] = p.pwts[q];
   }
   __syncthreads();
@@ -726,283 +781,553 @@ __device__ __forceinline__ float qmm_ld_cluster(const float* p, uint32_t rank) {
   return v;
 }
 
-// Bytes of shared memory.
-__host__ __device__ inline size_t qmm_stage_bytes(int pitch, int KW, int TS) {
-  return (size_t)kQmmWarps * 16 * pitch + (size_t)KW * TS * kQmmRec;
+// Bytes of a slot: RW tiles of rows at this pitch, then TS records.
+__host__ __device__ inline uint32_t qmm_slot_bytes(int row_tiles, int pitch, int TS) {
+  return (uint32_t)(row_tiles * 16 * pitch + (TS * kQmmRec + 127) / 128 * 128);
 }
-inline size_t qmm_lists_bytes(int P) { return (size_t)P * (sizeof(QmmGroup) + 8); }
+inline size_t qmm_lists_bytes(int P) { return (size_t)P * (sizeof(QmmGroup) + 12); }
 
-// One task is one row tile (of one group for kQmmUp, of all groups for
-// kQmmDown); its units are (group, 256 of K).  A cluster of `split` CTAs
-// shares a task's units.
-template <int TYPE, int LAYOUT, int NT>
-__global__ void __launch_bounds__(kQmmThreads, 2) qmm_kernel(const QmmParams p) {
+// Bias, activation and residual (kQmmLinear), or the residual alone
+// (kQmmDown), for one finished sum.
+__device__ __forceinline__ void qmm_store(const QmmParams& p, int col, int row, float v) {
+  const int64_t at = (int64_t)col * p.n + row;
+  if (p.mode == kQmmLinear) {
+    if (p.bias) v += p.bias[row];
+    v = qmm_act(v, p.act);
+  }
+  if (p.dtype == NSQ_OUT_F32) {
+    if (p.residual) v += static_cast<const float*>(p.residual)[at];
+    static_cast<float*>(p.y)[at] = v;
+  } else {
+    if (p.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[at]);
+    static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+  }
+}
+
+// Where a column stands: its task (tile, and the group for kQmmUp), its unit
+// (u, of group g and column sb of K).
+struct QmmCursor {
+  int tile, g, sb, u;
+};
+
+template <int TYPE, int LAYOUT, int NT, int MODE>
+__global__ void __launch_bounds__(kQmmThreads, 2)
+    qmm_kernel(const __grid_constant__ QmmParams p, const __grid_constant__ CUtensorMap map0,
+               const __grid_constant__ CUtensorMap map1) {
   using F = QmmFmt<TYPE>;
   constexpr int BB = Fmt<TYPE>::BB;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int s_n;
+  constexpr int MT = F::MT;
+  constexpr int WR = 16 * MT;                       // weight rows of a warp
+  constexpr int OR = MODE == kQmmUp ? WR / 2 : WR;  // output rows of a warp
+  uint8_t* const smem = qmm_smem;
+  auto* const full = reinterpret_cast<uint64_t(*)[kQmmMaxStages]>(smem);           // [column][slot]
+  auto* const empty = reinterpret_cast<uint64_t(*)[kQmmMaxStages]>(smem + 256);
+  auto* const ready = reinterpret_cast<uint64_t(*)[2]>(smem + 512);                // [row tiles][buffer]
+  auto* const taken = reinterpret_cast<uint64_t(*)[2]>(smem + 640);
+  int* const s_n = reinterpret_cast<int*>(smem + 768);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int KW = p.KW, RW = p.RW, S = p.stages, TS = p.TS, YC = p.YC;
-  const int kw = warp % KW, rw = warp / KW;
-  const size_t stage_bytes = qmm_stage_bytes(F::PITCH, KW, TS);
-  float* ys = reinterpret_cast<float*>(smem + S * stage_bytes);  // [warp][YC][16]
-  float* red = ys + (size_t)kQmmWarps * YC * 16;                 // [YC][16 RW], for a split K
-  uint8_t* lists_mem = reinterpret_cast<uint8_t*>(red + (p.split > 1 ? YC * 16 * RW : 0));
+  const int pitch = p.rows_aligned ? F::PA : F::PG;
+  const uint32_t slot_bytes = qmm_slot_bytes(RW * MT, pitch, TS);
+  const uint32_t recs_at = RW * WR * pitch;          // of a slot
+  const uint32_t ring_bytes = S * KW * slot_bytes;
+  // partial sums [buffer][warp][YC][WR]; a split product keeps them in the
+  // ring, which is idle by then, except kQmmDown's, which grow unit by unit
+  const bool in_ring = MODE != kQmmDown && p.split > 1;
+  float* const ys = reinterpret_cast<float*>(smem + kQmmCtl + (in_ring ? 0 : ring_bytes));
+  const int ys_warp = YC * WR, ys_buf = kQmmWarps * ys_warp;
+  const uint32_t zeros = kQmmCtl + ring_bytes + (in_ring ? 0 : p.PB * ys_buf * 4);  // a record of zeros
   const int rank = p.split > 1 ? (int)qmm_cluster_rank() : 0;
   const int cta = blockIdx.x / p.split, nctas = gridDim.x / p.split;
-  const uint64_t pol = l2_policy_evict_first();
-  const int tile_rows = p.mode == kQmmUp ? 8 * RW : 16 * RW;
+  const int tile_rows = OR * RW;
   const int tiles = (int)((p.n + tile_rows - 1) / tile_rows);
 
-  QmmLists L{};
-  if (p.mode == kQmmUp) {
-    qmm_dep_wait();
-    qmm_dep_launch();
-    L = qmm_build_lists(p, lists_mem, reinterpret_cast<int32_t*>(smem), &s_n);
-  } else if (p.mode == kQmmDown) {
-    qmm_dep_wait();
-    qmm_dep_launch();
-    L = qmm_load_lists(p, lists_mem);
-  } else {
-    L.ngroups = 1;
-  }
-  const int tasks = p.mode == kQmmUp ? tiles * L.ngroups : tiles;
-  const int units = p.mode == kQmmDown ? L.ngroups * p.nsb : p.nsb;
-  const int u0 = (int)((int64_t)units * rank / p.split), u1 = (int)((int64_t)units * (rank + 1) / p.split);
-  const int steps = max(1, (units / p.split + (units % p.split ? 1 : 0) + KW - 1) / KW);
-
-  auto group_of = [&](int task, int u, int& sb) {  // group of a task's unit
-    if (p.mode == kQmmDown) {
-      const int g = u / p.nsb;
-      sb = u - g * p.nsb;
-      return g;
-    }
-    sb = u;
-    return p.mode == kQmmUp ? task / tiles : 0;
-  };
-  auto row_base = [&](int task) { return (int64_t)(p.mode == kQmmUp ? task % tiles : task) * tile_rows; };
-  // first byte of the unit in weight row r of this warp (r < 16)
-  auto unit_ptr = [&](int expert, int64_t base, int r, int sb) {
-    const uint8_t* w = p.w0;
-    int64_t row;
-    if (p.mode == kQmmUp) {
-      row = base + rw * 8 + (r & 7);
-      if (r >= 8) w = p.w1;
-    } else {
-      row = base + rw * 16 + r;
-    }
-    if (row >= p.n) row = p.n - 1;  // rows past the end repeat the last one; their sums are not written
-    return w + ((int64_t)expert * p.n + row) * p.rb + (int64_t)sb * F::CB;
-  };
-  auto issue_w = [&](int task, int step, int stage) {
-    const int u = u0 + step * KW + kw;
-    if (task >= tasks || u >= u1) return;
-    int sb;
-    const int g = group_of(task, u, sb);
-    const int expert = p.mode == kQmmLinear ? 0 : L.groups[g].expert;
-    const int64_t base = row_base(task);
-    const uint32_t dst = smem_u32(smem + stage * stage_bytes + (size_t)warp * 16 * F::PITCH);
-#pragma unroll
-    for (int i = 0; i < (16 * F::NCH + 31) / 32; ++i) {
-      const int idx = lane + 32 * i;
-      const int r = idx / F::NCH, ch = idx % F::NCH;
-      if (r < 16) {
-        const uint8_t* src = unit_ptr(expert, base, r, sb);
-        if constexpr (F::aligned) {
-          qmm_cp16(dst + r * F::PITCH + 16 * ch, src + 16 * ch, 16, pol);
-        } else {
-          const int mis = (int)(reinterpret_cast<uintptr_t>(src) & 15);
-          int need = F::CB;
-          if constexpr (Fmt<TYPE>::QK == 32) need = min(8, p.nblk - 8 * sb) * BB;
-          if (16 * ch < mis + need) {
-            const uint8_t* a = src - mis + 16 * ch;
-            const uint8_t* end = (p.mode == kQmmUp && r >= 8 ? p.w1 : p.w0) + p.wbytes;
-            qmm_cp16(dst + r * F::PITCH + 16 * ch, a, (int)min((int64_t)16, (int64_t)(end - a)), pol);
-          }
-        }
-      }
-    }
-  };
-  auto issue_b = [&](int task, int step, int stage) {
-    const int u = u0 + step * KW + kw;
-    if (task >= tasks || u >= u1) return;
-    int sb;
-    const int g = group_of(task, u, sb);
-    const int count = p.mode == kQmmLinear ? p.M : L.groups[g].count;
-    const int start = p.mode == kQmmLinear ? 0 : L.groups[g].start;
-    const uint32_t dst =
-        smem_u32(smem + stage * stage_bytes + (size_t)kQmmWarps * 16 * F::PITCH + (size_t)kw * TS * kQmmRec);
-    constexpr int RC = kQmmRec / 16;
-    for (int idx = rw * 32 + lane; idx < count * RC; idx += RW * 32) {
-      const int t = idx / RC, ch = idx - t * RC;
-      int row = t;
-      if (p.mode != kQmmLinear) {
-        row = L.plist[start + t];
-        if (p.mode == kQmmUp) row /= p.top_k;
-      }
-      qmm_cp16(dst + t * kQmmRec + 16 * ch, p.recs + ((int64_t)row * p.nsb + sb) * kQmmRec + 16 * ch);
-    }
-  };
-
-  // producer cursor
-  int ptask = cta, pstep = 0;
-  auto advance = [&](int& task, int& step) {
-    if (++step == steps) {
-      step = 0;
-      task += nctas;
-    }
-  };
-  for (int s = 0; s < S - 1; ++s) {
-    issue_w(ptask, pstep, s);
-    advance(ptask, pstep);
-  }
-  if (p.mode == kQmmLinear) {
-    // the weights do not depend on the kernels before; the records do
-    qmm_dep_wait();
-    qmm_dep_launch();
-  }
   {
-    int t = cta, st = 0;
-    for (int s = 0; s < S - 1; ++s) {
-      issue_b(t, st, s);
-      qmm_commit();
-      advance(t, st);
+    // the boxes' destination: a misaligned one would fault (the address is
+    // hidden from the compiler, which takes the declared alignment for granted)
+    uint32_t start = smem_u32(smem);
+    asm volatile("" : "+r"(start));
+    if (start & 127) {
+      report_status(NSQ_ERR_ALIGN);
+      return;
     }
   }
-
-  float tot[NT][2];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) tot[j][0] = tot[j][1] = 0.0f;
-  float* my_ys = ys + (size_t)warp * YC * 16;
-  const int lr = lane >> 2, lc = lane & 3;
-  int stage = 0;
-  for (int task = cta, step = 0; task < tasks;) {
-    qmm_wait(S);
-    __syncthreads();
-    {
-      const int ps = stage == 0 ? S - 1 : stage - 1;
-      issue_w(ptask, pstep, ps);
-      issue_b(ptask, pstep, ps);
-      qmm_commit();
-      advance(ptask, pstep);
-    }
-    if (p.mode == kQmmDown && step == 0) {
-      for (int i = lane; i < YC * 16; i += 32) my_ys[i] = 0.0f;
-      __syncwarp();
-    }
-    const int u = u0 + step * KW + kw;
-    if (u < u1) {
-      int sb;
-      const int g = group_of(task, u, sb);
-      const int count = p.mode == kQmmLinear ? p.M : L.groups[g].count;
-      const uint8_t* wst = smem + stage * stage_bytes + (size_t)warp * 16 * F::PITCH;
-      const uint8_t* bst = smem + stage * stage_bytes + (size_t)kQmmWarps * 16 * F::PITCH + (size_t)kw * TS * kQmmRec;
-      const uint8_t* r0 = wst + lr * F::PITCH;
-      const uint8_t* r1 = r0 + 8 * F::PITCH;
-      if constexpr (!F::aligned) {
-        const int expert = p.mode == kQmmLinear ? 0 : L.groups[g].expert;
-        const int64_t base = row_base(task);
-        r0 += reinterpret_cast<uintptr_t>(unit_ptr(expert, base, lr, sb)) & 15;
-        r1 += reinterpret_cast<uintptr_t>(unit_ptr(expert, base, lr + 8, sb)) & 15;
+  for (int i = threadIdx.x; i < kQmmRec / 4; i += kQmmThreads) reinterpret_cast<uint32_t*>(smem + zeros)[i] = 0u;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < KW; ++i) {
+      for (int k = 0; k < S; ++k) {
+        mbar_init(&full[i][k], 1);
+        mbar_init(&empty[i][k], RW);
       }
-      QmmB B;
-      B.c = lc;
-      B.flip = (lr & 1) * 4;
-      B.tok = lr >> 1;
-      B.count = count;
-      B.rec = bst + B.tok * kQmmRec + (lr & 1) * 512;
-      float uv[NT][2];
-      qmm_unit<TYPE, LAYOUT, NT>(r0, r1, B, min(8, p.nblk - 8 * sb), uv);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int t = 4 * j + lc;
-        if (t < count) {
-          const float s = *reinterpret_cast<const float*>(bst + t * kQmmRec + 1088);
-          if (p.mode == kQmmDown) {
-            const int pick = L.groups[g].start + t;
-            const float w = L.pwts[pick];
-            float* q = my_ys + (L.plist[pick] / p.top_k) * 16 + lr;
-            q[0] += w * (s * uv[j][0]);
-            q[8] += w * (s * uv[j][1]);
-          } else {
-            tot[j][0] += s * uv[j][0];
-            tot[j][1] += s * uv[j][1];
+    }
+    for (int i = 0; i < RW; ++i) {
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&ready[i][k], KW);
+        mbar_init(&taken[i][k], 1);
+      }
+    }
+    fence_mbar_init();
+  }
+  QmmLists L{};
+  if constexpr (MODE == kQmmLinear) {
+    L.ngroups = 1;
+    __syncthreads();
+  } else {
+    qmm_dep_wait();
+    qmm_dep_launch();
+    uint8_t* lists_mem = smem + zeros + kQmmRec;
+    if constexpr (MODE == kQmmUp) {
+      L = qmm_build_lists(p, lists_mem, reinterpret_cast<int32_t*>(smem + kQmmCtl), s_n);
+      fence_proxy_async_smem();  // the ring held the lists' scratch
+      __syncthreads();
+    } else {
+      L = qmm_load_lists(p, lists_mem);
+    }
+  }
+  const int units = MODE == kQmmDown ? L.ngroups * p.nsb : p.nsb;
+  const int u0 = p.split > 1 ? (int)((int64_t)units * rank / p.split) : 0;
+  const int u1 = p.split > 1 ? (int)((int64_t)units * (rank + 1) / p.split) : units;
+
+  // cursors: column kw takes units u0 + kw, u0 + kw + KW, ... of every task
+  const int up_dg = MODE == kQmmUp ? nctas / tiles : 0, up_dt = MODE == kQmmUp ? nctas - up_dg * tiles : nctas;
+  auto first_task = [&](QmmCursor& c) {
+    c.tile = cta;
+    c.g = 0;
+    if constexpr (MODE == kQmmUp) {
+      c.g = cta / tiles;
+      c.tile = cta - c.g * tiles;
+    }
+  };
+  auto first_unit = [&](QmmCursor& c, int kw) {
+    c.u = c.sb = u0 + kw;
+    if constexpr (MODE == kQmmDown) {
+      c.g = c.u / p.nsb;
+      c.sb = c.u - c.g * p.nsb;
+    }
+  };
+  auto live = [&](const QmmCursor& c) { return MODE == kQmmUp ? c.g < L.ngroups : c.tile < tiles; };
+  auto next_unit = [&](QmmCursor& c) {
+    c.u += KW;
+    c.sb += KW;
+    if constexpr (MODE == kQmmDown) {
+      while (c.sb >= p.nsb) {
+        c.sb -= p.nsb;
+        ++c.g;
+      }
+    }
+  };
+  auto next_task = [&](QmmCursor& c) {
+    c.tile += up_dt;
+    if constexpr (MODE == kQmmUp) {
+      c.g += up_dg;
+      if (c.tile >= tiles) {
+        c.tile -= tiles;
+        ++c.g;
+      }
+    }
+  };
+
+  bool ok = true;
+  if (warp == kQmmWarps) {
+    // ---- producer.  With TMA boxes lane (kw, t0) serves column kw: its t0-th
+    // lane issues the box and every lane its share of the records.  Without,
+    // the whole warp copies the rows of one column after the other.
+    const uint64_t pol = l2_policy_evict_first();
+    const uint32_t base = smem_u32(smem);  // slots are offsets from it
+    auto box = [&](const QmmCursor& c, uint32_t slot, uint64_t* bar) {
+      const int row0 = (MODE == kQmmLinear ? 0 : L.groups[c.g].expert) * (int)p.n + c.tile * tile_rows;
+      const int x = ((c.sb * F::CB) & ~15) / 2;  // 16-bit elements
+      if constexpr (MODE == kQmmUp) {
+        qmm_tma_2d(slot, &map0, x, row0, bar, pol);
+        qmm_tma_2d(slot + RW * (WR / 2) * pitch, &map1, x, row0, bar, pol);
+      } else {
+        qmm_tma_2d(slot, &map0, x, row0, bar, pol);
+      }
+    };
+    auto group_count = [&](const QmmCursor& c) { return MODE == kQmmLinear ? p.M : L.groups[c.g].count; };
+    auto record = [&](const QmmCursor& c, int t) {
+      int row = t;
+      if constexpr (MODE == kQmmUp) row = L.ptok[L.groups[c.g].start + t];
+      if constexpr (MODE == kQmmDown) row = L.plist[L.groups[c.g].start + t];
+      return p.recs + ((int64_t)row * p.nsb + c.sb) * kQmmRec;
+    };
+    if (p.rows_aligned) {
+      const int kw = lane & (KW - 1), t0 = lane / KW, dt = 32 / KW;
+      const uint32_t w_bytes = RW * WR * pitch;
+      QmmCursor c;
+      first_task(c);
+      first_unit(c, kw);
+      int n = 0;  // units of this column so far
+      if constexpr (MODE == kQmmLinear) {
+        // the weights do not depend on the kernels before: the first boxes go
+        // out ahead of the dependency wait
+        QmmCursor w = c;
+        for (int k = 0; k < S && t0 == 0 && live(w); ++k) {
+          while (live(w) && w.u >= u1) {
+            next_task(w);
+            first_unit(w, kw);
+            if (w.u >= u1) break;  // a column without units
+          }
+          if (!live(w) || w.u >= u1) break;
+          qmm_expect_tx(&full[kw][k], w_bytes);
+          box(w, base + kQmmCtl + (k * KW + kw) * slot_bytes, &full[kw][k]);
+          next_unit(w);
+        }
+        __syncwarp();
+        qmm_dep_wait();
+        qmm_dep_launch();
+      }
+      int stage = 0;
+      uint32_t phase = 0;
+      for (; ok && live(c); next_task(c)) {
+        for (first_unit(c, kw); c.u < u1; next_unit(c)) {
+          uint64_t* bar = &full[kw][stage];
+          if (n >= S && !mbar_wait_bounded(&empty[kw][stage], phase ^ 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes;
+          const int count = group_count(c);
+          if (t0 == 0) {
+            const bool early = MODE == kQmmLinear && n < S;
+            mbar_arrive_expect_tx(bar, (early ? 0 : w_bytes) + count * kQmmRec);
+            if (!early) box(c, base + slot, bar);
+          }
+          for (int t = t0; t < count; t += dt) bulk_g2s(smem + slot + recs_at + t * kQmmRec, record(c, t), kQmmRec, bar);
+          ++n;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1;
           }
         }
       }
-      __syncwarp();
+    } else {
+      if constexpr (MODE == kQmmLinear) {
+        qmm_dep_wait();
+        qmm_dep_launch();
+      }
+      // all columns step by step; a column's slot and phase go by its own count of units
+      int n[kQmmWarps];
+#pragma unroll
+      for (int k = 0; k < kQmmWarps; ++k) n[k] = 0;
+      QmmCursor c;
+      first_task(c);
+      for (; ok && live(c); next_task(c)) {
+        for (int s0 = 0; ok && u0 + s0 < u1; s0 += KW) {
+#pragma unroll
+          for (int kw = 0; kw < kQmmWarps; ++kw) {
+            const int u = u0 + s0 + kw;
+            if (kw >= KW || u >= u1 || !ok) continue;
+            QmmCursor d = c;
+            d.u = d.sb = u;
+            if constexpr (MODE == kQmmDown) {
+              d.g = u / p.nsb;
+              d.sb = u - d.g * p.nsb;
+            }
+            const int stage = n[kw] % S, turn = n[kw] / S;
+            ++n[kw];
+            uint64_t* bar = &full[kw][stage];
+            if (turn > 0 && !mbar_wait_bounded(&empty[kw][stage], (turn & 1) ^ 1)) {
+              ok = false;
+              continue;
+            }
+            fence_proxy_async_smem();  // a tensor's last bytes are stored by hand
+            const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes;
+            const int64_t row0 = (MODE == kQmmLinear ? 0 : (int64_t)L.groups[d.g].expert * p.n) + d.tile * tile_rows;
+            const int valid = (int)min((int64_t)tile_rows, p.n - (int64_t)d.tile * tile_rows);
+            int need = F::CB;
+            if constexpr (Fmt<TYPE>::QK == 32) need = min(8, p.nblk - 8 * d.sb) * BB;
+            const int64_t cap = p.wbytes & ~(int64_t)15;
+            auto span = [&](int r, const uint8_t*& w, int64_t& a, int64_t& e, int64_t& end) {
+              int rr = r;
+              w = p.w0;
+              if constexpr (MODE == kQmmUp) {
+                if (r >= RW * (WR / 2)) {
+                  rr -= RW * (WR / 2);
+                  w = p.w1;
+                }
+              }
+              if (rr >= valid) return false;
+              const int64_t at = (row0 + rr) * p.rb + (int64_t)d.sb * F::CB;
+              a = at & ~(int64_t)15;
+              end = at + need;
+              e = (end + 15) & ~(int64_t)15;
+              if (e > cap) e = cap > a ? cap : a;
+              return true;
+            };
+            const int count = group_count(d);
+            uint32_t bytes = lane < count ? kQmmRec : 0;
+            for (int r = lane; r < RW * WR; r += 32) {
+              const uint8_t* w;
+              int64_t a, e, end;
+              if (!span(r, w, a, e, end)) continue;
+              bytes += (uint32_t)(e - a);
+              for (int64_t i = e; i < end; ++i) smem[slot + r * pitch + (i - a)] = w[i];  // past the last whole 16 bytes
+            }
+            bytes = __reduce_add_sync(0xffffffffu, bytes);
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+            __syncwarp();
+            for (int r = lane; r < RW * WR; r += 32) {
+              const uint8_t* w;
+              int64_t a, e, end;
+              if (span(r, w, a, e, end) && e > a) bulk_g2s(smem + slot + r * pitch, w + a, (uint32_t)(e - a), bar);
+            }
+            if (lane < count) bulk_g2s(smem + slot + recs_at + lane * kQmmRec, record(d, lane), kQmmRec, bar);
+          }
+        }
+      }
     }
-    if (step == steps - 1) {
-      // ---- the task's sums
-      if (p.mode != kQmmDown) {
+  } else {
+    // ---- consumers
+    if constexpr (MODE == kQmmLinear) qmm_dep_wait();  // residual and outputs
+    const int kw = warp & (KW - 1), rw = warp / KW;
+    const int lr = lane >> 2, lc = lane & 3;
+    const bool split = p.split > 1;
+    float tot[MT][NT][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) tot[t][j][0] = tot[t][j][1] = 0.0f;
+    }
+    // rows of this lane in a slot: row half h of tile t
+    auto slot_row = [&](int t, int h) {
+      if constexpr (MODE == kQmmUp) {
+        return MT == 2 ? (t * RW + rw) * 16 + 8 * h + lr : (h * RW + rw) * 8 + lr;
+      } else {
+        return rw * WR + 16 * t + 8 * h + lr;
+      }
+    };
+    int stage = 0, seq = 0;
+    uint32_t phase = 0;
+    QmmCursor c;
+    first_task(c);
+    for (; ok && live(c); next_task(c), ++seq) {
+      const int buf = p.PB == 2 ? seq & 1 : 0, turn = p.PB == 2 ? seq >> 1 : seq;
+      float* my_ys = ys + buf * ys_buf + warp * ys_warp;
+      const bool own_ys = p.PB > 0 && !split;
+      if constexpr (MODE == kQmmDown) {
+        if (own_ys && turn > 0 && !mbar_wait_bounded(&taken[rw][buf], (turn & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        __syncwarp();
+        for (int i = lane; i < ys_warp; i += 32) my_ys[i] = 0.0f;
+        __syncwarp();
+      }
+      for (first_unit(c, kw); c.u < u1; next_unit(c)) {
+        if (!mbar_wait_bounded(&full[kw][stage], phase)) {
+          ok = false;
+          break;
+        }
+        __syncwarp();
+        const int count = MODE == kQmmLinear ? p.M : L.groups[c.g].count;
+        const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes;
+        uint32_t o[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = slot_row(t, h);
+            uint32_t mis = 0;
+            if constexpr (F::CB % 16 != 0 || Fmt<TYPE>::QK == 32) {
+              mis = (uint32_t)(c.sb * F::CB) & 15;
+              if (!p.rows_aligned) {
+                const int rr = MODE == kQmmUp && r >= RW * (WR / 2) ? r - RW * (WR / 2) : r;
+                const int64_t row = (MODE == kQmmLinear ? 0 : (int64_t)L.groups[c.g].expert * p.n) + c.tile * tile_rows + rr;
+                mis = (uint32_t)(row * p.rb + (int64_t)c.sb * F::CB) & 15;
+              }
+            }
+            o[t][h] = slot + r * pitch + mis;
+          }
+        }
+        float uv[MT][NT][2];
+        const int nv = min(8, p.nblk - 8 * c.sb);
+        // as many n-tiles as the group has tokens
+        auto unit = [&](auto N) {
+          constexpr int nt = decltype(N)::value;
+          const QmmB<nt> B(slot + recs_at, zeros, count, lr, lc);
+          float v[MT][nt][2];
+          qmm_unit<TYPE, LAYOUT, MT, nt>(o, lc, B, nv, v);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int j = 0; j < nt; ++j) {
+              uv[t][j][0] = v[t][j][0];
+              uv[t][j][1] = v[t][j][1];
+            }
+          }
+        };
+        if (NT == 1 || count <= 4) {
+          unit(std::integral_constant<int, 1>{});
+        } else if (NT == 2 || count <= 8) {
+          unit(std::integral_constant<int, NT < 2 ? NT : 2>{});
+        } else {
+          unit(std::integral_constant<int, NT>{});
+        }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          if (4 * j + lc < YC) {
-            my_ys[(4 * j + lc) * 16 + lr] = tot[j][0];
-            my_ys[(4 * j + lc) * 16 + lr + 8] = tot[j][1];
-          }
-          tot[j][0] = tot[j][1] = 0.0f;
-        }
-      }
-      __syncthreads();
-      const int64_t base = row_base(task);
-      auto sum_kw = [&](int col, int r) {  // over the KW warps of row r (0 .. 16 RW - 1)
-        const float* q = ys + ((size_t)(r >> 4) * KW * YC + col) * 16 + (r & 15);
-        float v = q[0];
-        for (int k = 1; k < KW; ++k) v += q[(size_t)k * YC * 16];
-        return v;
-      };
-      if (p.mode == kQmmUp) {
-        const int g = task / tiles, count = L.groups[g].count, start = L.groups[g].start;
-        for (int i = threadIdx.x; i < tile_rows * count; i += kQmmThreads) {
-          const int col = i / tile_rows, r = i - col * tile_rows;
-          const int64_t row = base + r;
-          if (row < p.n) {
-            const int q = (r >> 3) * 16 + (r & 7);
-            const float gate = sum_kw(col, q), up = sum_kw(col, q + 8);
-            p.h[(int64_t)L.plist[start + col] * p.n + row] = qmm_act(gate, p.act) * up;
-          }
-        }
-      } else {
-        const int cols = p.M;
-        if (p.split > 1) {
-          for (int i = threadIdx.x; i < tile_rows * cols; i += kQmmThreads) red[i] = sum_kw(i / tile_rows, i % tile_rows);
-          qmm_cluster_sync();
-        }
-        if (rank == 0) {
-          for (int i = threadIdx.x; i < tile_rows * cols; i += kQmmThreads) {
-            const int col = i / tile_rows, r = i - col * tile_rows;
-            const int64_t row = base + r;
-            if (row < p.n) {
-              float v;
-              if (p.split > 1) {
-                v = red[i];
-                for (int k = 1; k < p.split; ++k) v += qmm_ld_cluster(red + i, (uint32_t)k);
-              } else {
-                v = sum_kw(col, r);
+          const int tk = 4 * j + lc;
+          if (tk < count) {
+            float s = qmm_lds<float>(slot + recs_at + tk * kQmmRec + 1088);
+            if constexpr (MODE == kQmmDown) {
+              const int pick = L.groups[c.g].start + tk;
+              const float w = L.pwts[pick];
+              float* q = my_ys + L.ptok[pick] * WR + lr;
+#pragma unroll
+              for (int t = 0; t < MT; ++t) {
+                q[16 * t] += w * (s * uv[t][j][0]);
+                q[16 * t + 8] += w * (s * uv[t][j][1]);
               }
-              const int64_t at = (int64_t)col * p.n + row;
-              if (p.mode == kQmmLinear) {
-                if (p.bias) v += p.bias[row];
-                v = qmm_act(v, p.act);
-              }
-              if (p.dtype == NSQ_OUT_F32) {
-                if (p.residual) v += static_cast<const float*>(p.residual)[at];
-                static_cast<float*>(p.y)[at] = v;
-              } else {
-                if (p.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[at]);
-                static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+            } else {
+#pragma unroll
+              for (int t = 0; t < MT; ++t) {
+                tot[t][j][0] += s * uv[t][j][0];
+                tot[t][j][1] += s * uv[t][j][1];
               }
             }
           }
         }
-        if (p.split > 1) qmm_cluster_sync();  // the leader has read every rank's sums
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[kw][stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok || split) break;  // a split product has one task; its sums are joined below
+      const int row0 = c.tile * tile_rows + rw * OR;
+      if (p.PB == 0) {
+        // ---- KW == 1: outputs straight from the registers
+        const int cnt = MODE == kQmmLinear ? p.M : L.groups[c.g].count;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int tk = 4 * j + lc;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if constexpr (MODE == kQmmUp) {
+                // gate and up of an output row: row halves of one tile, or two tiles
+                if ((MT == 2 ? t : h) == 0 && tk < cnt) {
+                  const int row = row0 + (MT == 2 ? 8 * h : 0) + lr;
+                  const float up = MT == 2 ? tot[MT - 1][j][h] : tot[0][j][1];
+                  if (row < p.n) p.h[(int64_t)L.plist[L.groups[c.g].start + tk] * p.n + row] = qmm_act(tot[t][j][h], p.act) * up;
+                }
+              } else if constexpr (MODE == kQmmLinear) {
+                const int row = row0 + 16 * t + 8 * h + lr;
+                if (tk < cnt && row < p.n) qmm_store(p, tk, row, tot[t][j][h]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) tot[t][j][0] = tot[t][j][1] = 0.0f;
+        }
+        continue;
+      }
+      // ---- join the KW columns' sums: every warp leaves its own, one of them adds
+      if constexpr (MODE != kQmmDown) {
+        if (turn > 0 && !mbar_wait_bounded(&taken[rw][buf], (turn & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            if (4 * j + lc < YC) {
+              float* q = my_ys + (4 * j + lc) * WR + 16 * t + lr;
+              q[0] = tot[t][j][0];
+              q[8] = tot[t][j][1];
+            }
+            tot[t][j][0] = tot[t][j][1] = 0.0f;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ready[rw][buf]);
+      if (kw == (seq & (KW - 1))) {
+        if (!mbar_wait_bounded(&ready[rw][buf], turn & 1)) {
+          ok = false;
+          break;
+        }
+        __syncwarp();
+        const float* y0 = ys + buf * ys_buf + rw * KW * ys_warp;
+        auto sum_kw = [&](int col, int r) {
+          float v = y0[col * WR + r];
+          for (int k = 1; k < KW; ++k) v += y0[k * ys_warp + col * WR + r];
+          return v;
+        };
+        const int cnt = MODE == kQmmUp ? L.groups[c.g].count : p.M;
+        for (int i = lane; i < OR * cnt; i += 32) {
+          const int col = i / OR, r = i % OR;
+          if (row0 + r < p.n) {
+            if constexpr (MODE == kQmmUp) {
+              const float gate = sum_kw(col, r), up = sum_kw(col, r + OR);
+              p.h[(int64_t)L.plist[L.groups[c.g].start + col] * p.n + row0 + r] = qmm_act(gate, p.act) * up;
+            } else {
+              qmm_store(p, col, row0 + r, sum_kw(col, r));
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&taken[rw][buf]);
       }
     }
-    advance(task, step);
-    if (++stage == S) stage = 0;
+    if constexpr (MODE == kQmmLinear) {
+      if (split) {
+        // every warp of the CTA is done with the ring
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kQmmWarps) : "memory");
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            if (4 * j + lc < YC) {
+              float* q = ys + warp * ys_warp + (4 * j + lc) * WR + 16 * t + lr;
+              q[0] = tot[t][j][0];
+              q[8] = tot[t][j][1];
+            }
+          }
+        }
+      }
+    }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (MODE != kQmmUp) {
+    if (p.split > 1) {
+      // ---- a K split over the cluster: each rank adds its columns' sums into
+      // those of its first column, rank 0 adds the ranks' in order
+      __syncthreads();
+      const int outs = RW * WR * p.M;
+      auto place = [&](int i, int& col, int& r) -> float* {
+        col = i / (RW * WR);
+        r = i - col * (RW * WR);
+        return ys + (r / WR) * KW * ys_warp + col * WR + r % WR;
+      };
+      for (int i = threadIdx.x; i < outs; i += kQmmThreads) {
+        int col, r;
+        float* q = place(i, col, r);
+        float v = q[0];
+        for (int k = 1; k < KW; ++k) v += q[k * ys_warp];
+        q[0] = v;
+      }
+      qmm_cluster_sync();
+      if (rank == 0) {
+        for (int i = threadIdx.x; i < outs; i += kQmmThreads) {
+          int col, r;
+          const float* q = place(i, col, r);
+          float v = q[0];
+          for (int k = 1; k < p.split; ++k) v += qmm_ld_cluster(q, (uint32_t)k);
+          const int row = cta * tile_rows + r;
+          if (row < p.n) qmm_store(p, col, row, v);
+        }
+      }
+      qmm_cluster_sync();  // the leader has read every rank's sums
+    }
+  }
 }
 
 }  // namespace nsq

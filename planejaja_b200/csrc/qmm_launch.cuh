@@ -5,9 +5,9 @@
 
 namespace nsq {
 
-template <int TYPE, int LAYOUT, int NT>
-int launch_qmm_t(const QmmParams& p, int grid, size_t smem, cudaStream_t st) {
-  auto kern = qmm_kernel<TYPE, LAYOUT, NT>;
+template <int TYPE, int LAYOUT, int NT, int MODE>
+int launch_qmm_t(const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
+  auto kern = qmm_kernel<TYPE, LAYOUT, NT, MODE>;
   // the opt-in limit is set once per device; the launches ask for what they need
   static bool configured[64] = {};
   int dev = 0;
@@ -34,22 +34,29 @@ int launch_qmm_t(const QmmParams& p, int grid, size_t smem, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = p.split > 1 ? 2 : 1;
   note_launch();
-  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kern, p, maps[0], maps[1]) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
+}
+
+template <int TYPE, int LAYOUT, int NT>
+int launch_qmm_mode(const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
+  if (p.mode == kQmmLinear) return launch_qmm_t<TYPE, LAYOUT, NT, kQmmLinear>(p, maps, grid, smem, st);
+  if (p.mode == kQmmUp) return launch_qmm_t<TYPE, LAYOUT, NT, kQmmUp>(p, maps, grid, smem, st);
+  return launch_qmm_t<TYPE, LAYOUT, NT, kQmmDown>(p, maps, grid, smem, st);
 }
 
 template <int TYPE, int LAYOUT>
-int launch_qmm_layout(const QmmParams& p, int grid, size_t smem, cudaStream_t st) {
-  if (p.TS <= 4) return launch_qmm_t<TYPE, LAYOUT, 1>(p, grid, smem, st);
-  if (p.TS <= 8) return launch_qmm_t<TYPE, LAYOUT, 2>(p, grid, smem, st);
-  return launch_qmm_t<TYPE, LAYOUT, 4>(p, grid, smem, st);
+int launch_qmm_layout(const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
+  if (p.TS <= 4) return launch_qmm_mode<TYPE, LAYOUT, 1>(p, maps, grid, smem, st);
+  if (p.TS <= 8) return launch_qmm_mode<TYPE, LAYOUT, 2>(p, maps, grid, smem, st);
+  return launch_qmm_mode<TYPE, LAYOUT, 4>(p, maps, grid, smem, st);
 }
 
 template <int TYPE>
-int launch_qmm_type(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st) {
+int launch_qmm_type(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
   if constexpr (TYPE == NSQ_TYPE_Q5_K || TYPE == NSQ_TYPE_Q6_K) {
-    if (layout == NSQ_Q6K_NODESTOR) return launch_qmm_layout<TYPE, NSQ_Q6K_NODESTOR>(p, grid, smem, st);
+    if (layout == NSQ_Q6K_NODESTOR) return launch_qmm_layout<TYPE, NSQ_Q6K_NODESTOR>(p, maps, grid, smem, st);
   }
-  return launch_qmm_layout<TYPE, NSQ_Q6K_GGML>(p, grid, smem, st);
+  return launch_qmm_layout<TYPE, NSQ_Q6K_GGML>(p, maps, grid, smem, st);
 }
 
 }  // namespace nsq

@@ -2,7 +2,7 @@
 #include "qmm_launch.cuh"
 
 namespace nsq {
-int launch_qmm_q40(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st) {
-  return launch_qmm_type<NSQ_TYPE_Q4_0>(layout, p, grid, smem, st);
+int launch_qmm_q40(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
+  return launch_qmm_type<NSQ_TYPE_Q4_0>(layout, p, maps, grid, smem, st);
 }
 }  // namespace nsq

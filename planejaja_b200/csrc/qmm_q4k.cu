@@ -2,7 +2,7 @@
 #include "qmm_launch.cuh"
 
 namespace nsq {
-int launch_qmm_q4k(int layout, const QmmParams& p, int grid, size_t smem, cudaStream_t st) {
-  return launch_qmm_type<NSQ_TYPE_Q4_K>(layout, p, grid, smem, st);
+int launch_qmm_q4k(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
+  return launch_qmm_type<NSQ_TYPE_Q4_K>(layout, p, maps, grid, smem, st);
 }
 }  // namespace nsq
