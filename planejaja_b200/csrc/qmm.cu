@@ -17,84 +17,119 @@ int check_weights(const void* w, int type, int layout, int64_t K);
 int device_check(int* num_sms);
 
 constexpr int kPrepThreads = 32 * kQmmWarps;
-constexpr int kRouteTok = 8;  // tokens of one CTA's logits
+constexpr int kRouteTok = 8;    // tokens of a router row's pass
+constexpr int kRouteCtas = 8;   // CTAs (a cluster) that compute the logits
 
-// Activation records of rows x nsb units (one warp each) and, in the first
-// nlog CTAs, the router's logits.  Two experts' logits may lie arbitrarily
-// close, and a pick that flips changes the output by whole experts: products
-// of f32 are exact in f64, and the sums are f64.  The f64 units do 64 FMA per
-// SM and cycle; 16 tokens, 128 experts and K = 2048 take under half a
-// microsecond of them.
+// Activation records of rows x nsb units, one warp each.
 template <typename T>
-__global__ void __launch_bounds__(kPrepThreads) qmm_prep_kernel(const T* __restrict__ x, int rows, int64_t K, int nsb,
-                                                               int order, uint8_t* __restrict__ recs,
-                                                               const float* __restrict__ router, int E,
-                                                               double* __restrict__ logits, int nlog) {
-  qmm_dep_wait();
-  qmm_dep_launch();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if constexpr (sizeof(T) == 4) {
-    if ((int)blockIdx.x < nlog) {
-      __shared__ double part[kQmmWarps][kRouteTok];
-      const int e = blockIdx.x % E, m0 = (blockIdx.x / E) * kRouteTok;
-      const int mc = min(kRouteTok, rows - m0);
-      double acc[kRouteTok] = {};
-      const float* w = router + (int64_t)e * K;
-      const bool wide = ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(x)) & 15) == 0;  // K % 32 == 0
-      for (int64_t k = 4 * threadIdx.x; k < K; k += 4 * kPrepThreads) {
-        float4 a;
-        if (wide) {
-          a = *reinterpret_cast<const float4*>(w + k);
-        } else {
-          a = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
-        }
-        const double a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w;
-#pragma unroll
-        for (int t = 0; t < kRouteTok; ++t) {
-          if (t < mc) {
-            const T* xr = x + (int64_t)(m0 + t) * K + k;
-            float4 b;
-            if (wide) {
-              b = *reinterpret_cast<const float4*>(xr);
-            } else {
-              b = make_float4(xr[0], xr[1], xr[2], xr[3]);
-            }
-            acc[t] = fma(a0, (double)b.x, fma(a1, (double)b.y, fma(a2, (double)b.z, fma(a3, (double)b.w, acc[t]))));
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < kRouteTok; ++t) {
-        if (t < mc) {
-          double v = acc[t];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          if (lane == 0) part[warp][t] = v;
-        }
-      }
-      __syncthreads();
-      if ((int)threadIdx.x < mc) {
-        double v = 0.0;
-        for (int i = 0; i < kQmmWarps; ++i) v += part[i][threadIdx.x];
-        logits[(int64_t)(m0 + threadIdx.x) * E + e] = v;
-      }
-      return;
-    }
-  }
-  const int64_t job = (int64_t)(blockIdx.x - nlog) * kQmmWarps + warp;
-  if (job >= (int64_t)rows * nsb) return;
+__device__ __forceinline__ void make_records(const T* __restrict__ x, int64_t rows, int64_t K, int nsb, int order,
+                                             uint8_t* __restrict__ recs, int64_t block) {
+  const int64_t job = block * kQmmWarps + (threadIdx.x >> 5);
+  if (job >= rows * nsb) return;
   const int64_t row = job / nsb;
   const int sb = (int)(job - row * nsb);
-  qmm_make_record(x + row * K + 256 * sb, (int)min((int64_t)256, K - 256 * sb), order, recs + job * kQmmRec, lane);
+  qmm_make_record(x + row * K + 256 * sb, (int)min((int64_t)256, K - 256 * sb), order, recs + job * kQmmRec,
+                  threadIdx.x & 31);
 }
 
 template <typename T>
-static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* recs, const float* router, int E,
-                       double* logits, cudaStream_t st) {
+__global__ void __launch_bounds__(kPrepThreads) qmm_prep_kernel(const T* __restrict__ x, int64_t rows, int64_t K,
+                                                                int nsb, int order, uint8_t* __restrict__ recs) {
+  qmm_dep_wait();
+  qmm_dep_launch();
+  make_records(x, rows, K, nsb, order, recs, blockIdx.x);
+}
+
+// First kernel of a mixture-of-experts call: the first cluster computes the
+// router's logits, picks the experts and lists the picks by expert; the other
+// CTAs prepare the activation records.  Two experts' logits may lie
+// arbitrarily close, and a pick that flips changes the output by whole
+// experts: products of f32 are exact in f64, and the sums are f64.  One
+// cluster, because its barrier lets one kernel do it all: a grid-wide
+// computation of the logits needs a second launch, or every CTA of the next
+// kernel building the lists for itself (about 8 us of its start).
+__global__ void __launch_bounds__(kPrepThreads) moe_route_kernel(const __grid_constant__ QmmParams p,
+                                                                 const float* __restrict__ x,
+                                                                 const float* __restrict__ router, int64_t K, int order,
+                                                                 uint8_t* __restrict__ recs, double* __restrict__ logits) {
+  extern __shared__ __align__(16) int32_t route_mem[];
+  __shared__ double part[kQmmWarps * NSQ_MOE_MAX_TOKENS];  // [K share][expert][token]: KS * ne <= 8
+  qmm_dep_wait();
+  qmm_dep_launch();
+  if (blockIdx.x >= kRouteCtas) {
+    make_records(x, p.M, K, p.nsb, order, recs, blockIdx.x - kRouteCtas);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x;
+  if (router) {
+    // experts rank, rank + 8, ...; with few of them several warps share one's K
+    const int ne = p.E > rank ? (p.E - rank + kRouteCtas - 1) / kRouteCtas : 0;
+    const int KS = p.E <= kRouteCtas ? 8 : p.E <= 2 * kRouteCtas ? 4 : p.E <= 4 * kRouteCtas ? 2 : 1;
+    const int ks = warp % KS;
+    const bool wide = ((reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(x)) & 15) == 0;  // K % 32 == 0
+    for (int i = warp / KS; i < ne; i += kQmmWarps / KS) {
+      const float* w = router + (int64_t)(rank + kRouteCtas * i) * K;
+      for (int m0 = 0; m0 < p.M; m0 += kRouteTok) {
+        const int mc = min(kRouteTok, p.M - m0);
+        double acc[kRouteTok] = {};
+        for (int64_t k = 4 * (lane + 32 * ks); k < K; k += 128 * KS) {
+          float4 a;
+          if (wide) {
+            a = *reinterpret_cast<const float4*>(w + k);
+          } else {
+            a = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+          }
+          const double a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w;
+#pragma unroll
+          for (int t = 0; t < kRouteTok; ++t) {
+            if (t < mc) {
+              const float* xr = x + (int64_t)(m0 + t) * K + k;
+              float4 b;
+              if (wide) {
+                b = *reinterpret_cast<const float4*>(xr);
+              } else {
+                b = make_float4(xr[0], xr[1], xr[2], xr[3]);
+              }
+              acc[t] = fma(a0, (double)b.x, fma(a1, (double)b.y, fma(a2, (double)b.z, fma(a3, (double)b.w, acc[t]))));
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kRouteTok; ++t) {
+          if (t < mc) {
+            double v = acc[t];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == 0) {
+              if (KS == 1) {
+                logits[(int64_t)(m0 + t) * p.E + rank + kRouteCtas * i] = v;
+              } else {
+                part[(ks * ne + i) * p.M + m0 + t] = v;
+              }
+            }
+          }
+        }
+      }
+    }
+    if (KS > 1) {
+      __syncthreads();
+      for (int q = threadIdx.x; q < ne * p.M; q += kPrepThreads) {
+        const int i = q / p.M, m = q - i * p.M;
+        double v = part[q];
+        for (int k = 1; k < KS; ++k) v += part[k * ne * p.M + q];
+        logits[(int64_t)m * p.E + rank + kRouteCtas * i] = v;
+      }
+    }
+    qmm_cluster_sync();  // the logits of every rank, seen by rank 0
+  }
+  if (rank == 0) qmm_build_lists(p, route_mem);
+}
+
+template <typename T>
+static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* recs, cudaStream_t st) {
   const int nsb = (int)((K + 255) / 256);
-  const int nlog = router ? E * (int)((rows + kRouteTok - 1) / kRouteTok) : 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(nlog + (rows * nsb + kQmmWarps - 1) / kQmmWarps));
+  cfg.gridDim = dim3((unsigned)((rows * nsb + kQmmWarps - 1) / kQmmWarps));
   cfg.blockDim = dim3(kPrepThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -103,26 +138,47 @@ static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   note_launch();
-  return cudaLaunchKernelEx(&cfg, qmm_prep_kernel<T>, x, (int)rows, K, nsb, order, recs, router, E, logits, nlog) ==
-                 cudaSuccess
-             ? NSQ_OK
-             : NSQ_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, qmm_prep_kernel<T>, x, rows, K, nsb, order, recs) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
+}
+
+// The grid is whole clusters: cluster 0 routes, the rest make records.
+static int launch_route(const QmmParams& p, const float* x, const float* router, int64_t K, int order, uint8_t* recs,
+                        double* logits, cudaStream_t st) {
+  const int64_t P = (int64_t)p.M * p.top_k;
+  const int64_t rec_ctas = ((int64_t)p.M * p.nsb + kQmmWarps - 1) / kQmmWarps;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(kRouteCtas + (rec_ctas + kRouteCtas - 1) / kRouteCtas * kRouteCtas));
+  cfg.blockDim = dim3(kPrepThreads);
+  cfg.dynamicSmemBytes = (size_t)P * (8 + sizeof(QmmGroup));  // at most 24 KB
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kRouteCtas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  note_launch();
+  return cudaLaunchKernelEx(&cfg, moe_route_kernel, p, x, router, K, order, recs, logits) == cudaSuccess ? NSQ_OK
+                                                                                                          : NSQ_ERR_CUDA;
 }
 
 struct QmmShape {
   int CB, PA, PG, MT;
 };
 template <int TYPE>
-static constexpr QmmShape shape_t() {
-  return {QmmFmt<TYPE>::CB, QmmFmt<TYPE>::PA, QmmFmt<TYPE>::PG, QmmFmt<TYPE>::MT};
+static constexpr QmmShape shape_t(int TS) {
+  return {QmmFmt<TYPE>::CB, QmmFmt<TYPE>::PA, QmmFmt<TYPE>::PG, qmm_tiles<TYPE>(TS)};
 }
-static QmmShape qmm_shape(int type) {
+static QmmShape qmm_shape(int type, int TS) {
   switch (type) {
-    case NSQ_TYPE_Q4_K: return shape_t<NSQ_TYPE_Q4_K>();
-    case NSQ_TYPE_Q5_K: return shape_t<NSQ_TYPE_Q5_K>();
-    case NSQ_TYPE_Q6_K: return shape_t<NSQ_TYPE_Q6_K>();
-    case NSQ_TYPE_Q4_0: return shape_t<NSQ_TYPE_Q4_0>();
-    default: return shape_t<NSQ_TYPE_Q8_0>();
+    case NSQ_TYPE_Q4_K: return shape_t<NSQ_TYPE_Q4_K>(TS);
+    case NSQ_TYPE_Q5_K: return shape_t<NSQ_TYPE_Q5_K>(TS);
+    case NSQ_TYPE_Q6_K: return shape_t<NSQ_TYPE_Q6_K>(TS);
+    case NSQ_TYPE_Q4_0: return shape_t<NSQ_TYPE_Q4_0>(TS);
+    default: return shape_t<NSQ_TYPE_Q8_0>(TS);
   }
 }
 
@@ -154,7 +210,7 @@ static bool encode_rows(CUtensorMap* map, const uint8_t* w, int64_t rows, int64_
 
 // Plans and launches one product.  groups: the most groups there can be.
 static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream_t st, int num_sms) {
-  const QmmShape f = qmm_shape(type);
+  const QmmShape f = qmm_shape(type, p.TS);
   // columns of K per CTA: the records of a unit are read by the RW = 8 / KW
   // warps that share it, so more tokens want more rows per unit
   int KW = p.TS <= 2 ? 8 : p.TS <= 4 ? 4 : p.TS <= 8 ? 2 : 1;
@@ -176,7 +232,7 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
   const int64_t rows = p.wbytes / p.rb;
   p.rows_aligned = p.rb % 16 == 0 && rows <= 0x7FFFFFFF;
   if (p.rows_aligned) {
-    const int box_rows = p.RW * f.MT * (p.mode == kQmmUp ? 8 : 16);
+    const int box_rows = f.MT * (p.mode == kQmmUp ? 8 : 16);
     if (!encode_rows(&maps[0], p.w0, rows, p.rb, box_rows, f.PA)) p.rows_aligned = 0;
     if (p.mode == kQmmUp && !encode_rows(&maps[1], p.w1, rows, p.rb, box_rows, f.PA)) p.rows_aligned = 0;
   }
@@ -195,7 +251,7 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
   const size_t ring = p.stages * p.KW * slot;
   if (in_ring && ys > ring) return NSQ_ERR_SHAPE;
   const size_t smem = fixed + sums + ring;
-  if (smem > (size_t)kQmmSmemMax || ring < (size_t)P * 8) return NSQ_ERR_SHAPE;
+  if (smem > (size_t)kQmmSmemMax) return NSQ_ERR_SHAPE;
   const int64_t tasks = tiles * (p.mode == kQmmUp ? groups : 1);
   const int64_t grid = (p.split > 1 || tasks < slots ? tasks : slots) * p.split;
   switch (type) {
@@ -213,7 +269,7 @@ static bool act_ok(int act) { return act >= NSQ_ACT_NONE && act <= NSQ_ACT_RELU;
 
 // Workspace of a mixture-of-experts call, in this order.
 struct MoeSpace {
-  size_t logits, recs_x, h, recs_h, groups, plist, pwts, ngroups, total;
+  size_t logits, recs_x, h, recs_h, groups, plist, pwts, ptok, ngroups, total;
 };
 static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t top_k) {
   MoeSpace s{};
@@ -231,6 +287,7 @@ static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t to
   s.groups = take((size_t)P * sizeof(QmmGroup));
   s.plist = take((size_t)P * 4);
   s.pwts = take((size_t)P * 4);
+  s.ptok = take((size_t)P * 4);
   s.ngroups = take(4);
   s.total = at;
   return s;
@@ -269,12 +326,12 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   double* logits = reinterpret_cast<double*>(ws + s.logits);
-  if ((rc = launch_prep(x, M, D, qmm_order(moe->type_in, moe->layout_in), ws + s.recs_x, w_router, (int)E, logits, st)))
-    return rc;
   QmmParams p{};
   p.M = (int)M;
   p.top_k = (int)top_k;
-  p.TS = (int)(M < kQmmMaxTok ? M : kQmmMaxTok);
+  // tokens of a group: 16, or 8 where an expert has 4 or fewer on average
+  const int64_t cap = M * top_k <= 4 * E ? 8 : kQmmMaxTok;
+  p.TS = (int)(M < cap ? M : cap);
   p.E = (int)E;
   p.score = w_router ? score : -1;
   p.logits = logits;
@@ -285,6 +342,7 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   p.groups = reinterpret_cast<QmmGroup*>(ws + s.groups);
   p.plist = reinterpret_cast<int32_t*>(ws + s.plist);
   p.pwts = reinterpret_cast<float*>(ws + s.pwts);
+  p.ptok = reinterpret_cast<int32_t*>(ws + s.ptok);
   p.ngroups = reinterpret_cast<int32_t*>(ws + s.ngroups);
   p.act = moe->act;
   p.dtype = NSQ_OUT_F32;
@@ -302,10 +360,11 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   p.w1 = static_cast<const uint8_t*>(moe->w_up);
   p.wbytes = E * F * p.rb;
   p.recs = ws + s.recs_x;
+  if ((rc = launch_route(p, x, w_router, D, qmm_order(moe->type_in, moe->layout_in), ws + s.recs_x, logits, st)))
+    return rc;
   if ((rc = run_qmm(p, moe->type_in, moe->layout_in, P, st, num_sms))) return rc;
 
-  if ((rc = launch_prep(static_cast<const float*>(p.h), P, F, qmm_order(moe->type_down, moe->layout_down), ws + s.recs_h,
-                        nullptr, 0, nullptr, st)))
+  if ((rc = launch_prep(static_cast<const float*>(p.h), P, F, qmm_order(moe->type_down, moe->layout_down), ws + s.recs_h, st)))
     return rc;
 
   p.mode = kQmmDown;
@@ -355,8 +414,8 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   uint8_t* recs = static_cast<uint8_t*>(workspace);
   const int order = qmm_order(ggml_type, q6k_layout);
   rc = dtype == NSQ_OUT_F32
-           ? launch_prep(static_cast<const float*>(x), M, K, order, recs, nullptr, 0, nullptr, st)
-           : launch_prep(static_cast<const __nv_bfloat16*>(x), M, K, order, recs, nullptr, 0, nullptr, st);
+           ? launch_prep(static_cast<const float*>(x), M, K, order, recs, st)
+           : launch_prep(static_cast<const __nv_bfloat16*>(x), M, K, order, recs, st);
   if (rc) return rc;
   QmmParams p{};
   p.mode = kQmmLinear;
