@@ -40,6 +40,10 @@ __global__ void __launch_bounds__(kPrepThreads) qmm_prep_kernel(const T* __restr
   make_records(x, rows, K, nsb, order, recs, blockIdx.x);
 }
 
+__device__ __forceinline__ float4 load4(const float* p, bool wide) {
+  return wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+}
+
 // First kernel of a mixture-of-experts call: the first cluster computes the
 // router's logits, picks the experts and lists the picks by expert; the other
 // CTAs prepare the activation records.  Two experts' logits may lie
@@ -58,6 +62,10 @@ __global__ void __launch_bounds__(kPrepThreads) moe_route_kernel(const __grid_co
   qmm_dep_launch();
   if (blockIdx.x >= kRouteCtas) {
     make_records(x, p.M, K, p.nsb, order, recs, blockIdx.x - kRouteCtas);
+    const int64_t counters = (int64_t)p.M * p.top_k * ((p.n + 255) / 256);
+    for (int64_t i = (int64_t)(blockIdx.x - kRouteCtas) * kPrepThreads + threadIdx.x; i < counters;
+         i += (int64_t)(gridDim.x - kRouteCtas) * kPrepThreads)
+      p.done[i] = 0;
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x;
@@ -72,25 +80,29 @@ __global__ void __launch_bounds__(kPrepThreads) moe_route_kernel(const __grid_co
       for (int m0 = 0; m0 < p.M; m0 += kRouteTok) {
         const int mc = min(kRouteTok, p.M - m0);
         double acc[kRouteTok] = {};
-        for (int64_t k = 4 * (lane + 32 * ks); k < K; k += 128 * KS) {
-          float4 a;
-          if (wide) {
-            a = *reinterpret_cast<const float4*>(w + k);
-          } else {
-            a = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+        // eight 16-byte loads of the row are in flight: one at a time, a row of
+        // 2048 took 11 us
+        for (int64_t k0 = 4 * (lane + 32 * ks); k0 < K; k0 += 8 * 128 * KS) {
+          float4 a[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int64_t k = k0 + 128 * KS * q;
+            a[q] = k < K ? load4(w + k, wide) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           }
-          const double a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w;
 #pragma unroll
           for (int t = 0; t < kRouteTok; ++t) {
             if (t < mc) {
-              const float* xr = x + (int64_t)(m0 + t) * K + k;
-              float4 b;
-              if (wide) {
-                b = *reinterpret_cast<const float4*>(xr);
-              } else {
-                b = make_float4(xr[0], xr[1], xr[2], xr[3]);
+              float4 b[8];
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const int64_t k = k0 + 128 * KS * q;
+                b[q] = k < K ? load4(x + (int64_t)(m0 + t) * K + k, wide) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               }
-              acc[t] = fma(a0, (double)b.x, fma(a1, (double)b.y, fma(a2, (double)b.z, fma(a3, (double)b.w, acc[t]))));
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                acc[t] = fma((double)a[q].x, (double)b[q].x,
+                             fma((double)a[q].y, (double)b[q].y,
+                                 fma((double)a[q].z, (double)b[q].z, fma((double)a[q].w, (double)b[q].w, acc[t]))));
             }
           }
         }
@@ -211,47 +223,69 @@ static bool encode_rows(CUtensorMap* map, const uint8_t* w, int64_t rows, int64_
 // Plans and launches one product.  groups: the most groups there can be.
 static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream_t st, int num_sms) {
   const QmmShape f = qmm_shape(type, p.TS);
-  // columns of K per CTA: the records of a unit are read by the RW = 8 / KW
-  // warps that share it, so more tokens want more rows per unit
-  int KW = p.TS <= 2 ? 8 : p.TS <= 4 ? 4 : p.TS <= 8 ? 2 : 1;
   const int64_t most_units = p.mode == kQmmDown ? groups * p.nsb : p.nsb;
-  while (KW > 1 && KW / 2 >= most_units) KW /= 2;
-  p.KW = KW;
-  p.RW = kQmmWarps / KW;
-  const int64_t tile_rows = (p.mode == kQmmUp ? 8 : 16) * f.MT * p.RW;
-  const int64_t tiles = (p.n + tile_rows - 1) / tile_rows;
   const int64_t slots = 2 * (int64_t)num_sms;
-  p.split = 1;
-  if (p.mode != kQmmUp) {
-    // a K split over a cluster while the tiles leave half of the CTA slots
-    // empty and every CTA keeps a unit per column
-    while (p.split < 8 && tiles * p.split * 2 <= slots && most_units >= (int64_t)p.split * 2 * KW) p.split *= 2;
+  const int P = p.mode == kQmmLinear ? 0 : p.M * p.top_k;
+  const size_t fixed = kQmmCtl + kQmmRec + qmm_lists_bytes(P);
+  const size_t ys = (size_t)kQmmWarps * p.YC * 16 * f.MT * 4;
+  const int pitch = p.rb % 16 == 0 ? f.PA : f.PG;
+  // Columns of K per CTA (KW), the rest of the 8 warps being row tiles: the
+  // choice with the least time by a simple model.  A CTA's work is its rounds
+  // of tiles x the bytes of a tile, the records of a unit being fetched once
+  // for its RW row tiles; a K split over a cluster fills CTA slots that the
+  // tiles leave empty, as long as every column keeps a unit.
+  double best = 0;
+  size_t smem = 0;
+  for (int KW = 1; KW <= kQmmWarps; KW *= 2) {
+    if (KW > 1 && KW / 2 >= most_units) break;
+    QmmParams t = p;
+    t.KW = KW;
+    t.RW = kQmmWarps / KW;
+    const int64_t rows = (int64_t)(p.mode == kQmmUp ? 8 : 16) * f.MT * t.RW;
+    const int64_t tiles = (p.n + rows - 1) / rows;
+    t.split = 1;
+    if (p.mode != kQmmUp)
+      while (t.split < 8 && tiles * t.split * 2 <= slots && most_units >= (int64_t)t.split * 2 * KW) t.split *= 2;
+    const size_t slot = qmm_slot_bytes(t.RW * f.MT, pitch, p.TS);
+    const bool in_ring = p.mode != kQmmDown && t.split > 1;
+    // buffers of partial sums: none where one column holds the whole K, two so
+    // that a task's are joined while the next one runs
+    t.PB = p.mode != kQmmDown && t.split == 1 && KW == 1 ? 0 : t.split > 1 ? 1 : 2;
+    if (p.mode == kQmmDown && t.PB == 2 && fixed + 2 * ys + 2 * KW * slot > (size_t)kQmmSmemHalf) t.PB = 1;
+    const size_t sums = (in_ring ? 0 : p.mode == kQmmUp && t.PB == 0 ? 1 : t.PB) * ys;
+    t.stages = kQmmMaxStages;
+    while (t.stages > 2 && fixed + sums + t.stages * KW * slot > (size_t)kQmmSmemHalf) --t.stages;
+    const size_t need = fixed + sums + t.stages * KW * slot;
+    if (need > (size_t)kQmmSmemMax || (in_ring && ys > t.stages * KW * slot)) continue;
+    const int64_t here = need > (size_t)kQmmSmemHalf ? num_sms : slots;  // CTAs at a time
+    // (of the most groups there can be, an expert's share of the picks are fewer)
+    const int64_t ctas = tiles * (p.mode == kQmmUp ? (groups < p.E ? groups : p.E) : 1) * t.split;
+    const int64_t rounds = (ctas + here - 1) / here;
+    const double bytes = 16.0 * f.MT * t.RW * pitch + (p.TS < 4 ? p.TS : 0.5 * p.TS) * kQmmRec;
+    const double time = (double)rounds / t.split * bytes * (here == slots ? 1.0 : 0.6);
+    if (smem == 0 || time < best) {
+      best = time;
+      smem = need;
+      p.KW = t.KW;
+      p.RW = t.RW;
+      p.split = t.split;
+      p.PB = t.PB;
+      p.stages = t.stages;
+    }
   }
+  if (smem == 0) return NSQ_ERR_SHAPE;
+  const int64_t tile_rows = (int64_t)(p.mode == kQmmUp ? 8 : 16) * f.MT * p.RW;
+  const int64_t tiles = (p.n + tile_rows - 1) / tile_rows;
   // TMA boxes where every row starts 16-byte aligned (experts and tensors then do too)
   alignas(64) CUtensorMap maps[2] = {};
   const int64_t rows = p.wbytes / p.rb;
-  p.rows_aligned = p.rb % 16 == 0 && rows <= 0x7FFFFFFF;
+  p.rows_aligned = p.rb % 16 == 0;
   if (p.rows_aligned) {
+    if (rows > 0x7FFFFFFF) return NSQ_ERR_SHAPE;
     const int box_rows = f.MT * (p.mode == kQmmUp ? 8 : 16);
-    if (!encode_rows(&maps[0], p.w0, rows, p.rb, box_rows, f.PA)) p.rows_aligned = 0;
-    if (p.mode == kQmmUp && !encode_rows(&maps[1], p.w1, rows, p.rb, box_rows, f.PA)) p.rows_aligned = 0;
+    if (!encode_rows(&maps[0], p.w0, rows, p.rb, box_rows, f.PA)) return NSQ_ERR_CUDA;
+    if (p.mode == kQmmUp && !encode_rows(&maps[1], p.w1, rows, p.rb, box_rows, f.PA)) return NSQ_ERR_CUDA;
   }
-  const int P = p.mode == kQmmLinear ? 0 : p.M * p.top_k;
-  const size_t slot = qmm_slot_bytes(p.RW * f.MT, p.rows_aligned ? f.PA : f.PG, p.TS);
-  const size_t ys = (size_t)kQmmWarps * p.YC * 16 * f.MT * 4;
-  const bool in_ring = p.mode != kQmmDown && p.split > 1;
-  // buffers of partial sums: none where one column holds the whole K, two so
-  // that a task's are joined while the next one runs
-  p.PB = p.mode != kQmmDown && p.split == 1 && KW == 1 ? 0 : p.split > 1 ? 1 : 2;
-  const size_t fixed = kQmmCtl + kQmmRec + qmm_lists_bytes(P);
-  if (p.mode == kQmmDown && p.PB == 2 && fixed + 2 * ys + 2 * p.KW * slot > (size_t)kQmmSmemHalf) p.PB = 1;
-  const size_t sums = in_ring ? 0 : p.PB * ys;
-  p.stages = kQmmMaxStages;
-  while (p.stages > 2 && fixed + sums + p.stages * p.KW * slot > (size_t)kQmmSmemHalf) --p.stages;
-  const size_t ring = p.stages * p.KW * slot;
-  if (in_ring && ys > ring) return NSQ_ERR_SHAPE;
-  const size_t smem = fixed + sums + ring;
-  if (smem > (size_t)kQmmSmemMax) return NSQ_ERR_SHAPE;
   const int64_t tasks = tiles * (p.mode == kQmmUp ? groups : 1);
   const int64_t grid = (p.split > 1 || tasks < slots ? tasks : slots) * p.split;
   switch (type) {
@@ -269,7 +303,7 @@ static bool act_ok(int act) { return act >= NSQ_ACT_NONE && act <= NSQ_ACT_RELU;
 
 // Workspace of a mixture-of-experts call, in this order.
 struct MoeSpace {
-  size_t logits, recs_x, h, recs_h, groups, plist, pwts, ptok, ngroups, total;
+  size_t logits, recs_x, h, recs_h, groups, plist, pwts, ptok, ngroups, done, total;
 };
 static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t top_k) {
   MoeSpace s{};
@@ -289,6 +323,7 @@ static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t to
   s.pwts = take((size_t)P * 4);
   s.ptok = take((size_t)P * 4);
   s.ngroups = take(4);
+  s.done = take((size_t)(P * units_of(F)) * 4);
   s.total = at;
   return s;
 }
@@ -347,6 +382,9 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   p.act = moe->act;
   p.dtype = NSQ_OUT_F32;
   p.h = reinterpret_cast<float*>(ws + s.h);
+  p.recs_h = ws + s.recs_h;
+  p.done = reinterpret_cast<int32_t*>(ws + s.done);
+  p.order_h = qmm_order(moe->type_down, moe->layout_down);
   const int64_t P = M * top_k;
 
   p.mode = kQmmUp;
@@ -363,9 +401,6 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   if ((rc = launch_route(p, x, w_router, D, qmm_order(moe->type_in, moe->layout_in), ws + s.recs_x, logits, st)))
     return rc;
   if ((rc = run_qmm(p, moe->type_in, moe->layout_in, P, st, num_sms))) return rc;
-
-  if ((rc = launch_prep(static_cast<const float*>(p.h), P, F, qmm_order(moe->type_down, moe->layout_down), ws + s.recs_h, st)))
-    return rc;
 
   p.mode = kQmmDown;
   p.YC = p.M;

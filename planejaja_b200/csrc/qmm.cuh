@@ -4,19 +4,20 @@
 //
 //   out[t, n] = sum_k x[t, k] * W[n, k]         t: up to 16 tokens of a group
 //
-// Mathematics.  x = s X with integers |X| < 2^30 and one power of two s per
-// (token, 256 of K); X is four signed bytes ("limbs", X = sum 256^l X_l, each
+// Mathematics.  x = s X with integers |X| < 2^23 and one scale s per (token,
+// 256 of K); X is three signed bytes ("limbs", X = sum 256^l X_l, each
 // -128..127).  The formats' integers meet the limbs in mma.sync m16n8k32 / k16
-// (u8 x s8, exact s32 sums): 16 weight rows as A, two tokens of four limbs as
-// the eight columns of B.  The integer scale of a group multiplies its sum in
-// s32 too, so the first rounding comes after 256 weights:
+// (u8 x s8, exact s32 sums): 16 weight rows as A and eight columns as B,
+// which are two tokens of four limbs (the fourth is zero) or, from five tokens
+// on, one limb of eight tokens.  The integer scale of a group multiplies its
+// sum in s32 too, so the first rounding comes after 256 weights:
 //   Q4_K, Q5_K  sum sc_j (sum q X_l): |sum| < 2^29;  d times it in f32.  The
 //               mins enter through the limb sums T of 16 activations (at most
 //               2048, exact in fp16):  - dmin * sum m T  by one fp16 MMA
 //   Q6_K        the same with 16-weight groups; q - 32 through T
 //   Q4_0, Q8_0  one f32 scale per 32 weights; q - 8 through T
-// A limb's f32 value is off by 2^-24 of the limb's sum, the top limb's is all
-// that is seen: norm errors of a product are about 2e-7.
+// An activation is off by at most max / 2^24 of its 256, a limb's f32 value by
+// 2^-24 of the limb's sum: norm errors of a product are about 2e-7.
 //
 // Measured on B200: the byte MMA (4096 products), the fp16 MMA (2048), take 8
 // cycles of a scheduler each; logic, permutes, IMAD and fp16x2 take 2.  A
@@ -50,17 +51,20 @@ namespace nsq {
 
 // ---------------------------------------------------------------------------
 // Prepared activations: one record per (row, 256 of K).
-//   [0, 1024)     four limbs of 256 bytes: 16-byte unit 4i + c = the operands
-//                 of lane c of each quad in turn i; units of odd limbs are
-//                 exchanged (^ 4), so that the limbs of a token, which
-//                 neighbouring lanes read, lie in different banks
-//   [1024, 1152)  T, the sums of 16 consecutive X_l, as fp16: per limb and
-//                 lane c the groups 2c, 2c+1, 2c+8, 2c+9
-//   [1152, 1156)  s (NaN when a value is not finite)
-// Which k a place holds goes by the format of the weights (QmmOrder).
-constexpr int kQmmRec = 1168;
-constexpr int kQmmRecT = 1024;
-constexpr int kQmmRecS = 1152;
+//   [0, 768)    three limbs of 256 bytes: 16-byte unit 4i + c = the operands
+//               of lane c of each quad in turn i; units of the middle limb are
+//               exchanged (^ 4), so that neighbouring limbs of a token, which
+//               neighbouring lanes read, lie in different banks
+//   [768, 864)  T, the sums of 16 consecutive X_l, as fp16: per limb and lane
+//               c the groups 2c, 2c+1, 2c+8, 2c+9
+//   [864, 868)  s (NaN when a value is not finite)
+// Which k a place holds goes by the format of the weights (QmmOrder).  In
+// shared memory records lie 960 bytes apart: neighbouring tokens then are in
+// different banks too.
+constexpr int kQmmRec = 880;
+constexpr int kQmmRecPitch = 960;
+constexpr int kQmmRecT = 768;
+constexpr int kQmmRecS = 864;
 constexpr int kQmmWarps = 8;
 constexpr int kQmmThreads = 32 * kQmmWarps;
 constexpr int kQmmMaxStages = 4;
@@ -96,10 +100,10 @@ __device__ __forceinline__ void qmm_runs(int order, int i, int c, int h, int& k0
 __device__ __forceinline__ uint32_t qmm_h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 qmm_u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// One warp turns 256 values (those at and after `valid` count as 0) into a record.
-template <typename T>
-__device__ __forceinline__ void qmm_make_record(const T* __restrict__ src, int valid, int order, uint8_t* rec,
-                                                int lane) {
+// One warp turns 256 values (those at and after `valid` count as 0) into a
+// record.  FRESH: values that other CTAs of this kernel wrote, read from L2.
+template <typename T, bool FRESH = false>
+__device__ __forceinline__ void qmm_make_record(const T* src, int valid, int order, uint8_t* rec, int lane) {
   const int i = lane >> 3, c = (lane >> 1) & 3, h = lane & 1;
   int k[2];
   qmm_runs(order, i, c, h, k[0], k[1]);
@@ -109,11 +113,13 @@ __device__ __forceinline__ void qmm_make_record(const T* __restrict__ src, int v
     if constexpr (sizeof(T) == 4) {
       const bool wide = ((reinterpret_cast<uintptr_t>(src) & 15) == 0) && k[r] + 4 <= valid;
       if (wide) {
-        const float4 f = *reinterpret_cast<const float4*>(src + k[r]);
+        const float4* q = reinterpret_cast<const float4*>(src + k[r]);
+        const float4 f = FRESH ? __ldcg(q) : *q;
         v[4 * r] = f.x; v[4 * r + 1] = f.y; v[4 * r + 2] = f.z; v[4 * r + 3] = f.w;
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * r + e] = k[r] + e < valid ? (float)src[k[r] + e] : 0.0f;
+        for (int e = 0; e < 4; ++e)
+          v[4 * r + e] = k[r] + e < valid ? (FRESH ? __ldcg(src + k[r] + e) : src[k[r] + e]) : 0.0f;
       }
     } else {
 #pragma unroll
@@ -124,42 +130,52 @@ __device__ __forceinline__ void qmm_make_record(const T* __restrict__ src, int v
 #pragma unroll
   for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
   mx = __reduce_max_sync(0xffffffffu, mx);
-  // exponent field E of the largest: s = 2^(E - 156), so that |X| < 2^30.  s
-  // may be subnormal; 1 / s may not overflow, so small values are scaled twice.
-  // Below 2^-120 the scale stays and values lose bits at 2^-149.
-  const int E = min(max((int)(mx >> 23), 7), 254);
-  float s = E >= 30 ? __uint_as_float((uint32_t)(E - 29) << 23) : __uint_as_float(1u << (E - 7));
+  // the largest value becomes kTop, one below the largest X = 127 (256^2 + 256
+  // + 1): its product with the rounded 1 / s may be half above.
+  // Values below 2^-63 get a power of two instead (s may be subnormal, and
+  // exact; 1 / s may not overflow, so they are scaled twice), with |X| < 2^22;
+  // below 2^-120 it stays and values lose bits at 2^-141.
+  constexpr float kTop = 8355710.0f;
+  const int E = (int)(mx >> 23);
+  float s, pre, inv;
+  if (E >= 64) {
+    const float m = __uint_as_float(mx);
+    pre = 1.0f;
+    inv = kTop / m;
+    s = m / kTop;
+  } else {
+    const int F = max(E, 7);  // s = 2^(F - 148)
+    pre = 18446744073709551616.0f;  // 2^64
+    inv = __uint_as_float((uint32_t)(127 + 148 - 64 - F) << 23);
+    s = F >= 22 ? __uint_as_float((uint32_t)(F - 21) << 23) : __uint_as_float(1u << (F + 1));
+  }
   if (mx >= 0x7F800000u) s = __uint_as_float(0x7FC00000u);  // infinity or NaN: this token alone is spoilt
-  const float pre = E < 64 ? 18446744073709551616.0f : 1.0f;  // 2^64
-  const float inv = __uint_as_float((uint32_t)(283 - (E < 64 ? E + 64 : E)) << 23);
-  int sum[2][4];
-  uint32_t limb[2][4];
+  int sum[2][3];
+  uint32_t limb[2][3];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     uint32_t y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int X = __float2int_rn((v[4 * r + e] * pre) * inv);
-      y[e] = ((uint32_t)X + 0x00808080u) ^ 0x00808080u;  // the bytes are the limbs
+      y[e] = ((uint32_t)X + 0x00008080u) ^ 0x00008080u;  // bytes 0, 1, 2 are the limbs
     }
     // transpose: byte l of the four words
     const uint32_t a = __byte_perm(y[0], y[1], 0x5140), b = __byte_perm(y[2], y[3], 0x5140);
-    const uint32_t d = __byte_perm(y[0], y[1], 0x7362), f = __byte_perm(y[2], y[3], 0x7362);
     limb[r][0] = __byte_perm(a, b, 0x5410);
     limb[r][1] = __byte_perm(a, b, 0x7632);
-    limb[r][2] = __byte_perm(d, f, 0x5410);
-    limb[r][3] = __byte_perm(d, f, 0x7632);
+    limb[r][2] = __byte_perm(__byte_perm(y[0], y[1], 0x0062), __byte_perm(y[2], y[3], 0x0062), 0x5410);
 #pragma unroll
-    for (int l = 0; l < 4; ++l) sum[r][l] = dp4a_ss(limb[r][l], 0x01010101u, 0);
+    for (int l = 0; l < 3; ++l) sum[r][l] = dp4a_ss(limb[r][l], 0x01010101u, 0);
   }
 #pragma unroll
-  for (int l = 0; l < 4; ++l)
+  for (int l = 0; l < 3; ++l)
     *reinterpret_cast<uint2*>(rec + 256 * l + 16 * ((4 * i + c) ^ (4 * (l & 1))) + 8 * h) =
         make_uint2(limb[0][l], limb[1][l]);
   // T: in the K45 order the lane's 8 values and its neighbour's (c ^ 1) are a
   // group; else each run is a quarter of one, over c
 #pragma unroll
-  for (int l = 0; l < 4; ++l) {
+  for (int l = 0; l < 3; ++l) {
     int t0 = order == kOrdK45 ? sum[0][l] + sum[1][l] : sum[0][l], t1 = sum[1][l];
     t0 += __shfl_xor_sync(0xffffffffu, t0, 2);
     t1 += __shfl_xor_sync(0xffffffffu, t1, 2);
@@ -210,6 +226,9 @@ struct QmmParams {
   void* y;
   // kQmmUp, kQmmDown
   float* h;                  // [M * top_k][n] (written by kQmmUp)
+  uint8_t* recs_h;           // its records for kQmmDown, made by kQmmUp's last finisher of each 256 rows,
+  int32_t* done;             // counted here, [group][256 rows], zeroed by the routing kernel
+  int order_h;
   int E, score;              // experts; -1: ids and wts are given, else they are outputs
   const double* logits;      // [M][E]
   const float* sel_bias;
@@ -298,11 +317,11 @@ template <> struct QmmFmt<NSQ_TYPE_Q6_K> { static constexpr int CB = 210, PA = 2
 template <> struct QmmFmt<NSQ_TYPE_Q4_0> { static constexpr int CB = 144, PA = 144, PG = 176, MT = 2; };
 template <> struct QmmFmt<NSQ_TYPE_Q8_0> { static constexpr int CB = 272, PA = 272, PG = 304, MT = 1; };
 
-// Row tiles of a warp for groups of up to TS tokens: one beyond 8 tokens, whose
+// Row tiles of a warp for groups of up to TS tokens: one beyond 4 tokens, whose
 // sums take the registers.
 template <int TYPE>
 __host__ __device__ constexpr int qmm_tiles(int TS) {
-  return TS > 8 ? 1 : QmmFmt<TYPE>::MT;
+  return TS > 4 ? 1 : QmmFmt<TYPE>::MT;
 }
 
 // All shared memory is addressed as an offset from this array, so that loads
@@ -316,28 +335,50 @@ __device__ __forceinline__ T qmm_lds(uint32_t off) {
   return *reinterpret_cast<const T*>(qmm_smem + off);
 }
 
-// Where this lane reads the B operands of NI n-tiles of two tokens: column n =
-// lane / 4 is limb n % 4 of token first + 2j + n / 4 (a record of zeros for
-// absent tokens).
-template <int NI>
+// Where this lane (column n = lane / 4) reads the B operands of NI n-tiles; a
+// record of zeros stands for absent tokens and the fourth limb.
+//   LIMBS == false: tile j holds tokens 2j and 2j + 1, column n limb n % 4 of token 2j + n / 4
+//   LIMBS == true:  tile j holds limb j % 3 of tokens 8 (j / 3) + n
+template <int NI, bool LIMBS>
 struct QmmB {
   uint32_t even[NI], odd[NI];  // units 4i + c of even and odd i, less 64 i
   uint32_t t[NI];              // the sums T
-  __device__ __forceinline__ QmmB(uint32_t recs, uint32_t zeros, int first, int count, int n, int c) {
-    const int limb = n & 3, flip = (limb & 1) * 64;
+  __device__ __forceinline__ QmmB(uint32_t recs, uint32_t zeros, int count, int n, int c) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const int tok = first + 2 * j + (n >> 2);
-      const uint32_t r = tok < count ? recs + tok * kQmmRec : zeros;
-      even[j] = r + 256 * limb + 16 * c + flip;
-      odd[j] = r + 256 * limb + 16 * c - flip;
-      t[j] = r + kQmmRecT + 32 * limb + 8 * c;
+      const int tok = LIMBS ? 8 * (j / 3) + n : 2 * j + (n >> 2), limb = LIMBS ? j % 3 : n & 3;
+      const uint32_t r = tok < count && limb < 3 ? recs + tok * kQmmRecPitch : zeros;
+      const int at = limb < 3 ? limb : 0, flip = (at & 1) * 64;
+      even[j] = r + 256 * at + 16 * c + flip;
+      odd[j] = r + 256 * at + 16 * c - flip;
+      t[j] = r + kQmmRecT + 32 * at + 8 * c;
     }
   }
   __device__ __forceinline__ uint4 unit(int j, int i) const {
     return qmm_lds<uint4>(((i & 1) ? odd[j] : even[j]) + 64 * i);
   }
 };
+// Values of a lane per row half: one of a token's two limb pairs per tile, or
+// (LIMBS) two whole tokens, 8g + 2c and 8g + 2c + 1, per three tiles.
+template <int NI, bool LIMBS>
+constexpr int kQmmVals = LIMBS ? NI / 3 * 2 : NI;
+// u += k * (the tiles' sums f as values)
+template <int NI, bool LIMBS>
+__device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], const float (&k)[2], const float (&f)[NI][4]) {
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    if constexpr (LIMBS) {
+#pragma unroll
+      for (int q = 0; q < NI / 3 * 2; ++q) {
+        const int j = q / 2 * 3, e = 2 * r + (q & 1);
+        u[q][r] = fmaf(k[r], fmaf(65536.0f, f[j + 2][e], fmaf(256.0f, f[j + 1][e], f[j][e])), u[q][r]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) u[j][r] = fmaf(k[r], fmaf(256.0f, f[j][2 * r + 1], f[j][2 * r]), u[j][r]);
+    }
+  }
+}
 
 // A weight row whose first byte lies at an even offset: words at even
 // offsets as two aligned words and a funnel shift.
@@ -378,15 +419,25 @@ __device__ __forceinline__ int qmm_s8(uint32_t w) {
   asm("prmt.b32 %0, %1, 0, %2;" : "=r"(v) : "r"(w), "n"(0x8880 + 0x1111 * b));
   return v;
 }
-// Sums of the columns 2c, 2c + 1 (two neighbouring limbs) as one value.
-__device__ __forceinline__ float qmm_limbs(float lo, float hi) { return fmaf(256.0f, hi, lo); }
-
-// One row tile's products of a unit for NI n-tiles: u[j][row half], this
-// lane's two limbs of token 2j + c / 2, without the scale s 256^(2 (c % 2)).
-// o: the shared-memory offsets of this lane's weight rows lane / 4 and
-// lane / 4 + 8; c = lane % 4; nv: valid 32-weight blocks (Q4_0, Q8_0).
-template <int TYPE, int LAYOUT, int NI>
-__device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const QmmB<NI>& B, int nv, float (&u)[NI][2]) {
+// One row tile's products of a unit for NI n-tiles: the values u (see QmmB)
+// per row half, without the token scale.  o: the shared-memory offsets of this
+// lane's weight rows lane / 4 and lane / 4 + 8; c = lane % 4; nv: valid
+// 32-weight blocks (Q4_0, Q8_0).
+template <int TYPE, int LAYOUT, int NI, bool LIMBS>
+__device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const QmmB<NI, LIMBS>& B, int nv,
+                                         float (&u)[kQmmVals<NI, LIMBS>][2]) {
+#pragma unroll
+  for (int q = 0; q < kQmmVals<NI, LIMBS>; ++q) u[q][0] = u[q][1] = 0.0f;
+  // u += k * (A against the sums T)
+  auto against_t = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const float (&k)[2]) {
+    float am[NI][4];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const uint2 b = qmm_lds<uint2>(B.t[j]);
+      qmm_mma_f16(am[j], a0, a1, a2, a3, b.x, b.y);
+    }
+    qmm_add<NI, LIMBS>(u, k, am);
+  };
   if constexpr (TYPE == NSQ_TYPE_Q4_K || TYPE == NSQ_TYPE_Q5_K) {
     const __half2 k1024 = __float2half2_rn(1024.0f);
     uint32_t sc[2][2];  // [row]: scales of sub-blocks 0..3 and 4..7
@@ -405,14 +456,7 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
         ma[r] = qmm_h2u(__hsub2(qmm_dup1024(m_lo, c), k1024));  // T's groups 2c, 2c+1 are sub-block c
         mb[r] = qmm_h2u(__hsub2(qmm_dup1024(m_hi, c), k1024));
       }
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const uint2 b = qmm_lds<uint2>(B.t[j]);
-        float am[4];
-        qmm_mma_f16(am, ma[0], ma[1], mb[0], mb[1], b.x, b.y);
-        u[j][0] = dm[0] * qmm_limbs(am[0], am[1]);
-        u[j][1] = dm[1] * qmm_limbs(am[2], am[3]);
-      }
+      against_t(ma[0], ma[1], mb[0], mb[1], dm);
     }
     constexpr int QS = TYPE == NSQ_TYPE_Q4_K ? 16 : 48;
     [[maybe_unused]] uint2 hg[2];
@@ -478,14 +522,13 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
         for (int e = 0; e < 4; ++e) hi[j][e] += acc[e] * so[e >> 1];
       }
     }
+    float f[NI][4];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      float f[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = (float)((TYPE == NSQ_TYPE_Q4_K ? 16 * lo[j][e] : lo[j][e]) + hi[j][e]);
-      u[j][0] += d[0] * qmm_limbs(f[0], f[1]);
-      u[j][1] += d[1] * qmm_limbs(f[2], f[3]);
+      for (int e = 0; e < 4; ++e) f[j][e] = (float)((TYPE == NSQ_TYPE_Q4_K ? 16 * lo[j][e] : lo[j][e]) + hi[j][e]);
     }
+    qmm_add<NI, LIMBS>(u, d, f);
   } else if constexpr (TYPE == NSQ_TYPE_Q4_0 || TYPE == NSQ_TYPE_Q8_0) {
     constexpr int BB = TYPE == NSQ_TYPE_Q4_0 ? 18 : 34;
     // the sums start at the bits of 1.5 * 2^23: as f32 they are that plus the
@@ -503,17 +546,8 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
           ta[r][q] = d | (d << 16);
         }
       }
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const uint2 b = qmm_lds<uint2>(B.t[j]);
-        float am[4];
-        qmm_mma_f16(am, ta[0][0], ta[1][0], ta[0][1], ta[1][1], b.x, b.y);
-        u[j][0] = -8.0f * qmm_limbs(am[0], am[1]);
-        u[j][1] = -8.0f * qmm_limbs(am[2], am[3]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) u[j][0] = u[j][1] = 0.0f;
+      const float k[2] = {-8.0f, -8.0f};
+      against_t(ta[0][0], ta[1][0], ta[0][1], ta[1][1], k);
     }
     qmm_for<8>([&](auto I) {
       constexpr int i = decltype(I)::value;
@@ -531,18 +565,17 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
           a[r][1] = rows[r].template word<BB * i + 18>(4 * c);
         }
       }
+      float f[NI][4];
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         const uint4 x = B.unit(j, i >> 1);
         int acc[4];
         qmm_mma_k32<TYPE == NSQ_TYPE_Q8_0>(acc, a[0][0], a[1][0], a[0][1], a[1][1], (i & 1) ? x.z : x.x, (i & 1) ? x.w : x.y,
                                            kMagic);
-        float f[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = __int_as_float(acc[e]) - kMagicF;
-        u[j][0] += d[0] * qmm_limbs(f[0], f[1]);
-        u[j][1] += d[1] * qmm_limbs(f[2], f[3]);
+        for (int e = 0; e < 4; ++e) f[j][e] = __int_as_float(acc[e]) - kMagicF;
       }
+      qmm_add<NI, LIMBS>(u, d, f);
     });
   } else {  // Q6_K
     const QmmRow rows[2] = {QmmRow(o[0]), QmmRow(o[1])};
@@ -565,13 +598,10 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
       ta[r][1] = qmm_h2u(__hsub2(qmm_u2h(__byte_perm((c < 2 ? sw[r][2] : sw[r][3]) ^ 0x80808080u, 0x64646464u, sel)), off));
     }
     int sum[NI][4];
+    const float k[2] = {-32.0f * d[0], -32.0f * d[1]};
+    against_t(ta[0][0], ta[1][0], ta[0][1], ta[1][1], k);
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const uint2 b = qmm_lds<uint2>(B.t[j]);
-      float am[4];
-      qmm_mma_f16(am, ta[0][0], ta[1][0], ta[0][1], ta[1][1], b.x, b.y);
-      u[j][0] = -32.0f * qmm_limbs(am[0], am[1]);
-      u[j][1] = -32.0f * qmm_limbs(am[2], am[3]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[j][e] = 0;
     }
@@ -625,12 +655,13 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
         }
       }
     });
+    float f[NI][4];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-        u[j][r] = d[r] * (u[j][r] + qmm_limbs((float)sum[j][2 * r], (float)sum[j][2 * r + 1]));
+      for (int e = 0; e < 4; ++e) f[j][e] = (float)sum[j][e];
     }
+    qmm_add<NI, LIMBS>(u, d, f);
   }
 }
 
@@ -814,7 +845,7 @@ __device__ __forceinline__ float qmm_ld_cluster(const float* p, uint32_t rank) {
 
 // Bytes of a slot: RW tiles of rows at this pitch, then TS records.
 __host__ __device__ inline uint32_t qmm_slot_bytes(int row_tiles, int pitch, int TS) {
-  return (uint32_t)(row_tiles * 16 * pitch + (TS * kQmmRec + 127) / 128 * 128);
+  return (uint32_t)(row_tiles * 16 * pitch + (TS * kQmmRecPitch + 127) / 128 * 128);
 }
 inline size_t qmm_lists_bytes(int P) { return (size_t)P * (sizeof(QmmGroup) + 12); }
 
@@ -841,14 +872,15 @@ struct QmmCursor {
   int tile, g, sb, u;
 };
 
-// NJ: n-tiles of two tokens that a group can have (1, 2, 4 or 8).
-template <int TYPE, int LAYOUT, int NJ, int MODE>
+// TC: the most tokens of a group (2, 4, 8 or 16).
+template <int TYPE, int LAYOUT, int TC, int MODE>
 __global__ void __launch_bounds__(kQmmThreads, 2)
     qmm_kernel(const __grid_constant__ QmmParams p, const __grid_constant__ CUtensorMap map0,
                const __grid_constant__ CUtensorMap map1) {
   using F = QmmFmt<TYPE>;
   constexpr int BB = Fmt<TYPE>::BB;
-  constexpr int MT = qmm_tiles<TYPE>(2 * NJ);
+  constexpr int MT = qmm_tiles<TYPE>(TC);
+  constexpr int NQ = TC == 2 ? 1 : TC <= 8 ? 2 : 4;  // values of a lane per row half
   constexpr int WR = 16 * MT;                       // weight rows of a warp
   constexpr int OR = MODE == kQmmUp ? WR / 2 : WR;  // output rows of a warp
   uint8_t* const smem = qmm_smem;
@@ -870,7 +902,8 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   const bool in_ring = MODE != kQmmDown && split;
   float* const ys = reinterpret_cast<float*>(smem + kQmmCtl + (in_ring ? 0 : ring_bytes));
   const int ys_warp = YC * WR, ys_buf = kQmmWarps * ys_warp;
-  const uint32_t zeros = kQmmCtl + ring_bytes + (in_ring ? 0 : p.PB * ys_buf * 4);  // a record of zeros
+  const int buffers = in_ring ? 0 : MODE == kQmmUp && p.PB == 0 ? 1 : p.PB;
+  const uint32_t zeros = kQmmCtl + ring_bytes + buffers * ys_buf * 4;  // a record of zeros
   const int rank = split ? (int)qmm_cluster_rank() : 0;
   const int cta = blockIdx.x / p.split, nctas = gridDim.x / p.split;
   const int tile_rows = OR * RW;
@@ -885,6 +918,10 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       report_status(NSQ_ERR_ALIGN);
       return;
     }
+  }
+  if (p.rows_aligned && threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map0)) : "memory");
+    if constexpr (MODE == kQmmUp) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map1)) : "memory");
   }
   for (int i = threadIdx.x; i < kQmmRec / 4; i += kQmmThreads) reinterpret_cast<uint32_t*>(smem + zeros)[i] = 0u;
   if (threadIdx.x == 0) {
@@ -1021,7 +1058,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       int row = lane;
       if constexpr (MODE == kQmmUp) row = L.ptok[L.groups[pc.g].start + lane];
       if constexpr (MODE == kQmmDown) row = L.plist[L.groups[pc.g].start + lane];
-      bulk_g2s(dst + lane * kQmmRec, p.recs + ((int64_t)row * p.nsb + pc.sb) * kQmmRec, kQmmRec, bar);
+      bulk_g2s(dst + lane * kQmmRecPitch, p.recs + ((int64_t)row * p.nsb + pc.sb) * kQmmRec, kQmmRec, bar);
     }
   };
   const bool keeper = rw == (kw & (RW - 1));  // refills the column's records
@@ -1054,25 +1091,56 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   }
 
   bool ok = true;
-  float tot[MT][NJ][2];
+  float tot[MT][NQ][2];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) tot[t][j][0] = tot[t][j][1] = 0.0f;
+    for (int j = 0; j < NQ; ++j) tot[t][j][0] = tot[t][j][1] = 0.0f;
   }
-  // this warp's sums of a task into its shared-memory block [YC][WR]: the two
-  // lanes that share a token add their limbs and take a row half each
-  auto leave_sums = [&](float* to) {
+  // calls f(token, row of the warp, sum) for the sums of a task of `count`
+  // tokens and clears them: with up to 4 tokens the two lanes that share a
+  // token add their limbs and take a row half each, else a lane has whole ones
+  auto each_sum = [&](int count, auto&& f) {
+    const int half = lc & 1;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int tk = 2 * j + (lc >> 1), half = lc & 1;
+    for (int t = 0; t < MT; ++t) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const float give = half ? tot[t][j][0] : tot[t][j][1];
-        const float v = (half ? tot[t][j][1] : tot[t][j][0]) + __shfl_xor_sync(0xffffffffu, give, 1);
-        if (tk < YC) to[tk * WR + 16 * t + lr + 8 * half] = v;
-        tot[t][j][0] = tot[t][j][1] = 0.0f;
+      for (int q = 0; q < NQ; ++q) {
+        if (TC > 4 && count > 4) {
+          const int tk = 8 * (q >> 1) + 2 * lc + (q & 1);
+          f(tk, 16 * t + lr, tot[t][q][0]);
+          f(tk, 16 * t + lr + 8, tot[t][q][1]);
+        } else if (q < 2) {
+          const float give = half ? tot[t][q][0] : tot[t][q][1];
+          const float v = (half ? tot[t][q][1] : tot[t][q][0]) + __shfl_xor_sync(0xffffffffu, give, 1);
+          f(2 * q + (lc >> 1), 16 * t + lr + 8 * half, v);
+        }
+        tot[t][q][0] = tot[t][q][1] = 0.0f;
       }
+    }
+  };
+  auto leave_sums = [&](int count, float* to) {
+    each_sum(count, [&](int tk, int r, float v) {
+      if (tk < count) to[tk * WR + r] = v;
+    });
+  };
+  // kQmmUp: this warp has stored h of OR rows from `row` on for the tokens of
+  // group g.  Whoever completes 256 rows makes their records.
+  auto finish_rows = [&](int g, int row) {
+    if (row >= p.n) return;
+    __syncwarp();
+    const int sb = row >> 8, valid = min(256, (int)p.n - 256 * sb), nsb = ((int)p.n + 255) >> 8;
+    int last = 0;
+    if (lane == 0) {
+      __threadfence();
+      last = atomicAdd(p.done + (int64_t)g * nsb + sb, 1) == (valid + OR - 1) / OR - 1;
+      __threadfence();
+    }
+    if (!__shfl_sync(0xffffffffu, last, 0)) return;
+    const int count = L.groups[g].count, start = L.groups[g].start;
+    for (int t = 0; t < count; ++t) {
+      const int64_t pick = L.plist[start + t];
+      qmm_make_record<float, true>(p.h + pick * p.n + 256 * sb, valid, p.order_h, p.recs_h + (pick * nsb + sb) * kQmmRec, lane);
     }
   };
   int stage = 0, seq = 0;
@@ -1132,42 +1200,52 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
           }
           o[h] = slot + my_rows + r * pitch + mis;
         }
-        // up to 8 tokens at a time, as many n-tiles as there are tokens
-        auto unit = [&](auto N, auto First) {
-          constexpr int ni = decltype(N)::value, j0 = decltype(First)::value;
-          const QmmB<ni> B(slot + recs_at, zeros, 2 * j0, count, lr, lc);
-          float v[ni][2];
-          qmm_unit<TYPE, LAYOUT, ni>(o, lc, B, nv, v);
+        auto unit = [&](auto N, auto Limbs) {
+          constexpr int ni = decltype(N)::value;
+          constexpr bool limbs = decltype(Limbs)::value;
+          constexpr int nq = kQmmVals<ni, limbs>;
+          const QmmB<ni, limbs> B(slot + recs_at, zeros, count, lr, lc);
+          float v[nq][2];
+          qmm_unit<TYPE, LAYOUT, ni, limbs>(o, lc, B, nv, v);
 #pragma unroll
-          for (int j = 0; j < ni; ++j) {
-            const int tk = 2 * (j0 + j) + (lc >> 1);
-            // the lane's limbs: 0, 1 or 2, 3 of this token
-            const float s = tk < count ? qmm_lds<float>(slot + recs_at + tk * kQmmRec + kQmmRecS) * (lc & 1 ? 65536.0f : 1.0f) : 0.0f;
+          for (int q = 0; q < nq; ++q) {
+            const int tk = limbs ? 8 * (q >> 1) + 2 * lc + (q & 1) : 2 * q + (lc >> 1);
+            float s = tk < count ? qmm_lds<float>(slot + recs_at + tk * kQmmRecPitch + kQmmRecS) : 0.0f;
+            if (!limbs && (lc & 1)) s *= 65536.0f;  // limbs 2, 3 of the token
+            float y0 = s * v[q][0], y1 = s * v[q][1];
             if constexpr (MODE == kQmmDown) {
-              float y0 = s * v[j][0], y1 = s * v[j][1];
-              y0 += __shfl_xor_sync(0xffffffffu, y0, 1);
-              y1 += __shfl_xor_sync(0xffffffffu, y1, 1);
-              if (tk < count) {  // the pair of lanes takes a row half each
+              if constexpr (!limbs) {  // the pair of lanes takes a row half each
+                y0 += __shfl_xor_sync(0xffffffffu, y0, 1);
+                y1 += __shfl_xor_sync(0xffffffffu, y1, 1);
+              }
+              if (tk < count) {
                 const int pick = L.groups[c.g].start + tk;
-                my_ys[L.ptok[pick] * WR + 16 * t + lr + 8 * (lc & 1)] += L.pwts[pick] * (lc & 1 ? y1 : y0);
+                const float w = L.pwts[pick];
+                float* to = my_ys + L.ptok[pick] * WR + 16 * t + lr;
+                if constexpr (limbs) {
+                  to[0] += w * y0;
+                  to[8] += w * y1;
+                } else {
+                  to[8 * (lc & 1)] += w * (lc & 1 ? y1 : y0);
+                }
               }
             } else {
-              tot[t][j0 + j][0] += s * v[j][0];
-              tot[t][j0 + j][1] += s * v[j][1];
+              tot[t][q][0] += y0;
+              tot[t][q][1] += y1;
             }
           }
         };
         using std::integral_constant;
-        constexpr integral_constant<int, 0> zero{};
-        if (NJ == 1 || count <= 2) {
-          unit(integral_constant<int, 1>{}, zero);
-        } else if (NJ == 2 || count <= 4) {
-          unit(integral_constant<int, NJ < 2 ? NJ : 2>{}, zero);
+        using std::false_type;
+        using std::true_type;
+        if (TC == 2 || count <= 2) {
+          unit(integral_constant<int, 1>{}, false_type{});
+        } else if (TC == 4 || count <= 4) {
+          if constexpr (TC > 2) unit(integral_constant<int, 2>{}, false_type{});
+        } else if (TC == 8 || count <= 8) {
+          if constexpr (TC > 4) unit(integral_constant<int, 3>{}, true_type{});
         } else {
-          unit(integral_constant<int, NJ < 4 ? NJ : 4>{}, zero);
-          if constexpr (NJ == 8) {
-            if (count > 8) unit(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-          }
+          if constexpr (TC > 8) unit(integral_constant<int, 6>{}, true_type{});
         }
       }
       __syncwarp();
@@ -1185,36 +1263,24 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     const int row0 = c.tile * tile_rows + rw * OR;
     const int cnt = MODE == kQmmUp ? L.groups[c.g].count : p.M;
     if (p.PB == 0) {
-      // ---- KW == 1: outputs straight from the registers, a row half per lane
-      // of the pair that shares a token
-      const int half = lc & 1;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int tk = 2 * j + (lc >> 1);
-        float v[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const float give = half ? tot[t][j][0] : tot[t][j][1];
-          v[t] = (half ? tot[t][j][1] : tot[t][j][0]) + __shfl_xor_sync(0xffffffffu, give, 1);
+      // ---- KW == 1: outputs straight from the registers (kQmmUp: through
+      // the warp's own block of shared memory, to bring gate and up together)
+      if constexpr (MODE == kQmmUp) {
+        float* own = ys + warp * ys_warp;
+        leave_sums(cnt, own);
+        __syncwarp();
+        for (int i = lane; i < OR * cnt; i += 32) {
+          const int col = i / OR, r = i % OR;
+          if (row0 + r < p.n)
+            p.h[(int64_t)L.plist[L.groups[c.g].start + col] * p.n + row0 + r] =
+                qmm_act(own[col * WR + r], p.act) * own[col * WR + r + OR];
         }
-        if constexpr (MODE == kQmmUp) {
-          // gate and up of an output row: the two tiles, or the two row halves of one
-          const float up = MT == 2 ? v[MT - 1] : __shfl_xor_sync(0xffffffffu, v[0], 1);
-          const int row = row0 + (MT == 2 ? 8 * half : 0) + lr;
-          if (tk < cnt && row < p.n && (MT == 2 || half == 0))
-            p.h[(int64_t)L.plist[L.groups[c.g].start + tk] * p.n + row] = qmm_act(v[0], p.act) * up;
-        } else if constexpr (MODE == kQmmLinear) {
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const int row = row0 + 16 * t + 8 * half + lr;
-            if (tk < cnt && row < p.n) qmm_store(p, tk, row, v[t]);
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) tot[t][j][0] = tot[t][j][1] = 0.0f;
+        finish_rows(c.g, row0);
+        __syncwarp();
+      } else if constexpr (MODE == kQmmLinear) {
+        each_sum(cnt, [&](int tk, int r, float v) {
+          if (tk < cnt && row0 + r < p.n) qmm_store(p, tk, row0 + r, v);
+        });
       }
       continue;
     }
@@ -1225,7 +1291,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         break;
       }
       __syncwarp();
-      leave_sums(my_ys);
+      leave_sums(cnt, my_ys);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&ready[rw][buf]);
@@ -1254,15 +1320,17 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&taken[rw][buf]);
+      if constexpr (MODE == kQmmUp) finish_rows(c.g, row0);
     }
   }
   if constexpr (MODE != kQmmUp) {
     if (split) {
       // ---- a K split over the cluster: each rank adds its columns' sums into
-      // those of its first column, rank 0 adds the ranks' in order
+      // those of its first column, then all ranks their share of the outputs,
+      // always over the ranks in order
       __syncthreads();  // every warp is done with the ring
       if constexpr (MODE == kQmmLinear) {
-        leave_sums(ys + warp * ys_warp);
+        leave_sums(p.M, ys + warp * ys_warp);
         __syncthreads();
       }
       const int outs = RW * WR * p.M;
@@ -1279,17 +1347,19 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         q[0] = v;
       }
       qmm_cluster_sync();
-      if (rank == 0) {
-        for (int i = threadIdx.x; i < outs; i += kQmmThreads) {
-          int col, r;
-          const float* q = place(i, col, r);
-          float v = q[0];
-          for (int k = 1; k < p.split; ++k) v += qmm_ld_cluster(q, (uint32_t)k);
-          const int row = cta * tile_rows + r;
-          if (row < p.n) qmm_store(p, col, row, v);
-        }
+      for (int i = rank * kQmmThreads + threadIdx.x; i < outs; i += p.split * kQmmThreads) {
+        int col, r;
+        const float* q = place(i, col, r);
+        float part[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) part[k] = k < p.split ? qmm_ld_cluster(q, (uint32_t)k) : 0.0f;
+        float v = part[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v += part[k];
+        const int row = cta * tile_rows + r;
+        if (row < p.n) qmm_store(p, col, row, v);
       }
-      qmm_cluster_sync();  // the leader has read every rank's sums
+      qmm_cluster_sync();  // every rank has read the others' sums
     }
   }
 }

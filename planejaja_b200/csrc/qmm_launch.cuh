@@ -5,9 +5,9 @@
 
 namespace nsq {
 
-template <int TYPE, int LAYOUT, int NJ, int MODE>
+template <int TYPE, int LAYOUT, int TC, int MODE>
 int launch_qmm_t(const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
-  auto kern = qmm_kernel<TYPE, LAYOUT, NJ, MODE>;
+  auto kern = qmm_kernel<TYPE, LAYOUT, TC, MODE>;
   // the opt-in limit is set once per device; the launches ask for what they need
   static bool configured[64] = {};
   int dev = 0;
@@ -37,19 +37,19 @@ int launch_qmm_t(const QmmParams& p, const CUtensorMap* maps, int grid, size_t s
   return cudaLaunchKernelEx(&cfg, kern, p, maps[0], maps[1]) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
 }
 
-template <int TYPE, int LAYOUT, int NJ>
+template <int TYPE, int LAYOUT, int TC>
 int launch_qmm_mode(const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
-  if (p.mode == kQmmLinear) return launch_qmm_t<TYPE, LAYOUT, NJ, kQmmLinear>(p, maps, grid, smem, st);
-  if (p.mode == kQmmUp) return launch_qmm_t<TYPE, LAYOUT, NJ, kQmmUp>(p, maps, grid, smem, st);
-  return launch_qmm_t<TYPE, LAYOUT, NJ, kQmmDown>(p, maps, grid, smem, st);
+  if (p.mode == kQmmLinear) return launch_qmm_t<TYPE, LAYOUT, TC, kQmmLinear>(p, maps, grid, smem, st);
+  if (p.mode == kQmmUp) return launch_qmm_t<TYPE, LAYOUT, TC, kQmmUp>(p, maps, grid, smem, st);
+  return launch_qmm_t<TYPE, LAYOUT, TC, kQmmDown>(p, maps, grid, smem, st);
 }
 
 template <int TYPE, int LAYOUT>
 int launch_qmm_layout(const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st) {
-  if (p.TS <= 2) return launch_qmm_mode<TYPE, LAYOUT, 1>(p, maps, grid, smem, st);
-  if (p.TS <= 4) return launch_qmm_mode<TYPE, LAYOUT, 2>(p, maps, grid, smem, st);
-  if (p.TS <= 8) return launch_qmm_mode<TYPE, LAYOUT, 4>(p, maps, grid, smem, st);
-  return launch_qmm_mode<TYPE, LAYOUT, 8>(p, maps, grid, smem, st);
+  if (p.TS <= 2) return launch_qmm_mode<TYPE, LAYOUT, 2>(p, maps, grid, smem, st);
+  if (p.TS <= 4) return launch_qmm_mode<TYPE, LAYOUT, 4>(p, maps, grid, smem, st);
+  if (p.TS <= 8) return launch_qmm_mode<TYPE, LAYOUT, 8>(p, maps, grid, smem, st);
+  return launch_qmm_mode<TYPE, LAYOUT, 16>(p, maps, grid, smem, st);
 }
 
 template <int TYPE>

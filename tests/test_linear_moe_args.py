@@ -39,16 +39,16 @@ def linear(lib, **kw):
     (_lib.ERR_SHAPE, dict(m=0)), (_lib.ERR_SHAPE, dict(m=-1)), (_lib.ERR_SHAPE, dict(m=17)),
     (_lib.ERR_SHAPE, dict(n=0)), (_lib.ERR_SHAPE, dict(n=1 << 25)), (_lib.ERR_SHAPE, dict(k=128)),
     (_lib.ERR_SHAPE, dict(t=Q8_0, k=48)), (_lib.ERR_SHAPE, dict(k=0)),
-    (_lib.ERR_WORKSPACE, dict(ws=None)), (_lib.ERR_WORKSPACE, dict(m=3, k=512, wsb=3 * 2 * 1168 - 1)),
+    (_lib.ERR_WORKSPACE, dict(ws=None)), (_lib.ERR_WORKSPACE, dict(m=3, k=512, wsb=3 * 2 * 880 - 1)),
 ])
 def test_linear_refusals(lib, want, kw):
     assert linear(lib, **kw) == want
 
 
 def test_linear_workspace_size(lib):
-    # one record of 1168 bytes per token and 256 of K
-    assert lib.nsq_linear_workspace_size(1, 256) == 1168
-    assert lib.nsq_linear_workspace_size(16, 896) == 16 * 4 * 1168
+    # one record of 880 bytes per token and 256 of K
+    assert lib.nsq_linear_workspace_size(1, 256) == 880
+    assert lib.nsq_linear_workspace_size(16, 896) == 16 * 4 * 880
     assert lib.nsq_linear_workspace_size(17, 256) == 0
     assert lib.nsq_linear_workspace_size(0, 256) == 0
 
