@@ -276,7 +276,7 @@ __device__ __forceinline__ bool wait_geq_bounded(const uint32_t* p, uint32_t wan
 enum TuneId : int {
   kTuneRowsR, kTuneRowsPPSM, kTuneRowsStages, kTuneRowsPre, kTuneRowsL2Hint, kTuneRowsCPS, kTuneRowsC,
   kTuneRowsBal, kTuneRowsCarve, kTuneMmaMinM, kTuneMmaPPS, kTuneMmaStages, kTuneGemvGeneral, kTuneGemmSplit,
-  kTuneGemmTok, kTuneTcMinM, kTuneTcA, kTuneCount
+  kTuneGemmTok, kTuneTcMinM, kTuneTcA, kTuneQmmKW, kTuneQmmSplit, kTuneCount
 };
 int tune(TuneId id, int dflt);
 // Counts one kernel launch (nsq_kernel_launches).

@@ -17,8 +17,7 @@ int check_weights(const void* w, int type, int layout, int64_t K);
 int device_check(int* num_sms);
 
 constexpr int kPrepThreads = 32 * kQmmWarps;
-constexpr int kRouteTok = 8;    // tokens of a router row's pass
-constexpr int kRouteCtas = 8;   // CTAs (a cluster) that compute the logits
+constexpr int kRouteTok = 8;  // tokens of one CTA's logits
 
 // Activation records of rows x nsb units, one warp each.
 template <typename T>
@@ -44,105 +43,95 @@ __device__ __forceinline__ float4 load4(const float* p, bool wide) {
   return wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
 }
 
-// First kernel of a mixture-of-experts call: the first cluster computes the
-// router's logits, picks the experts and lists the picks by expert; the other
-// CTAs prepare the activation records.  Two experts' logits may lie
-// arbitrarily close, and a pick that flips changes the output by whole
-// experts: products of f32 are exact in f64, and the sums are f64.  One
-// cluster, because its barrier lets one kernel do it all: a grid-wide
-// computation of the logits needs a second launch, or every CTA of the next
-// kernel building the lists for itself (about 8 us of its start).
-__global__ void __launch_bounds__(kPrepThreads) moe_route_kernel(const __grid_constant__ QmmParams p,
-                                                                 const float* __restrict__ x,
-                                                                 const float* __restrict__ router, int64_t K, int order,
-                                                                 uint8_t* __restrict__ recs, double* __restrict__ logits) {
+// First kernel of a mixture-of-experts call: the first nlog CTAs compute the
+// router's logits (one expert, eight tokens each), the others the activation
+// records; they also zero kQmmUp's counters.  With given picks the first CTA
+// lists them by expert.  Two experts' logits may lie arbitrarily close, and a
+// pick that flips changes the output by whole experts: products of f32 are
+// exact in f64, and the sums are f64.
+__global__ void __launch_bounds__(kPrepThreads) moe_logits_kernel(const __grid_constant__ QmmParams p,
+                                                                  const float* __restrict__ x,
+                                                                  const float* __restrict__ router, int64_t K, int order,
+                                                                  uint8_t* __restrict__ recs, double* __restrict__ logits,
+                                                                  int nlog) {
   extern __shared__ __align__(16) int32_t route_mem[];
-  __shared__ double part[kQmmWarps * NSQ_MOE_MAX_TOKENS];  // [K share][expert][token]: KS * ne <= 8
+  __shared__ double part[kQmmWarps][kRouteTok];
   qmm_dep_wait();
   qmm_dep_launch();
-  if (blockIdx.x >= kRouteCtas) {
-    make_records(x, p.M, K, p.nsb, order, recs, blockIdx.x - kRouteCtas);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((int)blockIdx.x >= nlog) {
+    make_records(x, p.M, K, p.nsb, order, recs, blockIdx.x - nlog);
     const int64_t counters = (int64_t)p.M * p.top_k * ((p.n + 255) / 256);
-    for (int64_t i = (int64_t)(blockIdx.x - kRouteCtas) * kPrepThreads + threadIdx.x; i < counters;
-         i += (int64_t)(gridDim.x - kRouteCtas) * kPrepThreads)
+    for (int64_t i = (int64_t)(blockIdx.x - nlog) * kPrepThreads + threadIdx.x; i < counters;
+         i += (int64_t)(gridDim.x - nlog) * kPrepThreads)
       p.done[i] = 0;
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x;
-  if (router) {
-    // experts rank, rank + 8, ...; with few of them several warps share one's K
-    const int ne = p.E > rank ? (p.E - rank + kRouteCtas - 1) / kRouteCtas : 0;
-    const int KS = p.E <= kRouteCtas ? 8 : p.E <= 2 * kRouteCtas ? 4 : p.E <= 4 * kRouteCtas ? 2 : 1;
-    const int ks = warp % KS;
-    const bool wide = ((reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(x)) & 15) == 0;  // K % 32 == 0
-    for (int i = warp / KS; i < ne; i += kQmmWarps / KS) {
-      const float* w = router + (int64_t)(rank + kRouteCtas * i) * K;
-      for (int m0 = 0; m0 < p.M; m0 += kRouteTok) {
-        const int mc = min(kRouteTok, p.M - m0);
-        double acc[kRouteTok] = {};
-        // eight 16-byte loads of the row are in flight: one at a time, a row of
-        // 2048 took 11 us
-        for (int64_t k0 = 4 * (lane + 32 * ks); k0 < K; k0 += 8 * 128 * KS) {
-          float4 a[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int64_t k = k0 + 128 * KS * q;
-            a[q] = k < K ? load4(w + k, wide) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          }
-#pragma unroll
-          for (int t = 0; t < kRouteTok; ++t) {
-            if (t < mc) {
-              float4 b[8];
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const int64_t k = k0 + 128 * KS * q;
-                b[q] = k < K ? load4(x + (int64_t)(m0 + t) * K + k, wide) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              }
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                acc[t] = fma((double)a[q].x, (double)b[q].x,
-                             fma((double)a[q].y, (double)b[q].y,
-                                 fma((double)a[q].z, (double)b[q].z, fma((double)a[q].w, (double)b[q].w, acc[t]))));
-            }
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < kRouteTok; ++t) {
-          if (t < mc) {
-            double v = acc[t];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) {
-              if (KS == 1) {
-                logits[(int64_t)(m0 + t) * p.E + rank + kRouteCtas * i] = v;
-              } else {
-                part[(ks * ne + i) * p.M + m0 + t] = v;
-              }
-            }
-          }
-        }
-      }
-    }
-    if (KS > 1) {
-      __syncthreads();
-      for (int q = threadIdx.x; q < ne * p.M; q += kPrepThreads) {
-        const int i = q / p.M, m = q - i * p.M;
-        double v = part[q];
-        for (int k = 1; k < KS; ++k) v += part[k * ne * p.M + q];
-        logits[(int64_t)m * p.E + rank + kRouteCtas * i] = v;
-      }
-    }
-    qmm_cluster_sync();  // the logits of every rank, seen by rank 0
+  if (!router) {
+    qmm_build_lists(p, route_mem);
+    return;
   }
-  if (rank == 0) qmm_build_lists(p, route_mem);
+  const int e = blockIdx.x % p.E, m0 = (int)blockIdx.x / p.E * kRouteTok;
+  const int mc = min(kRouteTok, p.M - m0);
+  const float* w = router + (int64_t)e * K;
+  const bool wide = ((reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(x)) & 15) == 0;  // K % 32 == 0
+  double acc[kRouteTok] = {};
+  // four 16-byte loads of the row are in flight
+  for (int64_t k0 = 4 * threadIdx.x; k0 < K; k0 += 4 * 4 * kPrepThreads) {
+    float4 a[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t k = k0 + 4 * kPrepThreads * q;
+      a[q] = k < K ? load4(w + k, wide) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int t = 0; t < kRouteTok; ++t) {
+      if (t < mc) {
+        float4 b[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t k = k0 + 4 * kPrepThreads * q;
+          b[q] = k < K ? load4(x + (int64_t)(m0 + t) * K + k, wide) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          acc[t] = fma((double)a[q].x, (double)b[q].x,
+                       fma((double)a[q].y, (double)b[q].y,
+                           fma((double)a[q].z, (double)b[q].z, fma((double)a[q].w, (double)b[q].w, acc[t]))));
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kRouteTok; ++t) {
+    if (t < mc) {
+      double v = acc[t];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) part[warp][t] = v;
+    }
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < mc) {
+    double v = 0.0;
+    for (int i = 0; i < kQmmWarps; ++i) v += part[i][threadIdx.x];
+    logits[(int64_t)(m0 + threadIdx.x) * p.E + e] = v;
+  }
 }
 
-template <typename T>
-static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* recs, cudaStream_t st) {
-  const int nsb = (int)((K + 255) / 256);
+// One CTA picks the experts from the logits and lists the picks by expert.
+__global__ void __launch_bounds__(512) moe_lists_kernel(const __grid_constant__ QmmParams p) {
+  extern __shared__ __align__(16) int32_t route_mem[];
+  qmm_dep_wait();
+  qmm_dep_launch();
+  qmm_build_lists(p, route_mem);
+}
+
+template <typename... Params, typename... Args>
+static int launch_pdl(void (*kern)(Params...), int64_t grid, int threads, size_t smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((rows * nsb + kQmmWarps - 1) / kQmmWarps));
-  cfg.blockDim = dim3(kPrepThreads);
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -150,31 +139,25 @@ static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   note_launch();
-  return cudaLaunchKernelEx(&cfg, qmm_prep_kernel<T>, x, rows, K, nsb, order, recs) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
 }
 
-// The grid is whole clusters: cluster 0 routes, the rest make records.
+template <typename T>
+static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* recs, cudaStream_t st) {
+  const int nsb = (int)((K + 255) / 256);
+  return launch_pdl(qmm_prep_kernel<T>, (rows * nsb + kQmmWarps - 1) / kQmmWarps, kPrepThreads, 0, st, x, rows, K, nsb,
+                    order, recs);
+}
+
 static int launch_route(const QmmParams& p, const float* x, const float* router, int64_t K, int order, uint8_t* recs,
                         double* logits, cudaStream_t st) {
-  const int64_t P = (int64_t)p.M * p.top_k;
+  const size_t lists = (size_t)p.M * p.top_k * (8 + sizeof(QmmGroup));  // at most 24 KB
+  const int nlog = router ? p.E * ((p.M + kRouteTok - 1) / kRouteTok) : 1;
   const int64_t rec_ctas = ((int64_t)p.M * p.nsb + kQmmWarps - 1) / kQmmWarps;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(kRouteCtas + (rec_ctas + kRouteCtas - 1) / kRouteCtas * kRouteCtas));
-  cfg.blockDim = dim3(kPrepThreads);
-  cfg.dynamicSmemBytes = (size_t)P * (8 + sizeof(QmmGroup));  // at most 24 KB
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kRouteCtas;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  note_launch();
-  return cudaLaunchKernelEx(&cfg, moe_route_kernel, p, x, router, K, order, recs, logits) == cudaSuccess ? NSQ_OK
-                                                                                                          : NSQ_ERR_CUDA;
+  const int rc = launch_pdl(moe_logits_kernel, nlog + rec_ctas, kPrepThreads, router ? 0 : lists, st, p, x, router, K,
+                            order, recs, logits, nlog);
+  if (rc || !router) return rc;
+  return launch_pdl(moe_lists_kernel, 1, 512, lists, st, p);
 }
 
 struct QmmShape {
@@ -238,6 +221,9 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
   size_t smem = 0;
   for (int KW = 1; KW <= kQmmWarps; KW *= 2) {
     if (KW > 1 && KW / 2 >= most_units) break;
+    if (const int only = tune(kTuneQmmKW, 0)) {
+      if (KW < only && KW < kQmmWarps && KW < most_units) continue;
+    }
     QmmParams t = p;
     t.KW = KW;
     t.RW = kQmmWarps / KW;
@@ -246,6 +232,8 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
     t.split = 1;
     if (p.mode != kQmmUp)
       while (t.split < 8 && tiles * t.split * 2 <= slots && most_units >= (int64_t)t.split * 2 * KW) t.split *= 2;
+    const int ts = tune(kTuneQmmSplit, 0);
+    if (p.mode != kQmmUp && (ts == 1 || ts == 2 || ts == 4 || ts == 8) && most_units >= (int64_t)ts * KW) t.split = ts;
     const size_t slot = qmm_slot_bytes(t.RW * f.MT, pitch, p.TS);
     const bool in_ring = p.mode != kQmmDown && t.split > 1;
     // buffers of partial sums: none where one column holds the whole K, two so

@@ -338,15 +338,15 @@ __device__ __forceinline__ T qmm_lds(uint32_t off) {
 // Where this lane (column n = lane / 4) reads the B operands of NI n-tiles; a
 // record of zeros stands for absent tokens and the fourth limb.
 //   LIMBS == false: tile j holds tokens 2j and 2j + 1, column n limb n % 4 of token 2j + n / 4
-//   LIMBS == true:  tile j holds limb j % 3 of tokens 8 (j / 3) + n
+//   LIMBS == true:  tile j holds limb j of token first + n
 template <int NI, bool LIMBS>
 struct QmmB {
   uint32_t even[NI], odd[NI];  // units 4i + c of even and odd i, less 64 i
   uint32_t t[NI];              // the sums T
-  __device__ __forceinline__ QmmB(uint32_t recs, uint32_t zeros, int count, int n, int c) {
+  __device__ __forceinline__ QmmB(uint32_t recs, uint32_t zeros, int first, int count, int n, int c) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const int tok = LIMBS ? 8 * (j / 3) + n : 2 * j + (n >> 2), limb = LIMBS ? j % 3 : n & 3;
+      const int tok = first + (LIMBS ? n : 2 * j + (n >> 2)), limb = LIMBS ? j : n & 3;
       const uint32_t r = tok < count && limb < 3 ? recs + tok * kQmmRecPitch : zeros;
       const int at = limb < 3 ? limb : 0, flip = (at & 1) * 64;
       even[j] = r + 256 * at + 16 * c + flip;
@@ -359,9 +359,9 @@ struct QmmB {
   }
 };
 // Values of a lane per row half: one of a token's two limb pairs per tile, or
-// (LIMBS) two whole tokens, 8g + 2c and 8g + 2c + 1, per three tiles.
+// (LIMBS, three tiles) two whole tokens, 2c and 2c + 1.
 template <int NI, bool LIMBS>
-constexpr int kQmmVals = LIMBS ? NI / 3 * 2 : NI;
+constexpr int kQmmVals = LIMBS ? 2 : NI;
 // u += k * (the tiles' sums f as values)
 template <int NI, bool LIMBS>
 __device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], const float (&k)[2], const float (&f)[NI][4]) {
@@ -369,9 +369,9 @@ __device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], cons
   for (int r = 0; r < 2; ++r) {
     if constexpr (LIMBS) {
 #pragma unroll
-      for (int q = 0; q < NI / 3 * 2; ++q) {
-        const int j = q / 2 * 3, e = 2 * r + (q & 1);
-        u[q][r] = fmaf(k[r], fmaf(65536.0f, f[j + 2][e], fmaf(256.0f, f[j + 1][e], f[j][e])), u[q][r]);
+      for (int q = 0; q < 2; ++q) {
+        const int e = 2 * r + q;
+        u[q][r] = fmaf(k[r], fmaf(65536.0f, f[2][e], fmaf(256.0f, f[1][e], f[0][e])), u[q][r]);
       }
     } else {
 #pragma unroll
@@ -687,38 +687,52 @@ __device__ __forceinline__ void qmm_route(const QmmParams& p, int m, int lane, i
   const double* l = p.logits + (int64_t)m * p.E;
   const bool sig = p.score == NSQ_SCORE_SIGMOID_NORM;
   const bool by_score = sig || p.sel_bias;  // else the order of the logits is that of the scores
-  double mx = -INFINITY, sum = 0.0;
+  double v[EP];  // logits, then scores where the order needs them, of experts lane, lane + 32, ...
+  double mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < EP; ++i) {
+    v[i] = 0.0;
+    if (lane + 32 * i < p.E) {
+      v[i] = l[lane + 32 * i];
+      mx = fmax(mx, v[i]);
+    }
+  }
+  double sum = 1.0;
   if (!sig) {
-    for (int e = lane; e < p.E; e += 32) mx = fmax(mx, l[e]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (p.score == NSQ_SCORE_SOFTMAX || by_score) {
+      sum = 0.0;
+#pragma unroll 1
       for (int e = lane; e < p.E; e += 32) sum += exp(l[e] - mx);
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
   }
-  auto score = [&](double v) { return sig ? 1.0 / (1.0 + exp(-v)) : sum > 0.0 ? exp(v - mx) / sum : exp(v - mx); };
+  auto score = [&](double x) { return sig ? 1.0 / (1.0 + exp(-x)) : exp(x - mx) / sum; };
   uint64_t key[EP];
 #pragma unroll
   for (int i = 0; i < EP; ++i) {
-    const int e = lane + 32 * i;
     key[i] = 0;
-    if (e < p.E) {
-      const double v = l[e];
-      key[i] = qmm_key(by_score ? score(v) + (p.sel_bias ? (double)p.sel_bias[e] : 0.0) : v);
+    if (32 * i < p.E) {
+      const int e = lane + 32 * i;
+      if (by_score) v[i] = score(v[i]);
+      if (e < p.E) key[i] = qmm_key(by_score && p.sel_bias ? v[i] + (double)p.sel_bias[e] : v[i]);
     }
   }
-  double total = 0.0, mine = 0.0;  // lane j keeps pick j's score
+  double mine = 0.0;  // lane j keeps pick j's score (or logit)
   int mine_id = 0;
+#pragma unroll 1
   for (int j = 0; j < p.top_k; ++j) {
     uint64_t best = 0;
+    double at_best = 0.0;
     int at = 0x7FFFFFFF;
 #pragma unroll
     for (int i = 0; i < EP; ++i) {
       if (key[i] > best) {
         best = key[i];
         at = lane + 32 * i;
+        at_best = v[i];
       }
     }
     const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
@@ -729,16 +743,19 @@ __device__ __forceinline__ void qmm_route(const QmmParams& p, int m, int lane, i
     for (int i = 0; i < EP; ++i) {
       if (lane + 32 * i == id) key[i] = 0;
     }
-    const double s = score(l[id]);
-    total += s;
+    const double got = __shfl_sync(0xffffffffu, at_best, id & 31);
     if (lane == j) {
-      mine = s;
+      mine = got;
       mine_id = id;
     }
   }
+  const double s = by_score ? mine : score(mine);
+  double total = lane < p.top_k ? s : 0.0;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane < p.top_k) {
     ids[lane] = mine_id;
-    wts[lane] = (float)((p.score == NSQ_SCORE_SOFTMAX ? mine : mine / total) * (double)p.scale);
+    wts[lane] = (float)((p.score == NSQ_SCORE_SOFTMAX ? s : s / total) * (double)p.scale);
   }
 }
 
@@ -817,12 +834,13 @@ __device__ __forceinline__ QmmLists qmm_load_lists(const QmmParams& p, uint8_t* 
   L.plist = reinterpret_cast<int32_t*>(L.groups + P);
   L.pwts = reinterpret_cast<float*>(L.plist + P);
   L.ptok = reinterpret_cast<int32_t*>(L.pwts + P);
-  L.ngroups = *p.ngroups;
+  // from L2: kQmmDown reads them while the kernel before it still runs
+  L.ngroups = __ldcg(p.ngroups);
   for (int q = threadIdx.x; q < P; q += kQmmThreads) {  // entries past the lists' ends are not used
-    reinterpret_cast<int4*>(L.groups)[q] = reinterpret_cast<const int4*>(p.groups)[q];
-    L.plist[q] = p.plist[q];
-    L.ptok[q] = p.ptok[q];
-    L.pwts[q] = p.pwts[q];
+    reinterpret_cast<int4*>(L.groups)[q] = __ldcg(reinterpret_cast<const int4*>(p.groups) + q);
+    L.plist[q] = __ldcg(p.plist + q);
+    L.ptok[q] = __ldcg(p.ptok + q);
+    L.pwts[q] = __ldcg(p.pwts + q);
   }
   return L;
 }
@@ -851,17 +869,25 @@ inline size_t qmm_lists_bytes(int P) { return (size_t)P * (sizeof(QmmGroup) + 12
 
 // Bias, activation and residual (kQmmLinear), or the residual alone
 // (kQmmDown), for one finished sum.
-static __device__ __noinline__ void qmm_store(const QmmParams& p, int col, int row, float v) {
+struct QmmAdd {
+  float bias, residual;
+};
+__device__ __forceinline__ QmmAdd qmm_adds(const QmmParams& p, int col, int row) {
+  QmmAdd a{0.0f, 0.0f};
   const int64_t at = (int64_t)col * p.n + row;
-  if (p.mode == kQmmLinear) {
-    if (p.bias) v += p.bias[row];
-    v = qmm_act(v, p.act);
-  }
+  if (p.mode == kQmmLinear && p.bias) a.bias = p.bias[row];
+  if (p.residual)
+    a.residual = p.dtype == NSQ_OUT_F32 ? static_cast<const float*>(p.residual)[at]
+                                        : __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[at]);
+  return a;
+}
+static __device__ __noinline__ void qmm_store(const QmmParams& p, int col, int row, float v, QmmAdd a) {
+  const int64_t at = (int64_t)col * p.n + row;
+  if (p.mode == kQmmLinear) v = qmm_act(v + a.bias, p.act);
+  v += a.residual;
   if (p.dtype == NSQ_OUT_F32) {
-    if (p.residual) v += static_cast<const float*>(p.residual)[at];
     static_cast<float*>(p.y)[at] = v;
   } else {
-    if (p.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[at]);
     static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
   }
 }
@@ -943,8 +969,12 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   if constexpr (MODE == kQmmLinear) {
     L.ngroups = 1;
   } else {
-    qmm_dep_wait();
-    qmm_dep_launch();
+    if constexpr (MODE == kQmmUp) {
+      qmm_dep_wait();
+      qmm_dep_launch();
+    }
+    // kQmmDown does not wait here: the lists' kernel was complete before any
+    // CTA of kQmmUp let this kernel start
     L = qmm_load_lists(p, smem + zeros + kQmmRec);
   }
   __syncthreads();
@@ -1041,7 +1071,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       if (valid) {
         for (int64_t i = e; i < end; ++i) dst[i - a] = w[i];
       }
-      fence_proxy_async_smem();
+      if (e < end) fence_proxy_async_smem();
       const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
       if (lane == 0) mbar_arrive_expect_tx(bar, total);
       __syncwarp();
@@ -1062,8 +1092,8 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     }
   };
   const bool keeper = rw == (kw & (RW - 1));  // refills the column's records
-  if constexpr (MODE == kQmmLinear) {
-    // the weights do not depend on the kernels before; records, residual and
+  if constexpr (MODE != kQmmUp) {
+    // the weights do not depend on the kernel before; records, residual and
     // outputs do
     const QmmCursor start = pc;
     const bool had = more;
@@ -1200,16 +1230,16 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
           }
           o[h] = slot + my_rows + r * pitch + mis;
         }
-        auto unit = [&](auto N, auto Limbs) {
+        auto unit = [&](auto N, auto Limbs, int first) {
           constexpr int ni = decltype(N)::value;
           constexpr bool limbs = decltype(Limbs)::value;
           constexpr int nq = kQmmVals<ni, limbs>;
-          const QmmB<ni, limbs> B(slot + recs_at, zeros, count, lr, lc);
+          const QmmB<ni, limbs> B(slot + recs_at, zeros, first, count, lr, lc);
           float v[nq][2];
           qmm_unit<TYPE, LAYOUT, ni, limbs>(o, lc, B, nv, v);
 #pragma unroll
           for (int q = 0; q < nq; ++q) {
-            const int tk = limbs ? 8 * (q >> 1) + 2 * lc + (q & 1) : 2 * q + (lc >> 1);
+            const int tk = first + (limbs ? 2 * lc + q : 2 * q + (lc >> 1));
             float s = tk < count ? qmm_lds<float>(slot + recs_at + tk * kQmmRecPitch + kQmmRecS) : 0.0f;
             if (!limbs && (lc & 1)) s *= 65536.0f;  // limbs 2, 3 of the token
             float y0 = s * v[q][0], y1 = s * v[q][1];
@@ -1229,9 +1259,12 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
                   to[8 * (lc & 1)] += w * (lc & 1 ? y1 : y0);
                 }
               }
-            } else {
+            } else if (NQ <= 2 || first == 0) {
               tot[t][q][0] += y0;
               tot[t][q][1] += y1;
+            } else {
+              tot[t][NQ - 2 + (q & 1)][0] += y0;
+              tot[t][NQ - 2 + (q & 1)][1] += y1;
             }
           }
         };
@@ -1239,13 +1272,13 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         using std::false_type;
         using std::true_type;
         if (TC == 2 || count <= 2) {
-          unit(integral_constant<int, 1>{}, false_type{});
+          unit(integral_constant<int, 1>{}, false_type{}, 0);
         } else if (TC == 4 || count <= 4) {
-          if constexpr (TC > 2) unit(integral_constant<int, 2>{}, false_type{});
-        } else if (TC == 8 || count <= 8) {
-          if constexpr (TC > 4) unit(integral_constant<int, 3>{}, true_type{});
-        } else {
-          if constexpr (TC > 8) unit(integral_constant<int, 6>{}, true_type{});
+          if constexpr (TC > 2) unit(integral_constant<int, 2>{}, false_type{}, 0);
+        } else if constexpr (TC > 4) {
+          // eight tokens at a time (all sixteen at once would not fit the registers)
+#pragma unroll 1
+          for (int first = 0; first < (TC > 8 ? count : 8); first += 8) unit(integral_constant<int, 3>{}, true_type{}, first);
         }
       }
       __syncwarp();
@@ -1279,7 +1312,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         __syncwarp();
       } else if constexpr (MODE == kQmmLinear) {
         each_sum(cnt, [&](int tk, int r, float v) {
-          if (tk < cnt && row0 + r < p.n) qmm_store(p, tk, row0 + r, v);
+          if (tk < cnt && row0 + r < p.n) qmm_store(p, tk, row0 + r, v, qmm_adds(p, tk, row0 + r));
         });
       }
       continue;
@@ -1314,7 +1347,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
             const float gate = sum_kw(col, r), up = sum_kw(col, r + OR);
             p.h[(int64_t)L.plist[L.groups[c.g].start + col] * p.n + row0 + r] = qmm_act(gate, p.act) * up;
           } else {
-            qmm_store(p, col, row0 + r, sum_kw(col, r));
+            qmm_store(p, col, row0 + r, sum_kw(col, r), qmm_adds(p, col, row0 + r));
           }
         }
       }
@@ -1346,8 +1379,16 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         for (int k = 1; k < KW; ++k) v += q[k * ys_warp];
         q[0] = v;
       }
+      // what the first output adds is under way while the ranks meet
+      const int i0 = rank * kQmmThreads + threadIdx.x;
+      QmmAdd add{};
+      if (i0 < outs) {
+        int col, r;
+        place(i0, col, r);
+        if (cta * tile_rows + r < p.n) add = qmm_adds(p, col, cta * tile_rows + r);
+      }
       qmm_cluster_sync();
-      for (int i = rank * kQmmThreads + threadIdx.x; i < outs; i += p.split * kQmmThreads) {
+      for (int i = i0; i < outs; i += p.split * kQmmThreads) {
         int col, r;
         const float* q = place(i, col, r);
         float part[8];
@@ -1357,7 +1398,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
 #pragma unroll
         for (int k = 1; k < 8; ++k) v += part[k];
         const int row = cta * tile_rows + r;
-        if (row < p.n) qmm_store(p, col, row, v);
+        if (row < p.n) qmm_store(p, col, row, v, i == i0 ? add : qmm_adds(p, col, row));
       }
       qmm_cluster_sync();  // every rank has read the others' sums
     }
