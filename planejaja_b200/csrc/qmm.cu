@@ -18,6 +18,8 @@ int device_check(int* num_sms);
 
 constexpr int kPrepThreads = 32 * kQmmWarps;
 constexpr int kRouteTok = 8;  // tokens of one CTA's logits
+constexpr int kQmmMaxCtas = 320;  // of a product: two per SM
+constexpr size_t kTicketBytes = (size_t)kQmmMaxCtas * kQmmWarps * 4;
 
 // Activation records of rows x nsb units, one warp each.
 template <typename T>
@@ -33,9 +35,11 @@ __device__ __forceinline__ void make_records(const T* __restrict__ x, int64_t ro
 
 template <typename T>
 __global__ void __launch_bounds__(kPrepThreads) qmm_prep_kernel(const T* __restrict__ x, int64_t rows, int64_t K,
-                                                                int nsb, int order, uint8_t* __restrict__ recs) {
+                                                                int nsb, int order, uint8_t* __restrict__ recs,
+                                                                int32_t* __restrict__ tickets) {
   qmm_dep_wait();
   qmm_dep_launch();
+  for (int i = blockIdx.x * kPrepThreads + threadIdx.x; i < (int)(kTicketBytes / 4); i += gridDim.x * kPrepThreads) tickets[i] = 0;
   make_records(x, rows, K, nsb, order, recs, blockIdx.x);
 }
 
@@ -45,7 +49,7 @@ __device__ __forceinline__ float4 load4(const float* p, bool wide) {
 
 // First kernel of a mixture-of-experts call: the first nlog CTAs compute the
 // router's logits (one expert, eight tokens each), the others the activation
-// records; they also zero kQmmUp's counters.  With given picks the first CTA
+// records; they also zero the counters of the products.  With given picks the first CTA
 // lists them by expert.  Two experts' logits may lie arbitrarily close, and a
 // pick that flips changes the output by whole experts: products of f32 are
 // exact in f64, and the sums are f64.
@@ -65,6 +69,9 @@ __global__ void __launch_bounds__(kPrepThreads) moe_logits_kernel(const __grid_c
     for (int64_t i = (int64_t)(blockIdx.x - nlog) * kPrepThreads + threadIdx.x; i < counters;
          i += (int64_t)(gridDim.x - nlog) * kPrepThreads)
       p.done[i] = 0;
+    for (int i = (blockIdx.x - nlog) * kPrepThreads + threadIdx.x; i < (int)(2 * kTicketBytes / 4);
+         i += (gridDim.x - nlog) * kPrepThreads)
+      p.tickets[i] = 0;
     return;
   }
   if (!router) {
@@ -143,15 +150,15 @@ static int launch_pdl(void (*kern)(Params...), int64_t grid, int threads, size_t
 }
 
 template <typename T>
-static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* recs, cudaStream_t st) {
+static int launch_prep(const T* x, int64_t rows, int64_t K, int order, uint8_t* recs, int32_t* tickets, cudaStream_t st) {
   const int nsb = (int)((K + 255) / 256);
   return launch_pdl(qmm_prep_kernel<T>, (rows * nsb + kQmmWarps - 1) / kQmmWarps, kPrepThreads, 0, st, x, rows, K, nsb,
-                    order, recs);
+                    order, recs, tickets);
 }
 
 static int launch_route(const QmmParams& p, const float* x, const float* router, int64_t K, int order, uint8_t* recs,
                         double* logits, cudaStream_t st) {
-  const size_t lists = (size_t)p.M * p.top_k * (8 + sizeof(QmmGroup));  // at most 24 KB
+  const size_t lists = ((size_t)3 * p.M * p.top_k + p.E) * 4;  // at most 14 KB
   const int nlog = router ? p.E * ((p.M + kRouteTok - 1) / kRouteTok) : 1;
   const int64_t rec_ctas = ((int64_t)p.M * p.nsb + kQmmWarps - 1) / kQmmWarps;
   const int rc = launch_pdl(moe_logits_kernel, nlog + rec_ctas, kPrepThreads, router ? 0 : lists, st, p, x, router, K,
@@ -207,18 +214,19 @@ static bool encode_rows(CUtensorMap* map, const uint8_t* w, int64_t rows, int64_
 static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream_t st, int num_sms) {
   const QmmShape f = qmm_shape(type, p.TS);
   const int64_t most_units = p.mode == kQmmDown ? groups * p.nsb : p.nsb;
-  const int64_t slots = 2 * (int64_t)num_sms;
+  const int64_t slots = 2 * (int64_t)num_sms < kQmmMaxCtas ? 2 * (int64_t)num_sms : kQmmMaxCtas;
   const int P = p.mode == kQmmLinear ? 0 : p.M * p.top_k;
-  const size_t fixed = kQmmCtl + kQmmRec + qmm_lists_bytes(P);
+  const size_t fixed = kQmmCtl + qmm_lists_bytes(P);
   const size_t ys = (size_t)kQmmWarps * p.YC * 16 * f.MT * 4;
   const int pitch = p.rb % 16 == 0 ? f.PA : f.PG;
-  // Columns of K per CTA (KW), the rest of the 8 warps being row tiles: the
-  // choice with the least time by a simple model.  A CTA's work is its rounds
-  // of tiles x the bytes of a tile, the records of a unit being fetched once
-  // for its RW row tiles; a K split over a cluster fills CTA slots that the
-  // tiles leave empty, as long as every column keeps a unit.
+  // Columns of K per CTA (KW), the rest of the 8 warps being row tiles, and
+  // whether tasks are divided: the choice with the least time by a simple
+  // model.  A CTA's time is its steps x (the bytes of its rows, and those of
+  // the records that its row tiles share), and about three steps to put
+  // divided tasks together.
   double best = 0;
   size_t smem = 0;
+  int64_t grid = 0;
   for (int KW = 1; KW <= kQmmWarps; KW *= 2) {
     if (KW > 1 && KW / 2 >= most_units) break;
     if (const int only = tune(kTuneQmmKW, 0)) {
@@ -227,43 +235,40 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
     QmmParams t = p;
     t.KW = KW;
     t.RW = kQmmWarps / KW;
-    const int64_t rows = (int64_t)(p.mode == kQmmUp ? 8 : 16) * f.MT * t.RW;
-    const int64_t tiles = (p.n + rows - 1) / rows;
-    t.split = 1;
-    if (p.mode != kQmmUp)
-      while (t.split < 8 && tiles * t.split * 2 <= slots && most_units >= (int64_t)t.split * 2 * KW) t.split *= 2;
-    const int ts = tune(kTuneQmmSplit, 0);
-    if (p.mode != kQmmUp && (ts == 1 || ts == 2 || ts == 4 || ts == 8) && most_units >= (int64_t)ts * KW) t.split = ts;
     const size_t slot = qmm_slot_bytes(t.RW * f.MT, pitch, p.TS);
-    const bool in_ring = p.mode != kQmmDown && t.split > 1;
-    // buffers of partial sums: none where one column holds the whole K, two so
-    // that a task's are joined while the next one runs
-    t.PB = p.mode != kQmmDown && t.split == 1 && KW == 1 ? 0 : t.split > 1 ? 1 : 2;
-    if (p.mode == kQmmDown && t.PB == 2 && fixed + 2 * ys + 2 * KW * slot > (size_t)kQmmSmemHalf) t.PB = 1;
-    const size_t sums = (in_ring ? 0 : p.mode == kQmmUp && t.PB == 0 ? 1 : t.PB) * ys;
+    // two buffers of partial sums let a task's be joined while the next runs
+    t.PB = KW > 1 && fixed + 2 * ys + 2 * KW * slot <= (size_t)kQmmSmemHalf ? 2 : 1;
     t.stages = kQmmMaxStages;
-    while (t.stages > 2 && fixed + sums + t.stages * KW * slot > (size_t)kQmmSmemHalf) --t.stages;
-    const size_t need = fixed + sums + t.stages * KW * slot;
-    if (need > (size_t)kQmmSmemMax || (in_ring && ys > t.stages * KW * slot)) continue;
-    const int64_t here = need > (size_t)kQmmSmemHalf ? num_sms : slots;  // CTAs at a time
-    // (of the most groups there can be, an expert's share of the picks are fewer)
-    const int64_t ctas = tiles * (p.mode == kQmmUp ? (groups < p.E ? groups : p.E) : 1) * t.split;
-    const int64_t rounds = (ctas + here - 1) / here;
-    const double bytes = 16.0 * f.MT * t.RW * pitch + (p.TS < 4 ? p.TS : 0.5 * p.TS) * kQmmRec;
-    const double time = (double)rounds / t.split * bytes * (here == slots ? 1.0 : 0.6);
-    if (smem == 0 || time < best) {
-      best = time;
-      smem = need;
-      p.KW = t.KW;
-      p.RW = t.RW;
-      p.split = t.split;
-      p.PB = t.PB;
-      p.stages = t.stages;
+    while (t.stages > 2 && fixed + t.PB * ys + t.stages * KW * slot > (size_t)kQmmSmemHalf) --t.stages;
+    const size_t need = fixed + t.PB * ys + t.stages * KW * slot;
+    if (need > (size_t)kQmmSmemMax) continue;
+    const int64_t here = need > (size_t)kQmmSmemHalf ? slots / 2 : slots;  // CTAs at a time
+    const int64_t rows = (int64_t)(p.mode == kQmmUp ? 8 : 16) * f.MT * t.RW;
+    // (an expert's share of the picks usually is one group)
+    const int64_t tasks = (p.n + rows - 1) / rows * (p.mode == kQmmUp ? (groups < p.E ? groups : p.E) : 1);
+    const int64_t units = p.mode == kQmmDown ? (groups < p.E ? groups : p.E) * p.nsb : p.nsb;
+    const int64_t st = (units + KW - 1) / KW;
+    const double bytes = KW * (16.0 * f.MT * t.RW * pitch + (p.TS < 4 ? p.TS : 0.5 * p.TS) * kQmmRec) / here;
+    for (int whole = 1; whole >= 0; --whole) {
+      const int only = tune(kTuneQmmSplit, -1);
+      if (only >= 0 && whole == (only > 0)) continue;
+      const int64_t steps = whole ? (tasks + here - 1) / here * st : (tasks * st + here - 1) / here + 3;
+      const double time = steps * bytes;
+      if (smem == 0 || time < best) {
+        best = time;
+        smem = need;
+        p.KW = t.KW;
+        p.RW = t.RW;
+        p.PB = t.PB;
+        p.stages = t.stages;
+        p.whole = whole;
+        grid = here;
+        if (whole && p.mode != kQmmUp && tasks < grid) grid = tasks;
+        if (!whole && p.mode != kQmmUp && tasks * st < grid) grid = tasks * st;
+      }
     }
   }
   if (smem == 0) return NSQ_ERR_SHAPE;
-  const int64_t tile_rows = (int64_t)(p.mode == kQmmUp ? 8 : 16) * f.MT * p.RW;
-  const int64_t tiles = (p.n + tile_rows - 1) / tile_rows;
   // TMA boxes where every row starts 16-byte aligned (experts and tensors then do too)
   alignas(64) CUtensorMap maps[2] = {};
   const int64_t rows = p.wbytes / p.rb;
@@ -274,8 +279,6 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
     if (!encode_rows(&maps[0], p.w0, rows, p.rb, box_rows, f.PA)) return NSQ_ERR_CUDA;
     if (p.mode == kQmmUp && !encode_rows(&maps[1], p.w1, rows, p.rb, box_rows, f.PA)) return NSQ_ERR_CUDA;
   }
-  const int64_t tasks = tiles * (p.mode == kQmmUp ? groups : 1);
-  const int64_t grid = (p.split > 1 || tasks < slots ? tasks : slots) * p.split;
   switch (type) {
     case NSQ_TYPE_Q4_K: return launch_qmm_q4k(layout, p, maps, (int)grid, smem, st);
     case NSQ_TYPE_Q5_K: return launch_qmm_q5k(layout, p, maps, (int)grid, smem, st);
@@ -287,12 +290,21 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
 }
 
 static int64_t units_of(int64_t K) { return (K + 255) / 256; }
+// Workspace of divided tasks: two parts of up to 8 row tiles per CTA, tickets.
+static size_t parts_bytes(int64_t tokens, int64_t TS) {
+  return (size_t)kQmmMaxCtas * 2 * kQmmWarps * (TS > 4 ? 16 : 32) * tokens * 4;
+}
 static bool act_ok(int act) { return act >= NSQ_ACT_NONE && act <= NSQ_ACT_RELU; }
 
 // Workspace of a mixture-of-experts call, in this order.
 struct MoeSpace {
-  size_t logits, recs_x, h, recs_h, groups, plist, pwts, ptok, ngroups, done, total;
+  size_t logits, recs_x, h, recs_h, groups, plist, pwts, ptok, ngroups, done, tickets, parts, total;
 };
+// Tokens of a group: 16, or 8 where an expert has 4 or fewer on average.
+static int64_t moe_group(int64_t E, int64_t M, int64_t top_k) {
+  const int64_t cap = M * top_k <= 4 * E ? 8 : kQmmMaxTok;
+  return M < cap ? M : cap;
+}
 static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t top_k) {
   MoeSpace s{};
   const int64_t P = M * top_k;
@@ -312,6 +324,8 @@ static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t to
   s.ptok = take((size_t)P * 4);
   s.ngroups = take(4);
   s.done = take((size_t)(P * units_of(F)) * 4);
+  s.tickets = take(2 * kTicketBytes);  // of both products
+  s.parts = take(parts_bytes(M, moe_group(E, M, top_k)));
   s.total = at;
   return s;
 }
@@ -352,9 +366,9 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   QmmParams p{};
   p.M = (int)M;
   p.top_k = (int)top_k;
-  // tokens of a group: 16, or 8 where an expert has 4 or fewer on average
-  const int64_t cap = M * top_k <= 4 * E ? 8 : kQmmMaxTok;
-  p.TS = (int)(M < cap ? M : cap);
+  p.TS = (int)moe_group(E, M, top_k);
+  p.parts = reinterpret_cast<float*>(ws + s.parts);
+  p.tickets = reinterpret_cast<int32_t*>(ws + s.tickets);
   p.E = (int)E;
   p.score = w_router ? score : -1;
   p.logits = logits;
@@ -391,6 +405,7 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   if ((rc = run_qmm(p, moe->type_in, moe->layout_in, P, st, num_sms))) return rc;
 
   p.mode = kQmmDown;
+  p.tickets += kTicketBytes / 4;
   p.YC = p.M;
   p.n = D;
   p.K = F;
@@ -412,9 +427,11 @@ using namespace nsq;
 
 extern "C" {
 
+static size_t linear_records(int64_t M, int64_t K) { return ((size_t)(M * units_of(K)) * kQmmRec + 255) & ~size_t(255); }
+
 size_t nsq_linear_workspace_size(int64_t M, int64_t K) {
   if (M < 1 || M > NSQ_GEMV_MAX_M || K < 1) return 0;
-  return (size_t)(M * units_of(K)) * kQmmRec;
+  return linear_records(M, K) + kTicketBytes + parts_bytes(M, M);
 }
 
 int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, const float* bias, int act,
@@ -436,11 +453,13 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* recs = static_cast<uint8_t*>(workspace);
   const int order = qmm_order(ggml_type, q6k_layout);
-  rc = dtype == NSQ_OUT_F32
-           ? launch_prep(static_cast<const float*>(x), M, K, order, recs, st)
-           : launch_prep(static_cast<const __nv_bfloat16*>(x), M, K, order, recs, st);
-  if (rc) return rc;
   QmmParams p{};
+  p.tickets = reinterpret_cast<int32_t*>(recs + linear_records(M, K));
+  p.parts = reinterpret_cast<float*>(recs + linear_records(M, K) + kTicketBytes);
+  rc = dtype == NSQ_OUT_F32
+           ? launch_prep(static_cast<const float*>(x), M, K, order, recs, p.tickets, st)
+           : launch_prep(static_cast<const __nv_bfloat16*>(x), M, K, order, recs, p.tickets, st);
+  if (rc) return rc;
   p.mode = kQmmLinear;
   p.M = p.TS = p.YC = (int)M;
   p.top_k = 1;

@@ -205,7 +205,7 @@ struct QmmGroup {
 enum QmmMode : int { kQmmLinear = 0, kQmmUp = 1, kQmmDown = 2 };
 
 struct QmmParams {
-  int mode, RW, KW, stages, split;
+  int mode, RW, KW, stages;
   int TS;        // token slots of a unit (the largest group)
   int YC;        // columns of the partial sums: TS, or M for kQmmDown
   int M, top_k;  // tokens; picks per token
@@ -213,7 +213,10 @@ struct QmmParams {
   int nsb;       // units of a weight row: ceil(K / 256)
   int nblk;      // K / 32
   int rows_aligned;  // every row starts 16-byte aligned: TMA boxes
-  int PB;            // buffers of partial sums (0: outputs straight from registers)
+  int PB;            // buffers of partial sums
+  int whole;         // tasks are not divided
+  float* parts;      // sums of divided tasks, [CTA][2][row tile][YC][WR]
+  int32_t* tickets;  // steps of them that are done, [CTA][row tile], zeroed by the kernel before
   int64_t n, K, rb;          // rows of one expert, K, bytes of a row
   const uint8_t* w0;         // weights (kQmmUp: gate)
   const uint8_t* w1;         // kQmmUp: up
@@ -311,7 +314,7 @@ static __device__ __noinline__ float qmm_act(float v, int act) {
 // Two row tiles share their B operands and bookkeeping; the wider formats
 // have one, for the depth of the ring.
 template <int TYPE> struct QmmFmt;
-template <> struct QmmFmt<NSQ_TYPE_Q4_K> { static constexpr int CB = 144, PA = 160, PG = 160, MT = 2; };
+template <> struct QmmFmt<NSQ_TYPE_Q4_K> { static constexpr int CB = 144, PA = 144, PG = 144, MT = 2; };
 template <> struct QmmFmt<NSQ_TYPE_Q5_K> { static constexpr int CB = 176, PA = 176, PG = 176, MT = 2; };
 template <> struct QmmFmt<NSQ_TYPE_Q6_K> { static constexpr int CB = 210, PA = 240, PG = 240, MT = 1; };
 template <> struct QmmFmt<NSQ_TYPE_Q4_0> { static constexpr int CB = 144, PA = 144, PG = 176, MT = 2; };
@@ -335,27 +338,38 @@ __device__ __forceinline__ T qmm_lds(uint32_t off) {
   return *reinterpret_cast<const T*>(qmm_smem + off);
 }
 
-// Where this lane (column n = lane / 4) reads the B operands of NI n-tiles; a
-// record of zeros stands for absent tokens and the fourth limb.
-//   LIMBS == false: tile j holds tokens 2j and 2j + 1, column n limb n % 4 of token 2j + n / 4
+// Where this lane (column n = lane / 4) reads the B operands of n-tile j.
+//   LIMBS == false: tile j holds tokens first + 2j and first + 2j + 1, column n
+//                   limb n % 4 of token first + 2j + n / 4 (limb 3: limb 0
+//                   again, its sums are not used)
 //   LIMBS == true:  tile j holds limb j of token first + n
-template <int NI, bool LIMBS>
+// Columns of absent tokens hold what was there; their sums are not used.
+template <bool LIMBS>
 struct QmmB {
-  uint32_t even[NI], odd[NI];  // units 4i + c of even and odd i, less 64 i
-  uint32_t t[NI];              // the sums T
-  __device__ __forceinline__ QmmB(uint32_t recs, uint32_t zeros, int first, int count, int n, int c) {
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int tok = first + (LIMBS ? n : 2 * j + (n >> 2)), limb = LIMBS ? j : n & 3;
-      const uint32_t r = tok < count && limb < 3 ? recs + tok * kQmmRecPitch : zeros;
-      const int at = limb < 3 ? limb : 0, flip = (at & 1) * 64;
-      even[j] = r + 256 * at + 16 * c + flip;
-      odd[j] = r + 256 * at + 16 * c - flip;
-      t[j] = r + kQmmRecT + 32 * at + 8 * c;
+  uint32_t base[2];  // units 4i + c of even and odd i (less 64 i), of the limb with its units in order
+  uint32_t t;        // the sums T
+  float k256;        // what the second limb of a pair of columns counts
+  __device__ __forceinline__ QmmB(uint32_t recs, int first, int n, int c) {
+    if constexpr (LIMBS) {
+      const uint32_t r = recs + (first + n) * kQmmRecPitch;
+      base[0] = base[1] = r + 16 * c;
+      t = r + kQmmRecT + 8 * c;
+    } else {
+      const int limb = (n & 3) == 3 ? 0 : n & 3, flip = (limb & 1) * 64;
+      const uint32_t r = recs + (first + (n >> 2)) * kQmmRecPitch;
+      base[0] = r + 256 * limb + 16 * c + flip;
+      base[1] = r + 256 * limb + 16 * c - flip;
+      t = r + kQmmRecT + 32 * limb + 8 * c;
     }
+    k256 = c & 1 ? 0.0f : 256.0f;
   }
   __device__ __forceinline__ uint4 unit(int j, int i) const {
-    return qmm_lds<uint4>(((i & 1) ? odd[j] : even[j]) + 64 * i);
+    // the middle limb's units are exchanged
+    if constexpr (LIMBS) return qmm_lds<uint4>(base[0] + 256 * j + (j == 1 ? 64 * (i ^ 1) : 64 * i));
+    return qmm_lds<uint4>(base[i & 1] + 2 * kQmmRecPitch * j + 64 * i);
+  }
+  __device__ __forceinline__ uint2 sums(int j) const {
+    return qmm_lds<uint2>(t + (LIMBS ? 32 * j : 2 * kQmmRecPitch * j));
   }
 };
 // Values of a lane per row half: one of a token's two limb pairs per tile, or
@@ -364,7 +378,8 @@ template <int NI, bool LIMBS>
 constexpr int kQmmVals = LIMBS ? 2 : NI;
 // u += k * (the tiles' sums f as values)
 template <int NI, bool LIMBS>
-__device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], const float (&k)[2], const float (&f)[NI][4]) {
+__device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], const float (&k)[2], const float (&f)[NI][4],
+                                        float k256) {
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     if constexpr (LIMBS) {
@@ -375,7 +390,7 @@ __device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], cons
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) u[j][r] = fmaf(k[r], fmaf(256.0f, f[j][2 * r + 1], f[j][2 * r]), u[j][r]);
+      for (int j = 0; j < NI; ++j) u[j][r] = fmaf(k[r], fmaf(k256, f[j][2 * r + 1], f[j][2 * r]), u[j][r]);
     }
   }
 }
@@ -424,7 +439,7 @@ __device__ __forceinline__ int qmm_s8(uint32_t w) {
 // lane's weight rows lane / 4 and lane / 4 + 8; c = lane % 4; nv: valid
 // 32-weight blocks (Q4_0, Q8_0).
 template <int TYPE, int LAYOUT, int NI, bool LIMBS>
-__device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const QmmB<NI, LIMBS>& B, int nv,
+__device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const QmmB<LIMBS>& B, int nv,
                                          float (&u)[kQmmVals<NI, LIMBS>][2]) {
 #pragma unroll
   for (int q = 0; q < kQmmVals<NI, LIMBS>; ++q) u[q][0] = u[q][1] = 0.0f;
@@ -433,10 +448,10 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
     float am[NI][4];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const uint2 b = qmm_lds<uint2>(B.t[j]);
+      const uint2 b = B.sums(j);
       qmm_mma_f16(am[j], a0, a1, a2, a3, b.x, b.y);
     }
-    qmm_add<NI, LIMBS>(u, k, am);
+    qmm_add<NI, LIMBS>(u, k, am, B.k256);
   };
   if constexpr (TYPE == NSQ_TYPE_Q4_K || TYPE == NSQ_TYPE_Q5_K) {
     const __half2 k1024 = __float2half2_rn(1024.0f);
@@ -528,7 +543,7 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[j][e] = (float)((TYPE == NSQ_TYPE_Q4_K ? 16 * lo[j][e] : lo[j][e]) + hi[j][e]);
     }
-    qmm_add<NI, LIMBS>(u, d, f);
+    qmm_add<NI, LIMBS>(u, d, f, B.k256);
   } else if constexpr (TYPE == NSQ_TYPE_Q4_0 || TYPE == NSQ_TYPE_Q8_0) {
     constexpr int BB = TYPE == NSQ_TYPE_Q4_0 ? 18 : 34;
     // the sums start at the bits of 1.5 * 2^23: as f32 they are that plus the
@@ -575,7 +590,7 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[j][e] = __int_as_float(acc[e]) - kMagicF;
       }
-      qmm_add<NI, LIMBS>(u, d, f);
+      qmm_add<NI, LIMBS>(u, d, f, B.k256);
     });
   } else {  // Q6_K
     const QmmRow rows[2] = {QmmRow(o[0]), QmmRow(o[1])};
@@ -661,7 +676,7 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[j][e] = (float)sum[j][e];
     }
-    qmm_add<NI, LIMBS>(u, d, f);
+    qmm_add<NI, LIMBS>(u, d, f, B.k256);
   }
 }
 
@@ -682,8 +697,9 @@ __device__ __forceinline__ uint64_t qmm_key(double v) {  // ordered as v; NaN be
 }
 
 // One warp picks token m's experts: ids and weights of top_k picks.
+// EP: experts of a lane.
+template <int EP>
 __device__ __forceinline__ void qmm_route(const QmmParams& p, int m, int lane, int32_t* ids, float* wts) {
-  constexpr int EP = NSQ_MOE_MAX_EXPERTS / 32;
   const double* l = p.logits + (int64_t)m * p.E;
   const bool sig = p.score == NSQ_SCORE_SIGMOID_NORM;
   const bool by_score = sig || p.sel_bias;  // else the order of the logits is that of the scores
@@ -759,16 +775,25 @@ __device__ __forceinline__ void qmm_route(const QmmParams& p, int m, int lane, i
   }
 }
 
-// One CTA builds the lists.  mem: lists and 2 * P ints of scratch.
+// One CTA builds the lists.  mem: 3 P + E ints of shared memory.
 __device__ __forceinline__ void qmm_build_lists(const QmmParams& p, int32_t* mem) {
   const int P = p.M * p.top_k;
   int32_t* ids = mem;
   float* wts = reinterpret_cast<float*>(mem + P);
-  QmmGroup* starts = reinterpret_cast<QmmGroup*>(mem + 2 * P);  // by place in the order of (expert, pick)
+  int32_t* ranks = mem + 2 * P;
+  int32_t* first = mem + 3 * P;  // [E] picks of an expert so far, then its first place
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   if (p.score >= 0) {
     for (int m = warp; m < p.M; m += warps) {
-      qmm_route(p, m, lane, ids + m * p.top_k, wts + m * p.top_k);
+      int32_t* to = ids + m * p.top_k;
+      float* tw = wts + m * p.top_k;
+      if (p.E <= 32) {
+        qmm_route<1>(p, m, lane, to, tw);
+      } else if (p.E <= 128) {
+        qmm_route<4>(p, m, lane, to, tw);
+      } else {
+        qmm_route<NSQ_MOE_MAX_EXPERTS / 32>(p, m, lane, to, tw);
+      }
       __syncwarp();
       if (lane < p.top_k) {
         p.ids[m * p.top_k + lane] = ids[m * p.top_k + lane];
@@ -792,39 +817,51 @@ __device__ __forceinline__ void qmm_build_lists(const QmmParams& p, int32_t* mem
       wts[q] = w;
     }
   }
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) first[e] = 0;
   __syncthreads();
-  // place of a pick: the number of valid picks that come before it; groups
-  // start at every TS-th pick of an expert
-  for (int q = threadIdx.x; q < P; q += blockDim.x) {
-    const int e = ids[q];
-    if (e < 0) continue;
-    int pos = 0, rank = 0, same = 0;
-    for (int r = 0; r < P; ++r) {
-      const int o = ids[r];
-      pos += o >= 0 && (o < e || (o == e && r < q));
-      rank += o == e && r < q;
-      same += o == e;
+  if (warp != 0) return;
+  // one warp, 32 picks at a time: a pick's rank among its expert's picks
+  for (int b = 0; b < P; b += 32) {
+    const int q = b + lane, e = q < P ? ids[q] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    int base = 0;
+    if (e >= 0) base = first[e];
+    __syncwarp();
+    if (q < P) ranks[q] = base + __popc(same & ((1u << lane) - 1));
+    if (e >= 0 && lane == __ffs(same) - 1) first[e] = base + __popc(same);
+    __syncwarp();
+  }
+  // picks and groups of the experts before each: groups start at every TS-th
+  // pick of an expert
+  int picks = 0, groups = 0;
+  for (int b = 0; b < p.E; b += 32) {
+    const int e = b + lane, n = e < p.E ? first[e] : 0, m = (n + p.TS - 1) / p.TS;
+    int np = n, ng = m;  // inclusive sums over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, np, o), g = __shfl_up_sync(0xffffffffu, ng, o);
+      if (lane >= o) {
+        np += a;
+        ng += g;
+      }
     }
+    if (e < p.E) {
+      first[e] = picks + np - n;
+      for (int i = 0; i < m; ++i)
+        p.groups[groups + ng - m + i] = QmmGroup{e, picks + np - n + i * p.TS, min(p.TS, n - i * p.TS), 0};
+    }
+    picks += __shfl_sync(0xffffffffu, np, 31);
+    groups += __shfl_sync(0xffffffffu, ng, 31);
+  }
+  __syncwarp();
+  for (int q = lane; q < P; q += 32) {
+    if (ids[q] < 0) continue;
+    const int pos = first[ids[q]] + ranks[q];
     p.plist[pos] = q;
     p.pwts[pos] = wts[q];
     p.ptok[pos] = q / p.top_k;
-    starts[pos] = QmmGroup{e, pos, rank % p.TS == 0 ? min(p.TS, same - rank) : 0, 0};
   }
-  __syncthreads();
-  if (warp == 0) {
-    int valid = 0;
-    for (int q = lane; q < P; q += 32) valid += ids[q] >= 0;
-    valid = __reduce_add_sync(0xffffffffu, valid);
-    int n = 0;
-    for (int b = 0; b < valid; b += 32) {
-      const int q = b + lane;
-      const QmmGroup g = q < valid ? starts[q] : QmmGroup{0, 0, 0, 0};
-      const uint32_t starting = __ballot_sync(0xffffffffu, g.count > 0);
-      if (g.count > 0) p.groups[n + __popc(starting & ((1u << lane) - 1))] = g;
-      n += __popc(starting);
-    }
-    if (lane == 0) *p.ngroups = n;
-  }
+  if (lane == 0) *p.ngroups = groups;
 }
 
 __device__ __forceinline__ QmmLists qmm_load_lists(const QmmParams& p, uint8_t* mem) {
@@ -845,25 +882,11 @@ __device__ __forceinline__ QmmLists qmm_load_lists(const QmmParams& p, uint8_t* 
   return L;
 }
 
-__device__ __forceinline__ uint32_t qmm_cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void qmm_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float qmm_ld_cluster(const float* p, uint32_t rank) {
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-
 // Bytes of a slot: RW tiles of rows at this pitch, then TS records.
 __host__ __device__ inline uint32_t qmm_slot_bytes(int row_tiles, int pitch, int TS) {
-  return (uint32_t)(row_tiles * 16 * pitch + (TS * kQmmRecPitch + 127) / 128 * 128);
+  // whole n-tiles of tokens: absent ones are read too
+  const int tokens = TS <= 2 ? 2 : TS <= 4 ? 4 : TS <= 8 ? 8 : 16;
+  return (uint32_t)(row_tiles * 16 * pitch + (tokens * kQmmRecPitch + 127) / 128 * 128);
 }
 inline size_t qmm_lists_bytes(int P) { return (size_t)P * (sizeof(QmmGroup) + 12); }
 
@@ -892,13 +915,21 @@ static __device__ __noinline__ void qmm_store(const QmmParams& p, int col, int r
   }
 }
 
-// Where a column stands: its task (tile, and the group for kQmmUp), its unit
-// (u, of group g and column sb of K).
+// Where a column stands: its task (tile, and the group for kQmmUp), the step
+// in it, its unit (u, of group g and column sb of K), and the steps that the
+// CTA has left.
 struct QmmCursor {
-  int tile, g, sb, u;
+  int tile, g, s, u, sb, left;
 };
 
 // TC: the most tokens of a group (2, 4, 8 or 16).
+//
+// A task is one tile of output rows (of one group for kQmmUp); its units
+// (group and 256 of K) are dealt to the KW columns in turn, KW a step.  The
+// grid's CTAs share the steps of all tasks evenly, in order, so a CTA may
+// begin and end inside a task; p.whole keeps tasks whole.  A row tile's part
+// of a divided task goes to the workspace, and the last part to arrive adds
+// them up in the order of the CTAs.
 template <int TYPE, int LAYOUT, int TC, int MODE>
 __global__ void __launch_bounds__(kQmmThreads, 2)
     qmm_kernel(const __grid_constant__ QmmParams p, const __grid_constant__ CUtensorMap map0,
@@ -914,6 +945,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   auto* const used = reinterpret_cast<uint64_t(*)[kQmmMaxStages]>(smem + 256);
   auto* const ready = reinterpret_cast<uint64_t(*)[2]>(smem + 512);  // [row tile][buffer]
   auto* const taken = reinterpret_cast<uint64_t(*)[2]>(smem + 640);
+  int* const rows_done = reinterpret_cast<int*>(smem + 768);  // [task % 8] row tiles that stored h
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int KW = p.KW, RW = p.RW, S = p.stages, TS = p.TS, YC = p.YC;
   const int kw = warp & (KW - 1), rw = warp / KW;
@@ -922,16 +954,9 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   const uint32_t slot_bytes = qmm_slot_bytes(RW * MT, pitch, TS);
   const uint32_t recs_at = RW * WR * pitch;  // of a slot
   const uint32_t ring_bytes = S * KW * slot_bytes;
-  const bool split = p.split > 1;
-  // partial sums [buffer][warp][YC][WR]; a split product keeps them in the
-  // ring, which is idle by then, except kQmmDown's, which grow unit by unit
-  const bool in_ring = MODE != kQmmDown && split;
-  float* const ys = reinterpret_cast<float*>(smem + kQmmCtl + (in_ring ? 0 : ring_bytes));
+  // partial sums [buffer][warp][YC][WR]
+  float* const ys = reinterpret_cast<float*>(smem + kQmmCtl + ring_bytes);
   const int ys_warp = YC * WR, ys_buf = kQmmWarps * ys_warp;
-  const int buffers = in_ring ? 0 : MODE == kQmmUp && p.PB == 0 ? 1 : p.PB;
-  const uint32_t zeros = kQmmCtl + ring_bytes + buffers * ys_buf * 4;  // a record of zeros
-  const int rank = split ? (int)qmm_cluster_rank() : 0;
-  const int cta = blockIdx.x / p.split, nctas = gridDim.x / p.split;
   const int tile_rows = OR * RW;
   const int tiles = (int)((p.n + tile_rows - 1) / tile_rows);
 
@@ -945,12 +970,11 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       return;
     }
   }
-  if (p.rows_aligned && threadIdx.x == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map0)) : "memory");
-    if constexpr (MODE == kQmmUp) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map1)) : "memory");
-  }
-  for (int i = threadIdx.x; i < kQmmRec / 4; i += kQmmThreads) reinterpret_cast<uint32_t*>(smem + zeros)[i] = 0u;
   if (threadIdx.x == 0) {
+    if (p.rows_aligned) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map0)) : "memory");
+      if constexpr (MODE == kQmmUp) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map1)) : "memory");
+    }
     for (int i = 0; i < KW; ++i) {
       for (int k = 0; k < S; ++k) {
         mbar_init(&full[i][k], RW + 1);
@@ -963,6 +987,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         mbar_init(&taken[i][k], 1);
       }
     }
+    for (int i = 0; i < 8; ++i) rows_done[i] = 0;
     fence_mbar_init();
   }
   QmmLists L{};
@@ -975,32 +1000,45 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     }
     // kQmmDown does not wait here: the lists' kernel was complete before any
     // CTA of kQmmUp let this kernel start
-    L = qmm_load_lists(p, smem + zeros + kQmmRec);
+    L = qmm_load_lists(p, smem + kQmmCtl + ring_bytes + p.PB * ys_buf * 4);
   }
   __syncthreads();
-  const int units = MODE == kQmmDown ? L.ngroups * p.nsb : p.nsb;
-  const int u0 = split ? (int)((int64_t)units * rank / p.split) : 0;
-  const int u1 = split ? (int)((int64_t)units * (rank + 1) / p.split) : units;
 
-  // ---- cursors: column kw takes units u0 + kw, u0 + kw + KW, ... of every task
-  const int up_dg = MODE == kQmmUp ? nctas / tiles : 0, up_dt = MODE == kQmmUp ? nctas - up_dg * tiles : nctas;
-  auto live = [&](const QmmCursor& c) { return MODE == kQmmUp ? c.g < L.ngroups : c.tile < tiles; };
-  auto first_task = [&](QmmCursor& c) {
-    c.tile = cta;
-    c.g = 0;
-    if constexpr (MODE == kQmmUp) {
-      c.g = cta / tiles;
-      c.tile = cta - c.g * tiles;
-    }
-  };
-  auto first_unit = [&](QmmCursor& c) {
-    c.u = c.sb = u0 + kw;
+  // ---- this CTA's steps [a, b) of all tasks
+  const int units = MODE == kQmmDown ? L.ngroups * p.nsb : p.nsb;
+  const int st = max(1, (units + KW - 1) / KW);  // steps of a task
+  const int64_t tasks = MODE == kQmmUp ? (int64_t)tiles * L.ngroups : tiles;
+  const int64_t T = tasks * st;
+  // no more CTAs than steps, so that each of the G has a part of a divided task
+  const int64_t G = min((int64_t)gridDim.x, max(T, (int64_t)1)), me = min((int64_t)blockIdx.x, G);
+  const int64_t a = p.whole ? tasks * me / G * st : T * me / G;
+  const int64_t b = blockIdx.x >= G ? a : p.whole ? tasks * (me + 1) / G * st : T * (me + 1) / G;
+  auto set_unit = [&](QmmCursor& c) {
+    c.u = c.sb = c.s * KW + kw;
     if constexpr (MODE == kQmmDown) {
       c.g = c.u / p.nsb;
       c.sb = c.u - c.g * p.nsb;
     }
   };
-  auto next_unit = [&](QmmCursor& c) {
+  auto next_task = [&](QmmCursor& c) {
+    c.s = 0;
+    if constexpr (MODE == kQmmDown) {
+      c.g = kw / p.nsb;
+      c.u = kw;
+      c.sb = kw - c.g * p.nsb;
+    } else {
+      c.u = c.sb = kw;
+    }
+    ++c.tile;
+    if constexpr (MODE == kQmmUp) {
+      if (c.tile == tiles) {
+        c.tile = 0;
+        ++c.g;
+      }
+    }
+  };
+  auto next_step = [&](QmmCursor& c) {  // within a task
+    ++c.s;
     c.u += KW;
     c.sb += KW;
     if constexpr (MODE == kQmmDown) {
@@ -1010,37 +1048,44 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       }
     }
   };
-  auto next_task = [&](QmmCursor& c) {
-    c.tile += up_dt;
-    if constexpr (MODE == kQmmUp) {
-      c.g += up_dg;
-      if (c.tile >= tiles) {
-        c.tile -= tiles;
-        ++c.g;
+  QmmCursor c;
+  {
+    const int64_t task = a / st;
+    c.s = (int)(a - task * st);
+    c.left = (int)(b - a);
+    c.g = MODE == kQmmUp ? (int)(task / tiles) : 0;
+    c.tile = (int)(task - (int64_t)c.g * tiles);
+    set_unit(c);
+  }
+  auto expert_of = [&](const QmmCursor& q) { return MODE == kQmmLinear ? 0 : L.groups[q.g].expert; };
+  auto count_of = [&](const QmmCursor& q) { return MODE == kQmmLinear ? p.M : L.groups[q.g].count; };
+
+  // ---- refills.  The producing cursor runs S units ahead; a column without a
+  // unit in a step skips it.
+  QmmCursor pc = c;
+  auto settle = [&] {  // to the next step with a unit
+    while (pc.left > 0 && pc.u >= units) {
+      --pc.left;
+      if (pc.s + 1 == st) {
+        next_task(pc);
+      } else {
+        next_step(pc);
       }
     }
   };
-  auto expert_of = [&](const QmmCursor& c) { return MODE == kQmmLinear ? 0 : L.groups[c.g].expert; };
-  auto count_of = [&](const QmmCursor& c) { return MODE == kQmmLinear ? p.M : L.groups[c.g].count; };
-
-  // ---- refills.  The producing cursor runs S units ahead.
-  bool more = u0 + kw < u1;  // this column has units, and pc is at one of them
-  QmmCursor pc;
-  first_task(pc);
-  first_unit(pc);
-  more = more && live(pc);
   auto advance = [&] {
-    next_unit(pc);
-    if (pc.u >= u1) {
+    --pc.left;
+    if (pc.s + 1 == st) {
       next_task(pc);
-      first_unit(pc);
-      more = live(pc);
+    } else {
+      next_step(pc);
     }
+    settle();
   };
+  settle();
   const uint64_t pol = l2_policy_evict_first();
-  // this warp's weight rows of unit pc into a slot: in the order of tiles of
-  // 16 (kQmmUp: the gate rows of all tiles, then the up rows)
-  const uint32_t my_rows = rw * WR * pitch;
+  const uint32_t my_rows = rw * WR * pitch;  // of a slot
+  // this warp's weight rows of unit pc into a slot (kQmmUp: gate rows, then up rows)
   auto fill_rows = [&](int stage) {
     uint64_t* bar = &full[kw][stage];
     const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes + my_rows;
@@ -1062,20 +1107,20 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       const int r = up ? lane - WR / 2 : lane;
       const uint8_t* w = up ? p.w1 : p.w0;
       const int64_t at = ((int64_t)expert_of(pc) * p.n + first + r) * p.rb + (int64_t)pc.sb * F::CB;
-      const int64_t a = at & ~(int64_t)15, end = at + need, cap = p.wbytes & ~(int64_t)15;
+      const int64_t a16 = at & ~(int64_t)15, end = at + need, cap = p.wbytes & ~(int64_t)15;
       int64_t e = (end + 15) & ~(int64_t)15;
-      if (e > cap) e = cap > a ? cap : a;
+      if (e > cap) e = cap > a16 ? cap : a16;
       const bool valid = lane < WR && first + r < p.n;
       uint8_t* dst = smem + slot + lane * pitch;
-      const uint32_t bytes = valid ? (uint32_t)(e - a) : 0u;
-      if (valid) {
-        for (int64_t i = e; i < end; ++i) dst[i - a] = w[i];
+      const uint32_t bytes = valid ? (uint32_t)(e - a16) : 0u;
+      if (valid && e < end) {
+        for (int64_t i = e; i < end; ++i) dst[i - a16] = w[i];
+        fence_proxy_async_smem();
       }
-      if (e < end) fence_proxy_async_smem();
       const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
       if (lane == 0) mbar_arrive_expect_tx(bar, total);
       __syncwarp();
-      if (bytes) bulk_g2s_hint(dst, w + a, bytes, bar, pol);
+      if (bytes) bulk_g2s_hint(dst, w + a16, bytes, bar, pol);
     }
   };
   auto fill_records = [&](int stage) {
@@ -1096,8 +1141,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     // the weights do not depend on the kernel before; records, residual and
     // outputs do
     const QmmCursor start = pc;
-    const bool had = more;
-    for (int k = 0; k < S && more; ++k) {
+    for (int k = 0; k < S && pc.left > 0; ++k) {
       fill_rows(k);
       advance();
     }
@@ -1106,14 +1150,13 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     qmm_dep_launch();
     if (keeper) {
       pc = start;
-      more = had;
-      for (int k = 0; k < S && more; ++k) {
+      for (int k = 0; k < S && pc.left > 0; ++k) {
         fill_records(k);
         advance();
       }
     }
   } else {
-    for (int k = 0; k < S && more; ++k) {
+    for (int k = 0; k < S && pc.left > 0; ++k) {
       fill_rows(k);
       if (keeper) fill_records(k);
       advance();
@@ -1149,22 +1192,30 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       }
     }
   };
-  auto leave_sums = [&](int count, float* to) {
-    each_sum(count, [&](int tk, int r, float v) {
-      if (tk < count) to[tk * WR + r] = v;
-    });
-  };
-  // kQmmUp: this warp has stored h of OR rows from `row` on for the tokens of
-  // group g.  Whoever completes 256 rows makes their records.
-  auto finish_rows = [&](int g, int row) {
-    if (row >= p.n) return;
+  int stage = 0, seq = 0;
+  // kQmmUp: the sums of this row tile became h.  The CTA's last row tile of
+  // the task reports the task's rows; whoever completes 256 rows of h makes
+  // their records.  (A report per row tile would fence 8 times as often.)
+  auto report_rows = [&](int g, int row, int rows, int turns) {
     __syncwarp();
+    rows = min(rows, (int)p.n - row);
+    if (rows <= 0) return;
     const int sb = row >> 8, valid = min(256, (int)p.n - 256 * sb), nsb = ((int)p.n + 255) >> 8;
     int last = 0;
     if (lane == 0) {
-      __threadfence();
-      last = atomicAdd(p.done + (int64_t)g * nsb + sb, 1) == (valid + OR - 1) / OR - 1;
-      __threadfence();
+      bool mine = true;
+      if (turns > 1) {  // row tiles of this CTA
+        __threadfence_block();
+        int* count = rows_done + (seq & 7);  // warps of a CTA are at most S < 8 tasks apart
+        mine = atomicAdd(count, 1) == turns - 1;
+        if (mine) *count = 0;
+        __threadfence_block();
+      }
+      if (mine) {
+        __threadfence();
+        last = atomicAdd(p.done + (int64_t)g * nsb + sb, rows) + rows == valid;
+        __threadfence();
+      }
     }
     if (!__shfl_sync(0xffffffffu, last, 0)) return;
     const int count = L.groups[g].count, start = L.groups[g].start;
@@ -1173,235 +1224,204 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       qmm_make_record<float, true>(p.h + pick * p.n + 256 * sb, valid, p.order_h, p.recs_h + (pick * nsb + sb) * kQmmRec, lane);
     }
   };
-  int stage = 0, seq = 0;
   uint32_t phase = 0;
   int owed = -1;  // slot whose records are still to be refilled for pc
-  QmmCursor c;
-  first_task(c);
-  for (; ok && live(c); next_task(c), ++seq) {
+  for (; ok && c.left > 0; ++seq) {
+    // ---- one task, or this CTA's part of it
     const int buf = p.PB == 2 ? seq & 1 : 0, turn = p.PB == 2 ? seq >> 1 : seq;
+    const int s_first = c.s, n_steps = min(st - c.s, c.left);
+    const int tile = c.tile, task_g = c.g;
     float* my_ys = ys + buf * ys_buf + warp * ys_warp;
-    if constexpr (MODE == kQmmDown) {
-      if (!split && turn > 0 && !mbar_wait_bounded(&taken[rw][buf], (turn & 1) ^ 1)) {
-        ok = false;
-        break;
-      }
+    auto claim_ys = [&] {  // the buffer's last sums have been joined
+      if (KW > 1 && turn > 0 && !mbar_wait_bounded(&taken[rw][buf], (turn & 1) ^ 1)) ok = false;
       __syncwarp();
+    };
+    if constexpr (MODE == kQmmDown) {
+      claim_ys();
       for (int i = lane; i < ys_warp; i += 32) my_ys[i] = 0.0f;
       __syncwarp();
     }
-    for (first_unit(c); c.u < u1; next_unit(c)) {
-      if (owed >= 0) {
-        // the records of the slot used last: free when all RW warps are done
-        if (keeper) {
-          const uint32_t ph = owed > stage || (owed == stage && S == 1) ? phase ^ 1 : phase;
-          if (!mbar_wait_bounded(&used[kw][owed], ph)) {
-            ok = false;
-            break;
-          }
-          __syncwarp();
-          fill_records(owed);
-        }
-        owed = -1;
-        advance();
-      }
-      if (!mbar_wait_bounded(&full[kw][stage], phase)) {
-        ok = false;
-        break;
-      }
-      __syncwarp();
-      const int count = count_of(c);
-      const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes;
-      const int nv = min(8, p.nblk - 8 * c.sb);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        uint32_t o[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = MODE == kQmmUp && MT == 1 ? 8 * h + lr : 16 * t + 8 * h + lr;  // of this warp's rows
-          uint32_t mis = 0;
-          if constexpr (F::CB % 16 != 0 || Fmt<TYPE>::QK == 32) {
-            mis = (uint32_t)(c.sb * F::CB) & 15;
-            if (!p.rows_aligned) {
-              const int rr = MODE == kQmmUp && r >= WR / 2 ? r - WR / 2 : r;
-              const int64_t row = (int64_t)expert_of(c) * p.n + c.tile * tile_rows + rw * OR + rr;
-              mis = (uint32_t)(row * p.rb + (int64_t)c.sb * F::CB) & 15;
+    [[maybe_unused]] int task_count = 0;
+    if constexpr (MODE != kQmmDown) task_count = count_of(c);
+    for (int i = 0; i < n_steps && ok; ++i) {
+      if (c.u < units) {
+        if (owed >= 0) {
+          // the records of the slot used last: free when all RW warps are done
+          if (keeper) {
+            if (!mbar_wait_bounded(&used[kw][owed], owed > stage ? phase ^ 1 : phase)) {
+              ok = false;
+              break;
             }
+            __syncwarp();
+            fill_records(owed);
           }
-          o[h] = slot + my_rows + r * pitch + mis;
+          owed = -1;
+          advance();
         }
-        auto unit = [&](auto N, auto Limbs, int first) {
-          constexpr int ni = decltype(N)::value;
-          constexpr bool limbs = decltype(Limbs)::value;
-          constexpr int nq = kQmmVals<ni, limbs>;
-          const QmmB<ni, limbs> B(slot + recs_at, zeros, first, count, lr, lc);
-          float v[nq][2];
-          qmm_unit<TYPE, LAYOUT, ni, limbs>(o, lc, B, nv, v);
+        if (!mbar_wait_bounded(&full[kw][stage], phase)) {
+          ok = false;
+          break;
+        }
+        __syncwarp();
+        const int count = MODE == kQmmDown ? count_of(c) : task_count;
+        const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes;
+        const uint32_t recs = slot + recs_at;
+        const int nv = min(8, p.nblk - 8 * c.sb);
 #pragma unroll
-          for (int q = 0; q < nq; ++q) {
-            const int tk = first + (limbs ? 2 * lc + q : 2 * q + (lc >> 1));
-            float s = tk < count ? qmm_lds<float>(slot + recs_at + tk * kQmmRecPitch + kQmmRecS) : 0.0f;
-            if (!limbs && (lc & 1)) s *= 65536.0f;  // limbs 2, 3 of the token
-            float y0 = s * v[q][0], y1 = s * v[q][1];
-            if constexpr (MODE == kQmmDown) {
-              if constexpr (!limbs) {  // the pair of lanes takes a row half each
-                y0 += __shfl_xor_sync(0xffffffffu, y0, 1);
-                y1 += __shfl_xor_sync(0xffffffffu, y1, 1);
+        for (int t = 0; t < MT; ++t) {
+          uint32_t o[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = MODE == kQmmUp && MT == 1 ? 8 * h + lr : 16 * t + 8 * h + lr;  // of this warp's rows
+            uint32_t mis = 0;
+            if constexpr (F::CB % 16 != 0 || Fmt<TYPE>::QK == 32) {
+              mis = (uint32_t)(c.sb * F::CB) & 15;
+              if (!p.rows_aligned) {
+                const int rr = MODE == kQmmUp && r >= WR / 2 ? r - WR / 2 : r;
+                const uint32_t row = (uint32_t)expert_of(c) * (uint32_t)p.n + (uint32_t)(tile * tile_rows + rw * OR + rr);
+                mis = (row * (uint32_t)p.rb + (uint32_t)(c.sb * F::CB)) & 15;
               }
-              if (tk < count) {
-                const int pick = L.groups[c.g].start + tk;
-                const float w = L.pwts[pick];
-                float* to = my_ys + L.ptok[pick] * WR + 16 * t + lr;
-                if constexpr (limbs) {
-                  to[0] += w * y0;
-                  to[8] += w * y1;
-                } else {
-                  to[8 * (lc & 1)] += w * (lc & 1 ? y1 : y0);
+            }
+            o[h] = slot + my_rows + r * pitch + mis;
+          }
+          auto unit = [&](auto N, auto Limbs, int first) {
+            constexpr int ni = decltype(N)::value;
+            constexpr bool limbs = decltype(Limbs)::value;
+            constexpr int nq = kQmmVals<ni, limbs>;
+            const QmmB<limbs> B(recs, first, lr, lc);
+            float v[nq][2];
+            qmm_unit<TYPE, LAYOUT, ni, limbs>(o, lc, B, nv, v);
+#pragma unroll
+            for (int q = 0; q < nq; ++q) {
+              const int tk = first + (limbs ? 2 * lc + q : 2 * q + (lc >> 1));
+              float s = tk < count ? qmm_lds<float>(recs + tk * kQmmRecPitch + kQmmRecS) : 0.0f;
+              if (!limbs && (lc & 1)) s *= 65536.0f;  // limb 2 of the token
+              float y0 = s * v[q][0], y1 = s * v[q][1];
+              if constexpr (MODE == kQmmDown) {
+                if constexpr (!limbs) {  // the pair of lanes takes a row half each
+                  y0 += __shfl_xor_sync(0xffffffffu, y0, 1);
+                  y1 += __shfl_xor_sync(0xffffffffu, y1, 1);
                 }
+                if (tk < count) {
+                  const int pick = L.groups[c.g].start + tk;
+                  const float w = L.pwts[pick];
+                  float* to = my_ys + L.ptok[pick] * WR + 16 * t + lr;
+                  if constexpr (limbs) {
+                    to[0] += w * y0;
+                    to[8] += w * y1;
+                  } else {
+                    to[8 * (lc & 1)] += w * (lc & 1 ? y1 : y0);
+                  }
+                }
+              } else if (NQ <= 2 || first == 0) {
+                tot[t][q][0] += y0;
+                tot[t][q][1] += y1;
+              } else {
+                tot[t][NQ - 2 + (q & 1)][0] += y0;
+                tot[t][NQ - 2 + (q & 1)][1] += y1;
               }
-            } else if (NQ <= 2 || first == 0) {
-              tot[t][q][0] += y0;
-              tot[t][q][1] += y1;
-            } else {
-              tot[t][NQ - 2 + (q & 1)][0] += y0;
-              tot[t][NQ - 2 + (q & 1)][1] += y1;
             }
-          }
-        };
-        using std::integral_constant;
-        using std::false_type;
-        using std::true_type;
-        if (TC == 2 || count <= 2) {
-          unit(integral_constant<int, 1>{}, false_type{}, 0);
-        } else if (TC == 4 || count <= 4) {
-          if constexpr (TC > 2) unit(integral_constant<int, 2>{}, false_type{}, 0);
-        } else if constexpr (TC > 4) {
-          // eight tokens at a time (all sixteen at once would not fit the registers)
+          };
+          using std::integral_constant;
+          using std::false_type;
+          using std::true_type;
+          if (TC == 2 || count <= 2) {
+            unit(integral_constant<int, 1>{}, false_type{}, 0);
+          } else if (TC == 4 || count <= 4) {
+            if constexpr (TC > 2) unit(integral_constant<int, 2>{}, false_type{}, 0);
+          } else if constexpr (TC > 4) {
+            // eight tokens at a time (all sixteen at once would not fit the registers)
 #pragma unroll 1
-          for (int first = 0; first < (TC > 8 ? count : 8); first += 8) unit(integral_constant<int, 3>{}, true_type{}, first);
+            for (int first = 0; first < (TC > 8 ? count : 8); first += 8) unit(integral_constant<int, 3>{}, true_type{}, first);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&used[kw][stage]);
+        if (pc.left > 0) {
+          fill_rows(stage);
+          owed = stage;
+        }
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&used[kw][stage]);
-      if (more) {
-        fill_rows(stage);
-        owed = stage;
-      }
-      if (++stage == S) {
-        stage = 0;
-        phase ^= 1;
-      }
+      next_step(c);
     }
-    if (!ok || split) break;  // a split product has one task; its sums are joined below
-    const int row0 = c.tile * tile_rows + rw * OR;
-    const int cnt = MODE == kQmmUp ? L.groups[c.g].count : p.M;
-    if (p.PB == 0) {
-      // ---- KW == 1: outputs straight from the registers (kQmmUp: through
-      // the warp's own block of shared memory, to bring gate and up together)
-      if constexpr (MODE == kQmmUp) {
-        float* own = ys + warp * ys_warp;
-        leave_sums(cnt, own);
-        __syncwarp();
-        for (int i = lane; i < OR * cnt; i += 32) {
-          const int col = i / OR, r = i % OR;
-          if (row0 + r < p.n)
-            p.h[(int64_t)L.plist[L.groups[c.g].start + col] * p.n + row0 + r] =
-                qmm_act(own[col * WR + r], p.act) * own[col * WR + r + OR];
-        }
-        finish_rows(c.g, row0);
-        __syncwarp();
-      } else if constexpr (MODE == kQmmLinear) {
-        each_sum(cnt, [&](int tk, int r, float v) {
-          if (tk < cnt && row0 + r < p.n) qmm_store(p, tk, row0 + r, v, qmm_adds(p, tk, row0 + r));
-        });
-      }
-      continue;
-    }
-    // ---- join the KW columns' sums: every warp leaves its own, one of them adds
+    if (!ok) break;
+    c.left -= n_steps;
+    c.s = s_first + n_steps;  // (columns without a unit in the last step count it too)
+    const bool ends = c.s == st;
+    if (ends) next_task(c);
+    // ---- the sums: every column leaves its own; one of them adds them up
+    const int cnt = MODE == kQmmUp ? task_count : p.M;
     if constexpr (MODE != kQmmDown) {
-      if (turn > 0 && !mbar_wait_bounded(&taken[rw][buf], (turn & 1) ^ 1)) {
-        ok = false;
-        break;
-      }
-      __syncwarp();
-      leave_sums(cnt, my_ys);
+      claim_ys();
+      each_sum(cnt, [&](int tk, int r, float v) {
+        if (tk < cnt) my_ys[tk * WR + r] = v;
+      });
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&ready[rw][buf]);
-    if (kw == (seq & (KW - 1))) {
+    if (KW > 1) {
+      if (lane == 0) mbar_arrive(&ready[rw][buf]);
+      if (kw != (seq & (KW - 1))) continue;
       if (!mbar_wait_bounded(&ready[rw][buf], turn & 1)) {
         ok = false;
         break;
       }
       __syncwarp();
-      const float* y0 = ys + buf * ys_buf + rw * KW * ys_warp;
-      auto sum_kw = [&](int col, int r) {
-        float v = y0[col * WR + r];
-        for (int k = 1; k < KW; ++k) v += y0[k * ys_warp + col * WR + r];
-        return v;
-      };
+    }
+    const float* y0 = ys + buf * ys_buf + rw * KW * ys_warp;
+    auto joined = [&](int at) {
+      float v = y0[at];
+      for (int k = 1; k < KW; ++k) v += y0[k * ys_warp + at];
+      return v;
+    };
+    const int row0 = tile * tile_rows + rw * OR;
+    // writes the outputs of this row tile, sum(at) being the sum of place [token][row]
+    auto emit = [&](auto&& sum) {
       for (int i = lane; i < OR * cnt; i += 32) {
         const int col = i / OR, r = i % OR;
-        if (row0 + r < p.n) {
-          if constexpr (MODE == kQmmUp) {
-            const float gate = sum_kw(col, r), up = sum_kw(col, r + OR);
-            p.h[(int64_t)L.plist[L.groups[c.g].start + col] * p.n + row0 + r] = qmm_act(gate, p.act) * up;
-          } else {
-            qmm_store(p, col, row0 + r, sum_kw(col, r), qmm_adds(p, col, row0 + r));
-          }
+        if (row0 + r >= p.n) continue;
+        if constexpr (MODE == kQmmUp) {
+          const float gate = sum(col * WR + r), up = sum(col * WR + r + OR);
+          p.h[(int64_t)L.plist[L.groups[task_g].start + col] * p.n + row0 + r] = qmm_act(gate, p.act) * up;
+        } else {
+          const QmmAdd add = qmm_adds(p, col, row0 + r);
+          qmm_store(p, col, row0 + r, sum(col * WR + r), add);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&taken[rw][buf]);
-      if constexpr (MODE == kQmmUp) finish_rows(c.g, row0);
-    }
-  }
-  if constexpr (MODE != kQmmUp) {
-    if (split) {
-      // ---- a K split over the cluster: each rank adds its columns' sums into
-      // those of its first column, then all ranks their share of the outputs,
-      // always over the ranks in order
-      __syncthreads();  // every warp is done with the ring
-      if constexpr (MODE == kQmmLinear) {
-        leave_sums(p.M, ys + warp * ys_warp);
-        __syncthreads();
-      }
-      const int outs = RW * WR * p.M;
-      auto place = [&](int i, int& col, int& r) -> float* {
-        col = i / (RW * WR);
-        r = i - col * (RW * WR);
-        return ys + (r / WR) * KW * ys_warp + col * WR + r % WR;
+    };
+    if (s_first == 0 && ends) {
+      emit(joined);
+      if constexpr (MODE == kQmmUp) report_rows(task_g, tile * tile_rows, tile_rows, RW);
+    } else {
+      // ---- a part of a divided task
+      const int64_t f0 = MODE == kQmmUp ? ((int64_t)task_g * tiles + tile) * st : (int64_t)tile * st;
+      const int c_lo = (int)(((f0 + 1) * G - 1) / T), c_hi = (int)(((f0 + st) * G - 1) / T);
+      auto part_of = [&](int cta) {
+        return p.parts + ((int64_t)(cta * 2 + (cta == c_lo ? 1 : 0)) * kQmmWarps + rw) * ys_warp;
       };
-      for (int i = threadIdx.x; i < outs; i += kQmmThreads) {
-        int col, r;
-        float* q = place(i, col, r);
-        float v = q[0];
-        for (int k = 1; k < KW; ++k) v += q[k * ys_warp];
-        q[0] = v;
+      float* mine = part_of((int)blockIdx.x);
+      for (int i = lane; i < WR * cnt; i += 32) mine[i] = joined(i);
+      __syncwarp();
+      int last = 0;
+      if (lane == 0) {
+        __threadfence();
+        last = atomicAdd(p.tickets + c_lo * kQmmWarps + rw, n_steps) + n_steps == st;
+        __threadfence();
       }
-      // what the first output adds is under way while the ranks meet
-      const int i0 = rank * kQmmThreads + threadIdx.x;
-      QmmAdd add{};
-      if (i0 < outs) {
-        int col, r;
-        place(i0, col, r);
-        if (cta * tile_rows + r < p.n) add = qmm_adds(p, col, cta * tile_rows + r);
+      if (__shfl_sync(0xffffffffu, last, 0)) {
+        emit([&](int at) {
+          float v = 0.0f;
+          for (int q = c_lo; q <= c_hi; ++q) v += __ldcg(part_of(q) + at);
+          return v;
+        });
+        if constexpr (MODE == kQmmUp) report_rows(task_g, row0, OR, 1);
       }
-      qmm_cluster_sync();
-      for (int i = i0; i < outs; i += p.split * kQmmThreads) {
-        int col, r;
-        const float* q = place(i, col, r);
-        float part[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) part[k] = k < p.split ? qmm_ld_cluster(q, (uint32_t)k) : 0.0f;
-        float v = part[0];
-#pragma unroll
-        for (int k = 1; k < 8; ++k) v += part[k];
-        const int row = cta * tile_rows + r;
-        if (row < p.n) qmm_store(p, col, row, v, i == i0 ? add : qmm_adds(p, col, row));
-      }
-      qmm_cluster_sync();  // every rank has read the others' sums
     }
+    __syncwarp();
+    if (KW > 1 && lane == 0) mbar_arrive(&taken[rw][buf]);
   }
 }
 

@@ -24,15 +24,11 @@ int launch_qmm_t(const QmmParams& p, const CUtensorMap* maps, int grid, size_t s
   cfg.blockDim = dim3(kQmmThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)p.split;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  cfg.numAttrs = 1;
   note_launch();
   return cudaLaunchKernelEx(&cfg, kern, p, maps[0], maps[1]) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
 }

@@ -39,16 +39,19 @@ def linear(lib, **kw):
     (_lib.ERR_SHAPE, dict(m=0)), (_lib.ERR_SHAPE, dict(m=-1)), (_lib.ERR_SHAPE, dict(m=17)),
     (_lib.ERR_SHAPE, dict(n=0)), (_lib.ERR_SHAPE, dict(n=1 << 25)), (_lib.ERR_SHAPE, dict(k=128)),
     (_lib.ERR_SHAPE, dict(t=Q8_0, k=48)), (_lib.ERR_SHAPE, dict(k=0)),
-    (_lib.ERR_WORKSPACE, dict(ws=None)), (_lib.ERR_WORKSPACE, dict(m=3, k=512, wsb=3 * 2 * 880 - 1)),
+    (_lib.ERR_WORKSPACE, dict(ws=None)), (_lib.ERR_WORKSPACE, dict(m=3, k=512, wsb=3 * 2 * 880)),
 ])
 def test_linear_refusals(lib, want, kw):
     assert linear(lib, **kw) == want
 
 
 def test_linear_workspace_size(lib):
-    # one record of 880 bytes per token and 256 of K
-    assert lib.nsq_linear_workspace_size(1, 256) == 880
-    assert lib.nsq_linear_workspace_size(16, 896) == 16 * 4 * 880
+    # one record of 880 bytes per token and 256 of K (rounded up to 256), 8 tickets
+    # and two parts of 8 row tiles of 32 (16 beyond 4 tokens) rows for 320 CTAs
+    def size(m, k):
+        return -(-m * -(-k // 256) * 880 // 256) * 256 + 320 * 8 * 4 + 320 * 2 * 8 * (16 if m > 4 else 32) * m * 4
+    for m, k in ((1, 256), (4, 896), (5, 896), (16, 14336)):
+        assert lib.nsq_linear_workspace_size(m, k) == size(m, k)
     assert lib.nsq_linear_workspace_size(17, 256) == 0
     assert lib.nsq_linear_workspace_size(0, 256) == 0
 
