@@ -221,9 +221,9 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
   const int pitch = p.rb % 16 == 0 ? f.PA : f.PG;
   // Columns of K per CTA (KW), the rest of the 8 warps being row tiles, and
   // whether tasks are divided: the choice with the least time by a simple
-  // model.  A CTA's time is its steps x (the bytes of its rows, and those of
-  // the records that its row tiles share), and about three steps to put
-  // divided tasks together.
+  // model.  A CTA's time is its steps x (the bytes of its rows, and a third of
+  // those of the records that its row tiles share, which come from L2), and
+  // about three steps to put divided tasks together.
   double best = 0;
   size_t smem = 0;
   int64_t grid = 0;
@@ -248,7 +248,7 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
     const int64_t tasks = (p.n + rows - 1) / rows * (p.mode == kQmmUp ? (groups < p.E ? groups : p.E) : 1);
     const int64_t units = p.mode == kQmmDown ? (groups < p.E ? groups : p.E) * p.nsb : p.nsb;
     const int64_t st = (units + KW - 1) / KW;
-    const double bytes = KW * (16.0 * f.MT * t.RW * pitch + (p.TS < 4 ? p.TS : 0.5 * p.TS) * kQmmRec) / here;
+    const double bytes = KW * (16.0 * f.MT * t.RW * pitch + 0.3 * (p.TS < 4 ? p.TS : 0.5 * p.TS) * kQmmRec) / here;
     for (int whole = 1; whole >= 0; --whole) {
       const int only = tune(kTuneQmmSplit, -1);
       if (only >= 0 && whole == (only > 0)) continue;

@@ -314,7 +314,7 @@ static __device__ __noinline__ float qmm_act(float v, int act) {
 // Two row tiles share their B operands and bookkeeping; the wider formats
 // have one, for the depth of the ring.
 template <int TYPE> struct QmmFmt;
-template <> struct QmmFmt<NSQ_TYPE_Q4_K> { static constexpr int CB = 144, PA = 144, PG = 144, MT = 2; };
+template <> struct QmmFmt<NSQ_TYPE_Q4_K> { static constexpr int CB = 144, PA = 160, PG = 160, MT = 2; };
 template <> struct QmmFmt<NSQ_TYPE_Q5_K> { static constexpr int CB = 176, PA = 176, PG = 176, MT = 2; };
 template <> struct QmmFmt<NSQ_TYPE_Q6_K> { static constexpr int CB = 210, PA = 240, PG = 240, MT = 1; };
 template <> struct QmmFmt<NSQ_TYPE_Q4_0> { static constexpr int CB = 144, PA = 144, PG = 176, MT = 2; };
@@ -892,6 +892,11 @@ inline size_t qmm_lists_bytes(int P) { return (size_t)P * (sizeof(QmmGroup) + 12
 
 // Bias, activation and residual (kQmmLinear), or the residual alone
 // (kQmmDown), for one finished sum.
+__device__ __forceinline__ int qmm_add_acq_rel(int32_t* p, int v) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
 struct QmmAdd {
   float bias, residual;
 };
@@ -977,7 +982,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     }
     for (int i = 0; i < KW; ++i) {
       for (int k = 0; k < S; ++k) {
-        mbar_init(&full[i][k], RW + 1);
+        mbar_init(&full[i][k], RW == 1 ? 1 : RW + 1);  // rows of every warp, records (one warp: both at once)
         mbar_init(&used[i][k], RW);
       }
     }
@@ -1085,8 +1090,9 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   settle();
   const uint64_t pol = l2_policy_evict_first();
   const uint32_t my_rows = rw * WR * pitch;  // of a slot
-  // this warp's weight rows of unit pc into a slot (kQmmUp: gate rows, then up rows)
-  auto fill_rows = [&](int stage) {
+  // this warp's weight rows of unit pc into a slot (kQmmUp: gate rows, then up
+  // rows); more: bytes that follow on the same barrier phase
+  auto fill_rows = [&](int stage, uint32_t more) {
     uint64_t* bar = &full[kw][stage];
     const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes + my_rows;
     const int first = pc.tile * tile_rows + rw * OR;  // of the expert's rows
@@ -1095,7 +1101,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         const int row0 = expert_of(pc) * (int)p.n + first;
         const int x = ((pc.sb * F::CB) & ~15) / 2;  // 16-bit elements
         const uint32_t dst = smem_u32(smem) + slot;
-        mbar_arrive_expect_tx(bar, WR * pitch);
+        mbar_arrive_expect_tx(bar, WR * pitch + more);
         qmm_tma_2d(dst, &map0, x, row0, bar, pol);
         if constexpr (MODE == kQmmUp) qmm_tma_2d(dst + (WR / 2) * pitch, &map1, x, row0, bar, pol);
       }
@@ -1118,7 +1124,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         fence_proxy_async_smem();
       }
       const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
-      if (lane == 0) mbar_arrive_expect_tx(bar, total);
+      if (lane == 0) mbar_arrive_expect_tx(bar, total + more);
       __syncwarp();
       if (bytes) bulk_g2s_hint(dst, w + a16, bytes, bar, pol);
     }
@@ -1127,7 +1133,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     uint64_t* bar = &full[kw][stage];
     uint8_t* dst = smem + kQmmCtl + (stage * KW + kw) * slot_bytes + recs_at;
     const int count = count_of(pc);
-    if (lane == 0) mbar_arrive_expect_tx(bar, count * kQmmRec);
+    if (RW > 1 && lane == 0) mbar_arrive_expect_tx(bar, count * kQmmRec);
     __syncwarp();
     if (lane < count) {
       int row = lane;
@@ -1136,29 +1142,30 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       bulk_g2s(dst + lane * kQmmRecPitch, p.recs + ((int64_t)row * p.nsb + pc.sb) * kQmmRec, kQmmRec, bar);
     }
   };
-  const bool keeper = rw == (kw & (RW - 1));  // refills the column's records
+  // The column's warps refill the records of its units in turn: it takes a warp
+  // about 500 cycles (always the same one: the others wait 750 cycles a unit).
+  int rec_unit = kw;  // units of the column whose records were refilled, from kw on
+  auto my_turn = [&] { return rw == (rec_unit++ & (RW - 1)); };
   if constexpr (MODE != kQmmUp) {
     // the weights do not depend on the kernel before; records, residual and
     // outputs do
     const QmmCursor start = pc;
     for (int k = 0; k < S && pc.left > 0; ++k) {
-      fill_rows(k);
+      fill_rows(k, RW == 1 ? count_of(pc) * kQmmRec : 0);
       advance();
     }
     __syncwarp();
     qmm_dep_wait();
     qmm_dep_launch();
-    if (keeper) {
-      pc = start;
-      for (int k = 0; k < S && pc.left > 0; ++k) {
-        fill_records(k);
-        advance();
-      }
+    pc = start;
+    for (int k = 0; k < S && pc.left > 0; ++k) {
+      if (my_turn()) fill_records(k);
+      advance();
     }
   } else {
     for (int k = 0; k < S && pc.left > 0; ++k) {
-      fill_rows(k);
-      if (keeper) fill_records(k);
+      fill_rows(k, RW == 1 ? count_of(pc) * kQmmRec : 0);
+      if (my_turn()) fill_records(k);
       advance();
     }
   }
@@ -1211,11 +1218,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         if (mine) *count = 0;
         __threadfence_block();
       }
-      if (mine) {
-        __threadfence();
-        last = atomicAdd(p.done + (int64_t)g * nsb + sb, rows) + rows == valid;
-        __threadfence();
-      }
+      if (mine) last = qmm_add_acq_rel(p.done + (int64_t)g * nsb + sb, rows) + rows == valid;
     }
     if (!__shfl_sync(0xffffffffu, last, 0)) return;
     const int count = L.groups[g].count, start = L.groups[g].start;
@@ -1247,7 +1250,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       if (c.u < units) {
         if (owed >= 0) {
           // the records of the slot used last: free when all RW warps are done
-          if (keeper) {
+          if (my_turn()) {
             if (!mbar_wait_bounded(&used[kw][owed], owed > stage ? phase ^ 1 : phase)) {
               ok = false;
               break;
@@ -1336,10 +1339,16 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&used[kw][stage]);
+        if (RW > 1 && lane == 0) mbar_arrive(&used[kw][stage]);
         if (pc.left > 0) {
-          fill_rows(stage);
-          owed = stage;
+          if (RW == 1) {
+            fill_rows(stage, count_of(pc) * kQmmRec);
+            fill_records(stage);
+            advance();
+          } else {
+            fill_rows(stage, 0);
+            owed = stage;
+          }
         }
         if (++stage == S) {
           stage = 0;
@@ -1392,8 +1401,14 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         }
       }
     };
+    // the buffer is free as soon as it was read: the reports below take 1 to 2 us
+    auto release_ys = [&] {
+      __syncwarp();
+      if (KW > 1 && lane == 0) mbar_arrive(&taken[rw][buf]);
+    };
     if (s_first == 0 && ends) {
       emit(joined);
+      release_ys();
       if constexpr (MODE == kQmmUp) report_rows(task_g, tile * tile_rows, tile_rows, RW);
     } else {
       // ---- a part of a divided task
@@ -1404,13 +1419,9 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       };
       float* mine = part_of((int)blockIdx.x);
       for (int i = lane; i < WR * cnt; i += 32) mine[i] = joined(i);
-      __syncwarp();
+      release_ys();
       int last = 0;
-      if (lane == 0) {
-        __threadfence();
-        last = atomicAdd(p.tickets + c_lo * kQmmWarps + rw, n_steps) + n_steps == st;
-        __threadfence();
-      }
+      if (lane == 0) last = qmm_add_acq_rel(p.tickets + c_lo * kQmmWarps + rw, n_steps) + n_steps == st;
       if (__shfl_sync(0xffffffffu, last, 0)) {
         emit([&](int at) {
           float v = 0.0f;
@@ -1420,8 +1431,6 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         if constexpr (MODE == kQmmUp) report_rows(task_g, row0, OR, 1);
       }
     }
-    __syncwarp();
-    if (KW > 1 && lane == 0) mbar_arrive(&taken[rw][buf]);
   }
 }
 
