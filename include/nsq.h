@@ -307,10 +307,14 @@ int nsq_gemv_multi_xchg(const nsq_xsegment *segs, int nseg, const float *x, int6
  *   dtype     element type of x, residual and y: NSQ_OUT_F32 or NSQ_OUT_BF16
  *   bias      N f32, or NULL;  act: NSQ_ACT_*
  *   residual  [M x N] of dtype, or NULL; may be y itself
- * M = 1..16: fp16 hi + lo activations, exact products, f32 sums; about 3e-7
- * relative for f32 (bf16 results are rounded once).  K is a multiple of the
- * type's block.  `workspace` (nsq_linear_workspace_size(M, K) bytes, 16-byte
- * aligned) holds the prepared activations; one call at a time uses it. */
+ * M = 1..16: 24-bit activations per 256 of K, exact integer products, f32
+ * sums: f32 results are off by about 3e-7 of their norm, bf16 ones rounded
+ * once.  A token with an infinity or a NaN gives NaN throughout.  K is a
+ * multiple of the type's block.  `workspace` (nsq_linear_workspace_size(M, K)
+ * bytes, 16-byte aligned) is used by one call at a time.
+ * M > 16: bf16 only, K % 256 == 0, x and y 16-byte aligned; the product of
+ * nsq_gemm_bf16 (weights rounded to bf16, f32 sums), the epilogue in f32
+ * before the one rounding of the result.  No workspace. */
 #define NSQ_ACT_NONE 0
 #define NSQ_ACT_SILU 1      /* v / (1 + e^-v) */
 #define NSQ_ACT_GELU 2      /* v (1 + erf(v / sqrt 2)) / 2 */

@@ -15,6 +15,8 @@ int launch_qmm_q40(int layout, const QmmParams& p, const CUtensorMap* maps, int 
 int launch_qmm_q80(int layout, const QmmParams& p, const CUtensorMap* maps, int grid, size_t smem, cudaStream_t st);
 int check_weights(const void* w, int type, int layout, int64_t K);
 int device_check(int* num_sms);
+int run_gemm_epi(const uint8_t* w, int type, int layout, const void* x, const float* bias, int act, const void* residual,
+                 void* y, int64_t M, int64_t N, int64_t K, cudaStream_t st, int num_sms);
 
 constexpr int kPrepThreads = 32 * kQmmWarps;
 constexpr int kRouteTok = 8;  // tokens of one CTA's logits
@@ -440,12 +442,21 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   int rc = check_weights(w, ggml_type, q6k_layout, K);
   if (rc) return rc;
   if (!act_ok(act) || (dtype != NSQ_OUT_F32 && dtype != NSQ_OUT_BF16)) return NSQ_ERR_TYPE;
-  if (M < 1 || M > NSQ_GEMV_MAX_M || N < 1 || N > (int64_t)1 << 24 || K > (int64_t)1 << 24) return NSQ_ERR_SHAPE;
+  if (M < 1 || M > (int64_t)1 << 24 || N < 1 || N > (int64_t)1 << 24 || K > (int64_t)1 << 24) return NSQ_ERR_SHAPE;
+  const bool prompt = M > NSQ_GEMV_MAX_M;
+  if (prompt && (dtype != NSQ_OUT_BF16 || K % 256)) return NSQ_ERR_SHAPE;
   if (!x || !y) return NSQ_ERR_NULL;
   const uintptr_t mask = dtype == NSQ_OUT_F32 ? 3 : 1;
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & mask)
     return NSQ_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(bias) & 3) return NSQ_ERR_ALIGN;
+  if (prompt) {
+    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) return NSQ_ERR_ALIGN;
+    int sms = 0;
+    if ((rc = device_check(&sms))) return rc;
+    return run_gemm_epi(static_cast<const uint8_t*>(w), ggml_type, q6k_layout, x, bias, act, residual, y, M, N, K,
+                        static_cast<cudaStream_t>(stream), sms);
+  }
   if (!workspace || workspace_bytes < nsq_linear_workspace_size(M, K)) return NSQ_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NSQ_ERR_ALIGN;
   int num_sms = 0;

@@ -269,6 +269,10 @@ class CudaEngine:
         caller's, the call takes one from PyTorch's allocator, which keeps it from other streams and graphs."""
         if workspace is None:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise NsqError(_lib.ERR_TYPE, f"{what}: a workspace is contiguous uint8, not {workspace.dtype}")
+        else:
+            self._tensor(workspace, workspace.numel(), torch.uint8, f"{what}: workspace")
         index = self.device.index
         if index is None or index == torch.cuda.current_device():
             rc = fn(*args, workspace.data_ptr(), workspace.numel(), _stream_handle(self.device))

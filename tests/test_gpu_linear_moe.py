@@ -223,6 +223,92 @@ def test_linear_captured_with_one_workspace(eng):
         assert torch.equal(y, eng.linear(x, w, t, n, k, residual=res, act="silu"))
 
 
+def bf16(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).float().bfloat16().double().numpy()
+
+
+def prompt_bound(x, w, bias, act, residual):
+    """The product over weights rounded to bf16, in 64 bits, and what a bf16 result may be off by: the f32 sums
+    truncate at most once per 16 products and once per joined part (2^-23 of at most A = |x| . |w| each), the
+    activation's slope is at most 1.13 and its own error below 2^-20 of the sum, and the result is rounded once."""
+    v = x @ w.T
+    b = np.zeros(w.shape[0]) if bias is None else bias
+    e = 1.13 * 2.0 ** -23 * (x.shape[1] / 16 + 4) * (np.abs(x) @ np.abs(w).T + np.abs(b))
+    e = e + 2.0 ** -20 * np.abs(v + b)
+    v = act64(v + b, act)
+    v = v if residual is None else v + residual
+    return v, e + 2.0 ** -8 * (np.abs(v) + e)
+
+
+@pytest.mark.parametrize("t,layout", ALL, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [
+    (17, 1, 256),        # one output row, one column of K
+    (100, 129, 1280),    # a tile of one row; K splits of unequal length
+    (129, 300, 512),     # 256-token tiles, two of them
+    (600, 257, 2304),    # 256-token tiles again (few weight rows), split K
+])
+def test_linear_of_prompts(eng, oracle, t, layout, m, n, k):
+    r = np.random.default_rng(m + n)
+    raw = blocks(n, k, t, m)
+    x, b, s = (bf16(r.standard_normal(sh) * sc) for sh, sc in (((m, k), 1.0), (n, 1.0), ((m, n), 1.0)))
+    c = lambda a: torch.from_numpy(a).cuda().bfloat16()  # noqa: E731
+    act = ("none", "silu", "gelu", "gelu_tanh", "relu")[(m + t) % 5]
+    wd = eng.upload(raw)
+    w = bf16(dequant(oracle, raw, t, layout, n, k))
+    y = eng.linear(c(x), wd, t, n, k, bias=torch.from_numpy(b).float().cuda(), act=act, residual=c(s),
+                   q6k_layout=layout).double().cpu().numpy()
+    v, tol = prompt_bound(x, w, b, act, s)
+    assert np.all(np.abs(y - v) <= tol), (act, float((np.abs(y - v) / tol).max()))
+    # without an epilogue: the product that was there, bit for bit
+    plain = eng.linear(c(x), wd, t, n, k, q6k_layout=layout)
+    assert torch.equal(plain, eng.gemm_bf16(wd, t, c(x), n, k, q6k_layout=layout).reshape(m, n))
+
+
+@pytest.mark.parametrize("act", sorted(_lib.ACTS))
+def test_linear_of_prompts_every_epilogue(eng, oracle, act):
+    """512-token tiles without a K split and small ones with: each activation, with and without bias and residual."""
+    for m, n, k in ((513, 4900, 256), (40, 70, 1536)):
+        r = np.random.default_rng(m)
+        raw = blocks(n, k, Q4_K, m)
+        wd, w = eng.upload(raw), bf16(dequant(oracle, raw, Q4_K, 0, n, k))
+        x, b, s = bf16(3 * r.standard_normal((m, k))), bf16(r.standard_normal(n)), bf16(r.standard_normal((m, n)))
+        for bias, res in ((b, s), (b, None), (None, s), (None, None)):
+            t = lambda a, d: None if a is None else torch.from_numpy(a).cuda().to(d)  # noqa: E731
+            y = eng.linear(t(x, torch.bfloat16), wd, Q4_K, n, k, bias=t(bias, torch.float32), act=act,
+                           residual=t(res, torch.bfloat16)).double().cpu().numpy()
+            v, tol = prompt_bound(x, w, bias, act, res)
+            assert np.all(np.abs(y - v) <= tol), (m, act, float((np.abs(y - v) / tol).max()))
+
+
+def test_linear_of_prompts_in_place_rows_behind_and_captured(eng):
+    m, n, k = 333, 1003, 2816
+    wd = eng.upload(blocks(n, k, Q8_0, 6))
+    x = torch.randn(m, k, device="cuda").bfloat16()
+    bias = torch.randn(n, device="cuda")
+    big = torch.randn(m + 8, n, device="cuda").bfloat16()
+    before = big.clone()
+    want = eng.linear(x, wd, Q8_0, n, k, bias=bias, act="relu", residual=before[:m].contiguous())
+    eng.linear(x, wd, Q8_0, n, k, bias=bias, act="relu", residual=big[:m], out=big[:m])
+    assert torch.equal(big[:m], want) and torch.equal(big[m:], before[m:])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = eng.linear(x, wd, Q8_0, n, k, bias=bias, act="relu", residual=before[:m], sync=False)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    x[7, 3] = float("nan")
+    z = eng.linear(x, wd, Q8_0, n, k, bias=bias, act="relu", residual=before[:m])
+    keep = [i for i in range(m) if i != 7]
+    assert torch.equal(z[keep], want[keep]) and torch.isnan(z[7]).all()
+    for kw, status in ((dict(x=x.float()), _lib.ERR_SHAPE), (dict(x=x.reshape(-1)[1:1 + 32 * k].reshape(32, k)), _lib.ERR_ALIGN),
+                       (dict(k=2784, x=x[:, :2784].contiguous()), _lib.ERR_SHAPE)):
+        a = dict(x=x, w=wd, ggml_type=Q8_0, n=n, k=k)
+        a.update(kw)
+        with pytest.raises(_lib.NsqError) as e:
+            eng.linear(**a)
+        assert e.value.status == status, list(kw)
+
+
 def test_linear_refusals(eng):
     w = eng.upload(blocks(16, 256, Q4_K, 0))
     x = torch.zeros(2, 256, device="cuda")
