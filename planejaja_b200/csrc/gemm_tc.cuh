@@ -42,6 +42,7 @@
 
 #include <stdlib.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "nsq_common.cuh"
@@ -304,33 +305,75 @@ struct GemmParams {
   const __nv_bfloat16* residual;  // [M x N] or NULL, may be y
 };
 
-// The epilogue of 32 tokens m0 .. m0 + 31 of output row n, sums in v (f32, so
-// bias, activation and residual are applied before the one rounding to bf16).
-// Its loads and stores are those of the plain epilogue: 64 bytes per warp and
-// token.  Not inlined: the activations are 20 to 40 instructions an element,
-// once for each of 21 kernels.
-__device__ __forceinline__ float gemm_act(float v, int act) {
-  if (act == NSQ_ACT_SILU) return v / (1.0f + expf(-v));
-  if (act == NSQ_ACT_GELU) return 0.5f * v * erfcf(-0.70710678118654752f * v);
-  if (act == NSQ_ACT_GELU_TANH) return v / (1.0f + expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
-  if (act == NSQ_ACT_RELU) return v < 0.0f ? 0.0f : v;
-  return v;
+// v (1 + erf(v / sqrt 2)) / 2 = v Phi(v), with h = Phi(-|v|) = erfc(u) / 2 at
+// u = |v| / sqrt 2 written as e^(-u^2) P(t), t = 1 / (1 + u / 2); P is the
+// polynomial of degree 7 without a constant term fitted to e^(u^2) erfc(u) / 2
+// over u = 0..10 for the least largest relative error, 1.4e-6.  With the f32
+// roundings h is off by at most 8e-6 of itself for |v| <= 13 and 8e-7
+// absolutely: far inside the result's rounding to bf16, and a third of the
+// instructions of erfcf.
+__device__ __forceinline__ float gemm_gelu(float v) {
+  const float a = fabsf(v);
+  const float t = __fdividef(1.0f, fmaf(0.35355339f, a, 1.0f));
+  float h = 0.0441020165f;
+  h = fmaf(h, t, -0.178368577f);
+  h = fmaf(h, t, 0.194611529f);
+  h = fmaf(h, t, 0.0189458649f);
+  h = fmaf(h, t, 0.14075168f);
+  h = fmaf(h, t, 0.138791108f);
+  h = fmaf(h, t, 0.141165703f);
+  h *= t * __expf(-0.5f * a * a);
+  return v * (v > 0.0f ? 1.0f - h : h);
 }
-static __device__ __noinline__ void gemm_epilogue(const GemmParams& p, int64_t n, int64_t m0, float* v) {
-  const int count = (int)min((int64_t)32, p.M - m0);
-  const float bias = p.bias ? p.bias[n] : 0.0f;
-  const int64_t at = m0 * p.N + n;
-  const int act = p.act;
-#pragma unroll 1
-  for (int j0 = 0; j0 < count; j0 += 8) {
-    float r[8];
+
+// The epilogue of the C tokens m0 .. m0 + C - 1 of output row n, sums in
+// v[OFF ..]: bias, activation and residual in f32, one rounding to bf16.
+// Lanes are output rows, so a token's load or store is 64 bytes per warp, as
+// in the plain epilogue.  All of it stays in registers, the activation is
+// chosen once per C elements, and the residuals' loads are under way together
+// before the first is used.  (As one call per 8 elements on an array in
+// memory: Q4_K [14336 x 4096] at M = 512, 113 us against 60 for the plain
+// product.)
+template <int ACT, int C, int OFF, int L>
+__device__ __forceinline__ void gemm_act(float (&v)[L]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      r[j] = p.residual && j0 + j < count ? __bfloat162float(p.residual[at + (j0 + j) * p.N]) : 0.0f;
+  for (int j = OFF; j < OFF + C; ++j) {
+    if constexpr (ACT == NSQ_ACT_SILU) v[j] = __fdividef(v[j], 1.0f + __expf(-v[j]));
+    if constexpr (ACT == NSQ_ACT_GELU) v[j] = gemm_gelu(v[j]);
+    if constexpr (ACT == NSQ_ACT_GELU_TANH)
+      v[j] = __fdividef(v[j], 1.0f + __expf(-1.5957691216057308f * (v[j] + 0.044715f * v[j] * v[j] * v[j])));
+    if constexpr (ACT == NSQ_ACT_RELU) v[j] = v[j] < 0.0f ? 0.0f : v[j];
+  }
+}
+template <int C, int OFF, int L>
+__device__ __forceinline__ void gemm_epilogue(const GemmParams& p, int64_t n, int64_t m0, float (&v)[L]) {
+  const int count = (int)min((int64_t)C, p.M - m0);
+  const int64_t N = p.N, at = m0 * N + n;
+  const float bias = p.bias ? __ldg(p.bias + n) : 0.0f;
+  uint16_t r[C];
+  const bool add = p.residual != nullptr;
+  if (add) {
+    const uint16_t* res = reinterpret_cast<const uint16_t*>(p.residual) + at;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j0 + j < count) p.y[at + (j0 + j) * p.N] = __float2bfloat16_rn(gemm_act(v[j0 + j] + bias, act) + r[j]);
-    }
+    for (int j = 0; j < C; ++j) r[j] = j < count ? res[j * N] : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < C; ++j) v[OFF + j] += bias;
+  switch (p.act) {
+    case NSQ_ACT_SILU: gemm_act<NSQ_ACT_SILU, C, OFF>(v); break;
+    case NSQ_ACT_GELU: gemm_act<NSQ_ACT_GELU, C, OFF>(v); break;
+    case NSQ_ACT_GELU_TANH: gemm_act<NSQ_ACT_GELU_TANH, C, OFF>(v); break;
+    case NSQ_ACT_RELU: gemm_act<NSQ_ACT_RELU, C, OFF>(v); break;
+    default: break;
+  }
+  if (add) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[OFF + j] += __uint_as_float((uint32_t)r[j] << 16);
+  }
+  __nv_bfloat16* y = p.y + at;
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    if (j < count) y[j * N] = __float2bfloat16_rn(v[OFF + j]);
   }
 }
 
@@ -506,6 +549,18 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
         if (lane == 0) mbar_arrive(&raw_full[rs]);
       }
     }
+  } else if (EPI && warp == 3) {
+    // ---- the tile's residuals into L2 (this rank's share of the tokens):
+    // the epilogue reads them when nothing else is left to hide DRAM behind
+    if (p.residual) {
+      const int64_t bytes = 2 * (int64_t)rows_valid;
+      const int rows = (int)min((int64_t)TOK, p.M - m0);
+      for (int i = rank * 32 + lane; i < rows; i += 32 * split) {
+        const uint8_t* row = reinterpret_cast<const uint8_t*>(p.residual + (m0 + i) * p.N + n0);
+        for (int64_t o = 0; o < bytes; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + o));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(row + bytes - 2));
+      }
+    }
   } else if (warp >= GEMM_DQ_WARP0) {
     bool ok = true;
     if constexpr (kColumnWarps) {
@@ -632,7 +687,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
             float e[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) e[j] = __uint_as_float(v[j]);
-            if (n < p.N) gemm_epilogue(p, n, (int64_t)m0 + cc, e);
+            if (n < p.N) {  // 16 at a time: 32 sums and 32 residuals do not fit the registers
+              gemm_epilogue<16, 0>(p, n, (int64_t)m0 + cc, e);
+              gemm_epilogue<16, 16>(p, n, (int64_t)m0 + cc + 16, e);
+            }
           } else if (n < p.N) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -646,63 +704,68 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
   }
   if (split > 1) {
     // Split-K reduction through distributed shared memory, in rounds of 32
-    // accumulator columns per epilogue warp.  The non-leader ranks store
-    // their partial sums into the leader's shared memory (the stage and raw
-    // buffers, idle once the MMAs are done; slot [rank - 1][warp][lane][32]
-    // f32), the leader adds them in rank order and writes bf16.  Every
-    // thread of every CTA passes the same cluster barriers.
+    // accumulator columns (tokens) per epilogue warp.  A round's columns are
+    // shared out among the ranks in groups of four: every rank stores its
+    // partial sums of a group into the owner's shared memory (the stage and
+    // raw buffers, idle once the MMAs are done; slot [rank][warp][group][lane]
+    // of four f32, so a warp's store is 512 consecutive bytes), the owner adds
+    // them in rank order and writes bf16.  Every thread of every CTA passes
+    // the same cluster barriers.  (With one owner of everything, and a lane's
+    // 32 sums side by side, S = 4 cost 18 us on a 128-token tile.)
     constexpr int kRounds = TOK / 4 / 32;
-    float* slots = reinterpret_cast<float*>(smem);
+    float4* slots = reinterpret_cast<float4*>(smem);
     const bool epi_warp = warp >= GEMM_DQ_WARP0;
     const int qd = warp & 3;
     const int part = (warp - GEMM_DQ_WARP0) >> 2;
     const int ew = warp - GEMM_DQ_WARP0;  // 0..15
+    const int gmax = (8 + split - 1) / split;  // groups of one owner, at most
+    const int g0 = 8 * rank / split, g1 = 8 * (rank + 1) / split;
+    __syncwarp();
     gemm_cluster_sync();  // every CTA of the cluster is past its main loop
 #pragma unroll 1
     for (int rd = 0; rd < kRounds; ++rd) {
       const int cc = part * (TOK / 4) + 32 * rd;
-      uint32_t v[32];
       if (epi_warp) {
+        uint32_t v[32];
         if (have) {
           tc_ld_32x32b_x32(tmem_d + ((uint32_t)(32 * qd) << 16) + (uint32_t)cc, v);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0u;
         }
-        if (rank > 0) {
-          const uint32_t dst = gemm_cluster_map(slots + ((size_t)((rank - 1) * 16 + ew) * 32 + lane) * 32, 0);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) gemm_st_cluster_v4(dst + 4 * j, v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int g = 0; g < 8; ++g) {
+          const int owner = (split * (g + 1) - 1) / 8;  // the q with 8 q / split <= g < 8 (q + 1) / split
+          const int at = ((rank * 16 + ew) * gmax + g - 8 * owner / split) * 32 + lane;
+          gemm_st_cluster_v4(gemm_cluster_map(slots + at, (uint32_t)owner), v[4 * g], v[4 * g + 1], v[4 * g + 2],
+                             v[4 * g + 3]);
         }
       }
-      gemm_cluster_sync();  // partials of this round have landed in the leader
-      if (epi_warp && rank == 0) {
+      gemm_cluster_sync();  // partials of this round have landed
+      if (epi_warp && have) {
         const int64_t n = n0 + 32 * qd + lane;
-        float acc[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) acc[j] = __uint_as_float(v[j]);
-        for (int r = 1; r < split; ++r) {
-          const float4* src = reinterpret_cast<const float4*>(slots + ((size_t)((r - 1) * 16 + ew) * 32 + lane) * 32);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 f = src[j];
-            acc[4 * j] += f.x;
-            acc[4 * j + 1] += f.y;
-            acc[4 * j + 2] += f.z;
-            acc[4 * j + 3] += f.w;
+#pragma unroll 1
+        for (int g = g0; g < g1; ++g) {
+          float acc[4] = {};
+          for (int r = 0; r < split; ++r) {
+            const float4 f = slots[((r * 16 + ew) * gmax + g - g0) * 32 + lane];
+            acc[0] = r ? acc[0] + f.x : f.x;
+            acc[1] = r ? acc[1] + f.y : f.y;
+            acc[2] = r ? acc[2] + f.z : f.z;
+            acc[3] = r ? acc[3] + f.w : f.w;
           }
-        }
-        if constexpr (EPI) {
-          if (n < p.N && have) gemm_epilogue(p, n, (int64_t)m0 + cc, acc);
-        } else if (n < p.N && have) {
+          const int64_t m = (int64_t)m0 + cc + 4 * g;
+          if constexpr (EPI) {
+            if (n < p.N) gemm_epilogue<4, 0>(p, n, m, acc);
+          } else if (n < p.N) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int64_t m = (int64_t)m0 + cc + j;
-            if (m < p.M) p.y[m * p.N + n] = __float2bfloat16_rn(acc[j]);
+            for (int j = 0; j < 4; ++j) {
+              if (m + j < p.M) p.y[(m + j) * p.N + n] = __float2bfloat16_rn(acc[j]);
+            }
           }
         }
       }
-      gemm_cluster_sync();  // the leader is done with the slots of this round
+      gemm_cluster_sync();  // the owners are done with the slots of this round
     }
   }
   tc_fence_before();
@@ -775,9 +838,9 @@ static int launch_gemm_t(const void* x, const CUtensorMap& wmap, const GemmParam
                             (size_t)GEMM_RAW_STAGES * GEMM_BM * RawCol<TYPE>::pitch;
   int S = 1;
   const int64_t tiles = tiles_n * tiles_m, ncol = p.K / 256;
-  S = tune(kTuneGemmSplit, num_sms > 0 && tiles * 2 <= num_sms ? (int)(num_sms / tiles) : 1);
-  if (S > 4) S = 4;
-  while (S > 1 && (ncol < 2 * S || (size_t)(S - 1) * 16 * 32 * 32 * 4 > region)) --S;
+  S = tune(kTuneGemmSplit, EPI ? p.S : num_sms > 0 && tiles * 2 <= num_sms ? (int)(num_sms / tiles) : 1);
+  if (S > (EPI ? 8 : 4)) S = EPI ? 8 : 4;
+  while (S > 1 && (ncol < (EPI ? 1 : 2) * S || (!EPI && (size_t)(S - 1) * 16 * 32 * 32 * 4 > region))) --S;
   if (S < 1) S = 1;
   p.S = S;
   cudaLaunchConfig_t cfg = {};
@@ -794,6 +857,58 @@ static int launch_gemm_t(const void* x, const CUtensorMap& wmap, const GemmParam
   cfg.numAttrs = S > 1 ? 1 : 0;
   note_launch();
   return cudaLaunchKernelEx(&cfg, kern, map, wmap, p) == cudaSuccess ? NSQ_OK : NSQ_ERR_CUDA;
+}
+
+// Clusters of S of the kernel's CTAs (one per SM) that the device holds at
+// once: a GPC's SMs are no multiple of S.
+template <int TYPE, int LAYOUT, int TOK>
+static int gemm_clusters(int S, int num_sms) {
+  if (S == 1) return num_sms;
+  static std::atomic<int> known[64][9] = {};
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms / S;
+  if ((n = known[dev][S].load(std::memory_order_relaxed)) > 0) return n;
+  auto kern = gemm_tc_kernel<TYPE, LAYOUT, TOK, true>;
+  const size_t smem = gemm_smem_bytes<TYPE, TOK>();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)S);
+  cfg.blockDim = dim3(GEMM_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)S;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = num_sms / S > 0 ? num_sms / S : 1;
+  }
+  known[dev][S].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Token tile and split of nsq_linear's kernel: the least waves x (start + K
+// columns of a CTA x cost of one) + joining of the ranks' sums.  In tenths of
+// a column of a 128-token tile, which is 1.9 us, with Q4_K at N = K = 4096 and
+// M = 17 to 1000 (the other formats' ratios are close): columns of 256 and 512
+// tokens cost 3.2 and 3.3 us (the ring then holds no whole column); joins 2.5,
+// 6 and 11 us.  M = 333, N = 1003, K = 2816 (Q8_0): 128 tokens, S = 4 14 us;
+// 256 tokens, S = 4 18 us; 128 tokens, S = 8 (24 clusters, 2 waves) 25 us.
+// M = 1000, N = K = 4096: 512 tokens, S = 2 46 us; 256, S = 1 55; 128, S = 1 74.
+template <int TYPE, int LAYOUT, int TOK>
+static void gemm_consider(const GemmParams& p, int num_sms, int64_t* best, int* tok, int* split) {
+  constexpr int64_t kColumn = TOK == 128 ? 10 : TOK == 256 ? 17 : 18, kStart = TOK == 128 ? 37 : 25;
+  constexpr int64_t kJoin = TOK == 128 ? 13 : TOK == 256 ? 33 : 60;
+  const int64_t tiles = ((p.N + GEMM_BM - 1) / GEMM_BM) * ((p.M + TOK - 1) / TOK), ncol = p.K / 256;
+  for (int S = 1; S <= 8 && S <= ncol && tiles * S <= (S > 1 ? num_sms : INT64_MAX); ++S) {
+    const int cap = gemm_clusters<TYPE, LAYOUT, TOK>(S, num_sms > 0 ? num_sms : 1);
+    const int64_t waves = (tiles + cap - 1) / cap;
+    const int64_t cost = waves * (kStart + (ncol + S - 1) / S * kColumn) + (S > 1 ? kJoin : 0);
+    if (cost < *best) *best = cost, *tok = TOK, *split = S;
+  }
 }
 
 template <int TYPE, int LAYOUT, bool EPI>
@@ -815,6 +930,17 @@ static int run_gemm_t(const void* x, const GemmParams& p0, int tok, cudaStream_t
         p.wmap_ok = 1;
     }
   }
+  if constexpr (EPI) {
+    int64_t best = INT64_MAX;
+    int t = 128;
+    gemm_consider<TYPE, LAYOUT, 128>(p, num_sms, &best, &t, &p.S);
+    if (p.M > 128) gemm_consider<TYPE, LAYOUT, 256>(p, num_sms, &best, &t, &p.S);
+    if constexpr (gemm_stages<TYPE, 512>() >= 2) {
+      if (p.M > 256) gemm_consider<TYPE, LAYOUT, 512>(p, num_sms, &best, &t, &p.S);
+    }
+    const int te = tune(kTuneGemmTok, 0);
+    tok = te == 128 || te == 256 || te == 512 ? te : t;
+  }
   if (tok == 128) return launch_gemm_t<TYPE, LAYOUT, 128, EPI>(x, wmap, p, st, num_sms);
   if constexpr (gemm_stages<TYPE, 512>() >= 2) {
     if (tok == 512) return launch_gemm_t<TYPE, LAYOUT, 512, EPI>(x, wmap, p, st, num_sms);
@@ -829,7 +955,7 @@ static int run_gemm(const GemmParams& p0, int type, int layout, const void* x, c
   if (K % 256) return NSQ_ERR_SHAPE;  // whole 256-weight columns
   GemmParams p = p0;
   p.RB = (K / nsq_block_weights(type)) * nsq_block_bytes(type);
-  // tokens per CTA: 128 for short prompts, else 256 or 512 (NSQ_GEMM_TOK
+  // tokens per CTA (EPI chooses for itself): 128 for short prompts, else 256 or 512 (NSQ_GEMM_TOK
   // overrides); a 512-token tile reuses each dequantized weight tile twice
   // as often, where two 64-wide stages of it fit beside the raw bytes
   int tok = M <= 128 ? 128 : (M >= 512 ? 512 : 256);
