@@ -16,17 +16,17 @@
 //
 // Warp roles (384 threads):
 //   warp 0      : TMA producer -- one thread loads the x tile [TOK x 64]
-//                 (2-D tiled bulk tensor copy, 128B swizzle) per K block.
+//                 (2-D tiled bulk tensor copies, 128B swizzle) per K block.
 //   warp 1      : allocates TMEM; one thread issues 4 tcgen05.mma
 //                 (kind::f16, bf16 inputs, fp32 accumulate, K = 16 each)
-//                 per K block and commits them to the stage's "empty"
-//                 barrier, and finally to the accumulator barrier.
+//                 per K block and 256 tokens and commits them to the
+//                 stage's "empty" barrier, and finally to the accumulator's.
 //   warps 4..11 : dequant producers -- 2 threads per W row turn the GGUF
 //                 blocks of the K block into bf16 and store them in the
 //                 same 128B-swizzled K-major layout TMA uses; then the
 //                 epilogue: tcgen05.ld of the accumulator, bf16 convert,
 //                 store to y.
-// Stages form a 4-deep ring guarded by mbarriers.  Every wait is bounded
+// W and x tiles go round in rings guarded by mbarriers.  Every wait is bounded
 // (%globaltimer); a wait that gives up records NSQ_ERR_TIMEOUT and the
 // kernel winds down instead of hanging.
 //
@@ -68,13 +68,31 @@ template <> struct RawCol<NSQ_TYPE_Q4_0> { static constexpr int bytes = 144, pit
 template <> struct RawCol<NSQ_TYPE_Q8_0> { static constexpr int bytes = 272, pitch = 272; };
 template <> struct RawCol<NSQ_TYPE_Q6_K> { static constexpr int bytes = 210, pitch = 240; };
 
-// bf16 W / x stages (64-wide K blocks): as many as fit beside the raw ring
+// Stages (64-wide K blocks) of a W tile and a whole x tile that fit beside the
+// raw ring: the tile sizes and splits of nsq_gemm_bf16 are chosen by it.
 template <int TYPE, int TOK>
 __host__ __device__ constexpr int gemm_stages() {
   constexpr int fixed = 1024 + GEMM_RAW_STAGES * 128 * RawCol<TYPE>::pitch + 256;
   constexpr int per = 128 * 128 + TOK * 128;
   constexpr int n = (GEMM_SMEM_LIMIT - fixed) / per;
   return n > 6 ? 6 : n;
+}
+// W and x tiles share the stages of one ring; or go round in two rings of
+// their own where a 256-token tile then leaves room for the four W tiles that
+// kColumnWarps wants (Q4_K, N = K = 4096, M = 1000: 53 -> 42 us).  Elsewhere
+// two rings only cost the MMA thread a wait and a commit per K block (128
+// tokens, 14336 x 4096: 41 against 37 us; 512 tokens with half tiles freed
+// separately: 67 against 57 us, where shared memory's bandwidth binds: MMA
+// operands, x tiles and W tiles are 170 to 190 KB per 1024 cycles of MMA).
+template <int TYPE, int TOK>
+__host__ __device__ constexpr int gemm_w_stages() {
+  constexpr int avail = GEMM_SMEM_LIMIT - 1024 - GEMM_RAW_STAGES * 128 * RawCol<TYPE>::pitch - 256;
+  if (TOK == 256 && avail >= 4 * 16384 + 3 * 32768) return 4;
+  return gemm_stages<TYPE, TOK>();
+}
+template <int TYPE, int TOK>
+__host__ __device__ constexpr int gemm_x_stages() {
+  return gemm_stages<TYPE, TOK>();
 }
 
 // ---------------------------------------------------------------------------
@@ -401,29 +419,32 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
                                                                    const __grid_constant__ CUtensorMap wmap,
                                                                    const GemmParams p) {
   constexpr uint32_t W_STAGE = GEMM_BM * 128;  // bytes
-  constexpr uint32_t X_STAGE = TOK * 128;
   constexpr uint32_t RAW_STAGE = GEMM_BM * RawCol<TYPE>::pitch;
   constexpr int CB = RawCol<TYPE>::bytes;
   // UMMA N is at most 256: a 512-token tile is two MMAs per K step into
   // accumulator columns [0, 256) and [256, 512)
   constexpr int NH = TOK > 256 ? 2 : 1;
   constexpr int TN = TOK / NH;
+  constexpr uint32_t X_STAGE = TOK * 128;
   constexpr uint32_t IDESC = umma_idesc_bf16(GEMM_BM, TN);
-  constexpr int GEMM_STAGES = gemm_stages<TYPE, TOK>();
-  // When the ring holds a whole 256-wide column (four K stages, TOK = 128),
+  constexpr int GEMM_STAGES = gemm_w_stages<TYPE, TOK>(), X_STAGES = gemm_x_stages<TYPE, TOK>();
+  // When the ring holds a whole 256-wide column (four K stages),
   // dequant warp (q, h) writes K stage q of rows [32h, 32h + 32) of every
   // column: 64 weights per thread and one set of barrier waits per column,
   // instead of 16 weights per thread and per stage.
   constexpr bool kColumnWarps = GEMM_STAGES >= 4;
-  constexpr int kFullArrivals = 1 + (kColumnWarps ? 4 : GEMM_DQ_THREADS / 32);
+  constexpr bool kTwoRings = GEMM_STAGES != X_STAGES;
+  constexpr int kFullArrivals = (kTwoRings ? 0 : 1) + (kColumnWarps ? 4 : GEMM_DQ_THREADS / 32);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* w_sm = smem;
   uint8_t* x_sm = smem + GEMM_STAGES * W_STAGE;
-  uint8_t* raw_sm = x_sm + GEMM_STAGES * X_STAGE;
+  uint8_t* raw_sm = x_sm + X_STAGES * X_STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(raw_sm + GEMM_RAW_STAGES * RAW_STAGE);
   uint64_t* empty = full + GEMM_STAGES;
-  uint64_t* raw_full = empty + GEMM_STAGES;
+  uint64_t* x_full = kTwoRings ? empty + GEMM_STAGES : full;
+  uint64_t* x_empty = kTwoRings ? x_full + X_STAGES : empty;
+  uint64_t* raw_full = x_empty + X_STAGES;
   uint64_t* raw_empty = raw_full + GEMM_RAW_STAGES;
   uint64_t* accum = raw_empty + GEMM_RAW_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
@@ -444,6 +465,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
     for (int s = 0; s < GEMM_STAGES; ++s) {
       mbar_init(&full[s], kFullArrivals);
       mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; kTwoRings && s < X_STAGES; ++s) {
+      mbar_init(&x_full[s], 1);
+      mbar_init(&x_empty[s], 1);
     }
     for (int s = 0; s < GEMM_RAW_STAGES; ++s) {
       mbar_init(&raw_full[s], 1);
@@ -466,39 +491,54 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
   if (warp == 0) {
     // ---- x tiles: TMA 2-D, 128B swizzle
     if (lane == 0) {
+      int s = 0;
+      uint32_t par = 1;
       for (int kb = kb0; kb < kb1; ++kb) {
-        const int s = (kb - kb0) % GEMM_STAGES;
-        const uint32_t par = (uint32_t)(((kb - kb0) / GEMM_STAGES) & 1);
-        if (!mbar_wait_bounded(&empty[s], par ^ 1)) break;
-        mbar_arrive_expect_tx(&full[s], X_STAGE);
+        if (!mbar_wait_bounded(&x_empty[s], par)) break;
+        mbar_arrive_expect_tx(&x_full[s], X_STAGE);
 #pragma unroll
         for (int h = 0; h < NH; ++h)
-          tma_load_2d(x_sm + s * X_STAGE + h * TN * 128, &xmap, kb * GEMM_BK, m0 + h * TN, &full[s]);
+          tma_load_2d(x_sm + s * X_STAGE + h * TN * 128, &xmap, kb * GEMM_BK, m0 + h * TN, &x_full[s]);
+        if (++s == X_STAGES) {
+          s = 0;
+          par ^= 1;
+        }
       }
     }
   } else if (warp == 1) {
     // ---- MMA issue (one thread)
     if (lane == 0) {
-      const uint32_t w_base = smem_u32(w_sm), x_base = smem_u32(x_sm);
+      // (few instructions per K block: this thread's issue is on the critical
+      // path, one more wait and commit per block costs 10%)
+      const uint64_t w_desc = umma_desc_sw128(smem_u32(w_sm)), x_desc = umma_desc_sw128(smem_u32(x_sm));
       bool ok = true;
+      int s = 0, xs = 0;
+      uint32_t par = 0, xpar = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        const int s = (kb - kb0) % GEMM_STAGES;
-        const uint32_t par = (uint32_t)(((kb - kb0) / GEMM_STAGES) & 1);
-        if (!mbar_wait_bounded(&full[s], par)) {
+        if ((kTwoRings && !mbar_wait_bounded(&x_full[xs], xpar)) || !mbar_wait_bounded(&full[s], par)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const uint64_t wd = w_desc + (uint32_t)s * (W_STAGE / 16);  // (the address field counts 16 bytes)
+        const uint64_t xd = x_desc + (uint32_t)(kTwoRings ? xs : s) * (X_STAGE / 16);
 #pragma unroll
         for (int kk = 0; kk < GEMM_BK / 16; ++kk) {
-          const uint64_t ad = umma_desc_sw128(w_base + s * W_STAGE + kk * 32);
 #pragma unroll
-          for (int h = 0; h < NH; ++h) {
-            const uint64_t bd = umma_desc_sw128(x_base + s * X_STAGE + h * TN * 128 + kk * 32);
-            tc_mma_bf16(tmem_d + (uint32_t)(h * TN), ad, bd, IDESC, (kb != kb0 || kk != 0) ? 1u : 0u);
-          }
+          for (int h = 0; h < NH; ++h)
+            tc_mma_bf16(tmem_d + (uint32_t)(h * TN), wd + 2 * kk, xd + (uint32_t)(h * TN * 8 + 2 * kk), IDESC,
+                        (kb != kb0 || kk != 0) ? 1u : 0u);
         }
+        if (kTwoRings) tc_commit(&x_empty[xs]);
         tc_commit(&empty[s]);
+        if (++s == GEMM_STAGES) {
+          s = 0;
+          par ^= 1;
+        }
+        if (kTwoRings && ++xs == X_STAGES) {
+          xs = 0;
+          xpar ^= 1;
+        }
       }
       if (ok) tc_commit(accum);
     }
@@ -631,9 +671,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
     const int qq = (t >> 3) & 3;
     const int r = (t & 7) | ((t >> 5) << 3);
     const bool row_ok = r < rows_valid;
+    int s = 0;
+    uint32_t spar = 1;
     for (int kb = kb0; kb < kb1; ++kb) {
       const int c = kb >> 2, q = kb & 3, rs = (c - c0) % GEMM_RAW_STAGES;
-      const int s = (kb - kb0) % GEMM_STAGES;
       if (q == 0 && !mbar_wait_bounded(&raw_full[rs], (uint32_t)(((c - c0) / GEMM_RAW_STAGES) & 1))) {
         ok = false;
         break;
@@ -655,7 +696,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[rs]);
       }
-      if (!mbar_wait_bounded(&empty[s], (uint32_t)((((kb - kb0) / GEMM_STAGES) & 1) ^ 1))) {
+      if (!mbar_wait_bounded(&empty[s], spar)) {
         ok = false;
         break;
       }
@@ -668,6 +709,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
+      if (++s == GEMM_STAGES) {
+        s = 0;
+        spar ^= 1;
+      }
     }
     }
     // ---- epilogue: warp w reads TMEM lanes 32*(w%4).. (its W rows) for a
@@ -806,9 +851,14 @@ static int encode_xmap(CUtensorMap* map, const void* x, int64_t M, int64_t K, in
 
 template <int TYPE, int TOK>
 static size_t gemm_smem_bytes() {
-  constexpr int S = gemm_stages<TYPE, TOK>();
-  return 1024 + (size_t)S * (GEMM_BM * 128 + TOK * 128) + (size_t)GEMM_RAW_STAGES * GEMM_BM * RawCol<TYPE>::pitch +
-         (2 * S + 2 * GEMM_RAW_STAGES + 1) * 8 + 16;
+  constexpr int W = gemm_w_stages<TYPE, TOK>(), X = gemm_x_stages<TYPE, TOK>();
+  constexpr size_t bytes = 1024 + (size_t)W * GEMM_BM * 128 + (size_t)X * TOK * 128 +
+                           (size_t)GEMM_RAW_STAGES * GEMM_BM * RawCol<TYPE>::pitch +
+                           (2 * W + 2 * X + 2 * GEMM_RAW_STAGES + 1) * 8 + 16;
+  static_assert(bytes <= GEMM_SMEM_LIMIT && W >= 2 && X >= 2, "the rings do not fit");
+  // the joining of a split's sums uses up to 112 KB of the rings
+  static_assert((size_t)W * GEMM_BM * 128 + (size_t)X * TOK * 128 >= 7 * 16 * 2 * 32 * 16, "");
+  return bytes;
 }
 
 template <int TYPE, int LAYOUT, int TOK, bool EPI>
@@ -831,7 +881,7 @@ static int launch_gemm_t(const void* x, const CUtensorMap& wmap, const GemmParam
   GemmParams p = p0;
   const int64_t tiles_n = (p.N + GEMM_BM - 1) / GEMM_BM, tiles_m = (p.M + TOK - 1) / TOK;
   if (tiles_m > 65535) return NSQ_ERR_SHAPE;
-  // Split-K when the tiles leave most SMs idle: S CTAs per tile (cluster),
+  // Split-K (nsq_gemm_bf16; the order of its sums hangs on it) when the tiles leave most SMs idle: S CTAs per tile (cluster),
   // as many as the SMs allow, at most 4, each with >= 2 K columns, and no
   // more partial-sum slots than the leader's stage buffers hold.
   constexpr size_t region = (size_t)gemm_stages<TYPE, TOK>() * (GEMM_BM * 128 + TOK * 128) +
@@ -892,16 +942,17 @@ static int gemm_clusters(int S, int num_sms) {
 
 // Token tile and split of nsq_linear's kernel: the least waves x (start + K
 // columns of a CTA x cost of one) + joining of the ranks' sums.  In tenths of
-// a column of a 128-token tile, which is 1.9 us, with Q4_K at N = K = 4096 and
+// a column of a 128-token tile, which is 1.75 us, with Q4_K at N = K = 4096 and
 // M = 17 to 1000 (the other formats' ratios are close): columns of 256 and 512
-// tokens cost 3.2 and 3.3 us (the ring then holds no whole column); joins 2.5,
-// 6 and 11 us.  M = 333, N = 1003, K = 2816 (Q8_0): 128 tokens, S = 4 14 us;
-// 256 tokens, S = 4 18 us; 128 tokens, S = 8 (24 clusters, 2 waves) 25 us.
-// M = 1000, N = K = 4096: 512 tokens, S = 2 46 us; 256, S = 1 55; 128, S = 1 74.
+// tokens cost 2.3 and 3.3 us (3.0 for 256 without rings of their own); joins
+// 2.5, 6 and 11 us.  M = 333, N = 1003, K = 2816 (Q8_0): 128 tokens, S = 4
+// 14 us; 256 tokens, S = 4 18 us; 128 tokens, S = 8 (24 clusters, 2 waves)
+// 25 us.  M = 1000, N = K = 4096: 256 tokens, S = 1 42 us; 512, S = 2 46 us;
+// 128, S = 1 74 us.
 template <int TYPE, int LAYOUT, int TOK>
 static void gemm_consider(const GemmParams& p, int num_sms, int64_t* best, int* tok, int* split) {
-  constexpr int64_t kColumn = TOK == 128 ? 10 : TOK == 256 ? 17 : 18, kStart = TOK == 128 ? 37 : 25;
-  constexpr int64_t kJoin = TOK == 128 ? 13 : TOK == 256 ? 33 : 60;
+  constexpr int64_t kColumn = TOK == 128 ? 10 : TOK == 512 ? 19 : gemm_w_stages<TYPE, TOK>() >= 4 ? 13 : 17;
+  constexpr int64_t kStart = TOK == 128 ? 40 : 28, kJoin = TOK == 128 ? 13 : TOK == 256 ? 35 : 60;
   const int64_t tiles = ((p.N + GEMM_BM - 1) / GEMM_BM) * ((p.M + TOK - 1) / TOK), ncol = p.K / 256;
   for (int S = 1; S <= 8 && S <= ncol && tiles * S <= (S > 1 ? num_sms : INT64_MAX); ++S) {
     const int cap = gemm_clusters<TYPE, LAYOUT, TOK>(S, num_sms > 0 ? num_sms : 1);

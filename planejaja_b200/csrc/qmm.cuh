@@ -258,6 +258,16 @@ __device__ __forceinline__ void qmm_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
+// 16 bytes to shared memory; those past the first `bytes` are zeros and not read.
+__device__ __forceinline__ void qmm_cp_async(uint32_t dst, const uint8_t* src, int bytes, uint64_t pol) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes), "l"(pol)
+               : "memory");
+}
+// One arrival when all copies of this thread so far have landed.
+__device__ __forceinline__ void qmm_cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // fp16 MMA (mins against T), accumulating from zero.
 __device__ __forceinline__ void qmm_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                             uint32_t b1) {
@@ -982,7 +992,8 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     }
     for (int i = 0; i < KW; ++i) {
       for (int k = 0; k < S; ++k) {
-        mbar_init(&full[i][k], RW == 1 ? 1 : RW + 1);  // rows of every warp, records (one warp: both at once)
+        // rows of every warp (one arrival per warp, or per lane), records (one warp: with the rows)
+        mbar_init(&full[i][k], (p.rows_aligned ? RW : 32 * RW) + (RW > 1));
         mbar_init(&used[i][k], RW);
       }
     }
@@ -1106,27 +1117,28 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         if constexpr (MODE == kQmmUp) qmm_tma_2d(dst + (WR / 2) * pitch, &map1, x, row0, bar, pol);
       }
     } else {
-      // one lane per row; a tensor's bytes past its last whole 16 are stored by hand
+      // four lanes per row copy 16 bytes each at a time: one bulk copy per row
+      // takes 650 to 1300 cycles a unit to issue
       int need = F::CB;
       if constexpr (Fmt<TYPE>::QK == 32) need = min(8, p.nblk - 8 * pc.sb) * BB;
-      const bool up = MODE == kQmmUp && lane >= WR / 2;
-      const int r = up ? lane - WR / 2 : lane;
-      const uint8_t* w = up ? p.w1 : p.w0;
-      const int64_t at = ((int64_t)expert_of(pc) * p.n + first + r) * p.rb + (int64_t)pc.sb * F::CB;
-      const int64_t a16 = at & ~(int64_t)15, end = at + need, cap = p.wbytes & ~(int64_t)15;
-      int64_t e = (end + 15) & ~(int64_t)15;
-      if (e > cap) e = cap > a16 ? cap : a16;
-      const bool valid = lane < WR && first + r < p.n;
-      uint8_t* dst = smem + slot + lane * pitch;
-      const uint32_t bytes = valid ? (uint32_t)(e - a16) : 0u;
-      if (valid && e < end) {
-        for (int64_t i = e; i < end; ++i) dst[i - a16] = w[i];
-        fence_proxy_async_smem();
-      }
-      const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
-      if (lane == 0) mbar_arrive_expect_tx(bar, total + more);
+      if (more != 0 && lane == 0) qmm_expect_tx(bar, more);
       __syncwarp();
-      if (bytes) bulk_g2s_hint(dst, w + a16, bytes, bar, pol);
+      const int64_t row0 = (int64_t)expert_of(pc) * p.n + first;
+#pragma unroll 1
+      for (int r = lane >> 2; r < WR; r += 8) {
+        const int rr = MODE == kQmmUp && r >= WR / 2 ? r - WR / 2 : r;
+        const uint8_t* w = MODE == kQmmUp && r >= WR / 2 ? p.w1 : p.w0;
+        const int64_t at = (row0 + rr) * p.rb + (int64_t)pc.sb * F::CB, a16 = at & ~(int64_t)15;
+        const int64_t left = p.wbytes - a16;  // of the tensor
+        const int chunks = first + rr < p.n ? (int)((at + need - a16 + 15) >> 4) : 0;
+        const uint32_t dst = smem_u32(smem) + slot + r * pitch;
+#pragma unroll
+        for (int k = 0; k < (F::PG / 16 + 3) / 4; ++k) {
+          const int j = (lane & 3) + 4 * k;
+          if (j < chunks) qmm_cp_async(dst + 16 * j, w + a16 + 16 * j, (int)min((int64_t)16, left - 16 * j), pol);
+        }
+      }
+      qmm_cp_async_arrive(bar);
     }
   };
   auto fill_records = [&](int stage) {

@@ -249,6 +249,8 @@ class CudaEngine:
         """`t` as the library reads it: contiguous, of this dtype and size, on the engine's device."""
         if t is None:
             return None
+        if t.dtype is dtype and t.device == self.device and t.numel() == numel and t.is_contiguous():
+            return t  # small calls are bound by the host: the usual case first
         if t.dtype != dtype or not t.is_cuda:
             raise NsqError(_lib.ERR_TYPE, f"{what}: a {dtype} CUDA tensor is wanted, not {t.dtype} on {t.device}")
         if self.device.index is not None and t.device.index != self.device.index:
@@ -264,24 +266,27 @@ class CudaEngine:
             raise NsqError(_lib.ERR_SHAPE, f"{what}: the output has to be contiguous")
         return self._tensor(out, shape[0] * shape[1], dtype, what)
 
-    def _call(self, fn, what: str, nbytes: int, workspace: Optional[torch.Tensor], args, sync: bool) -> None:
+    def _call(self, fn, what: str, nbytes, workspace: Optional[torch.Tensor], args, sync: bool) -> None:
         """fn(*args, workspace, bytes, stream) with the engine's device current.  Without a workspace of the
-        caller's, the call takes one from PyTorch's allocator, which keeps it from other streams and graphs."""
+        caller's, the call takes one of nbytes() from PyTorch's allocator, which keeps it from other streams and
+        graphs."""
         if workspace is None:
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            workspace = torch.empty(nbytes() or 16, dtype=torch.uint8, device=self.device)
+        elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
             raise NsqError(_lib.ERR_TYPE, f"{what}: a workspace is contiguous uint8, not {workspace.dtype}")
         else:
             self._tensor(workspace, workspace.numel(), torch.uint8, f"{what}: workspace")
         index = self.device.index
-        if index is None or index == torch.cuda.current_device():
-            rc = fn(*args, workspace.data_ptr(), workspace.numel(), _stream_handle(self.device))
+        current = torch._C._cuda_getDevice()
+        if index is None or index == current:
+            rc = fn(*args, workspace.data_ptr(), workspace.numel(), torch._C._cuda_getCurrentRawStream(current))
         else:
             with torch.cuda.device(index):
                 rc = fn(*args, workspace.data_ptr(), workspace.numel(), _stream_handle(self.device))
         if rc:
             raise NsqError(rc, what)
-        self._sync(sync)
+        if sync:
+            torch.cuda.synchronize(self.device)
 
     def linear_workspace(self, m: int, n: int, k: int) -> torch.Tensor:
         """Workspace of `linear` calls of up to this size; one call at a time may use it."""
@@ -295,21 +300,24 @@ class CudaEngine:
 
         x [m, k], residual and y are f32 (m <= 16) or bf16; bias [n] f32; act one of "none", "silu", "gelu",
         "gelu_tanh", "relu".  `out` may be `residual`."""
-        if x.dtype not in (torch.float32, torch.bfloat16):
-            raise NsqError(_lib.ERR_TYPE, f"linear: activations are f32 or bf16, not {x.dtype}")
+        dtype = x.dtype
+        if dtype is not torch.float32 and dtype is not torch.bfloat16:
+            raise NsqError(_lib.ERR_TYPE, f"linear: activations are f32 or bf16, not {dtype}")
         if ggml_type not in FORMATS or act not in _lib.ACTS:
             raise NsqError(_lib.ERR_TYPE, f"linear: ggml type {ggml_type}, activation {act!r}")
-        if k < 1 or n < 1 or x.numel() % k or k % FORMATS[ggml_type].block_weights:
-            raise NsqError(_lib.ERR_SHAPE, f"linear: {x.numel()} activations, n = {n}, k = {k}")
-        m = x.numel() // k
-        _check_bytes(w, FORMATS[ggml_type].tensor_bytes(n, k), "linear: w")
-        x = self._tensor(x, m * k, x.dtype, "linear: x")
+        f = FORMATS[ggml_type]
+        size = x.numel()
+        if k < 1 or n < 1 or size % k or k % f.block_weights:
+            raise NsqError(_lib.ERR_SHAPE, f"linear: {size} activations, n = {n}, k = {k}")
+        m = size // k
+        _check_bytes(w, n * k // f.block_weights * f.block_bytes, "linear: w")
+        x = self._tensor(x, size, dtype, "linear: x")
         bias = self._tensor(bias, n, torch.float32, "linear: bias")
-        residual = self._tensor(residual, m * n, x.dtype, "linear: residual")
-        y = self._out(out, (m, n), x.dtype, "linear: out")
-        self._call(self.lib.nsq_linear, "nsq_linear", self.lib.nsq_linear_workspace_size(m, k) or 16, workspace,
+        residual = self._tensor(residual, m * n, dtype, "linear: residual")
+        y = self._out(out, (m, n), dtype, "linear: out")
+        self._call(self.lib.nsq_linear, "nsq_linear", lambda: self.lib.nsq_linear_workspace_size(m, k), workspace,
                    (_ptr(w), ggml_type, q6k_layout, _ptr(x), _ptr(bias), _lib.ACTS[act], _ptr(residual), _ptr(y),
-                    _lib.OUT_F32 if x.dtype == torch.float32 else _lib.OUT_BF16, m, n, k), sync)
+                    _lib.OUT_F32 if dtype is torch.float32 else _lib.OUT_BF16, m, n, k), sync)
         return y
 
     def moe_workspace(self, moe: MoeExperts, m: int, top_k: int) -> torch.Tensor:
@@ -332,7 +340,7 @@ class CudaEngine:
         weights = self._tensor(weights, m * top_k, torch.float32, "moe_ffn: weights")
         residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_ffn: residual")
         y = self._out(out, (m, moe.n_embd), torch.float32, "moe_ffn: out")
-        self._call(self.lib.nsq_moe_ffn, "nsq_moe_ffn", self.lib.nsq_moe_workspace_size(moe._ref, m, top_k) or 16,
+        self._call(self.lib.nsq_moe_ffn, "nsq_moe_ffn", lambda: self.lib.nsq_moe_workspace_size(moe._ref, m, top_k),
                    workspace, (moe._ref, _ptr(x), _ptr(ids), _ptr(weights), _ptr(residual), _ptr(y), m, top_k), sync)
         return y
 
@@ -357,7 +365,7 @@ class CudaEngine:
         ids = torch.empty((m, max(top_k, 0)), dtype=torch.int32, device=self.device)
         weights = torch.empty((m, max(top_k, 0)), dtype=torch.float32, device=self.device)
         self._call(self.lib.nsq_moe_layer, "nsq_moe_layer",
-                   self.lib.nsq_moe_workspace_size(moe._ref, m, top_k) or 16, workspace,
+                   lambda: self.lib.nsq_moe_workspace_size(moe._ref, m, top_k), workspace,
                    (moe._ref, _ptr(w_router), _lib.SCORES[score], _ptr(sel_bias), scale, _ptr(x), _ptr(residual),
                     _ptr(y), _ptr(ids), _ptr(weights), m, top_k), sync)
         return y, ids, weights
