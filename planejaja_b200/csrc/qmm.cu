@@ -218,14 +218,16 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
   const int64_t most_units = p.mode == kQmmDown ? groups * p.nsb : p.nsb;
   const int64_t slots = 2 * (int64_t)num_sms < kQmmMaxCtas ? 2 * (int64_t)num_sms : kQmmMaxCtas;
   const int P = p.mode == kQmmLinear ? 0 : p.M * p.top_k;
-  const size_t fixed = kQmmCtl + qmm_lists_bytes(P);
+  const size_t fixed = kQmmCtl + (P ? qmm_lists_bytes(P, p.E, p.TS) : 0);
   const size_t ys = (size_t)kQmmWarps * p.YC * 16 * f.MT * 4;
   const int pitch = p.rb % 16 == 0 ? f.PA : f.PG;
   // Columns of K per CTA (KW), the rest of the 8 warps being row tiles, and
   // whether tasks are divided: the choice with the least time by a simple
   // model.  A CTA's time is its steps x (the bytes of its rows, and a third of
   // those of the records that its row tiles share, which come from L2), and
-  // about three steps to put divided tasks together.
+  // about three steps to put divided tasks together; each doubling of KW costs
+  // 5% for the sums of its columns (1 token, two experts of [14336 x 4096]:
+  // KW = 1 61 us, KW = 8 with an eighth fewer steps 69 us).
   double best = 0;
   size_t smem = 0;
   int64_t grid = 0;
@@ -250,12 +252,13 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
     const int64_t tasks = (p.n + rows - 1) / rows * (p.mode == kQmmUp ? (groups < p.E ? groups : p.E) : 1);
     const int64_t units = p.mode == kQmmDown ? (groups < p.E ? groups : p.E) * p.nsb : p.nsb;
     const int64_t st = (units + KW - 1) / KW;
+    const int columns = KW == 1 ? 0 : KW == 2 ? 1 : KW == 4 ? 2 : 3;
     const double bytes = KW * (16.0 * f.MT * t.RW * pitch + 0.3 * (p.TS < 4 ? p.TS : 0.5 * p.TS) * kQmmRec) / here;
     for (int whole = 1; whole >= 0; --whole) {
       const int only = tune(kTuneQmmSplit, -1);
       if (only >= 0 && whole == (only > 0)) continue;
       const int64_t steps = whole ? (tasks + here - 1) / here * st : (tasks * st + here - 1) / here + 3;
-      const double time = steps * bytes;
+      const double time = steps * bytes * (1.0 + 0.05 * columns);
       if (smem == 0 || time < best) {
         best = time;
         smem = need;
@@ -294,7 +297,7 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
 static int64_t units_of(int64_t K) { return (K + 255) / 256; }
 // Workspace of divided tasks: two parts of up to 8 row tiles per CTA, tickets.
 static size_t parts_bytes(int64_t tokens, int64_t TS) {
-  return (size_t)kQmmMaxCtas * 2 * kQmmWarps * (TS > 4 ? 16 : 32) * tokens * 4;
+  return (size_t)kQmmMaxCtas * 2 * kQmmWarps * (TS > 8 ? 16 : 32) * tokens * 4;
 }
 static bool act_ok(int act) { return act >= NSQ_ACT_NONE && act <= NSQ_ACT_RELU; }
 

@@ -70,8 +70,8 @@ constexpr int kQmmThreads = 32 * kQmmWarps;
 constexpr int kQmmMaxStages = 4;
 constexpr int kQmmCtl = 1024;  // barriers and counters at the start of the shared memory
 constexpr int kQmmMaxTok = 16;  // tokens of a group
-constexpr int kQmmSmemMax = 227 * 1024 - 1024;   // dynamic shared memory of a CTA alone on its SM
-constexpr int kQmmSmemHalf = 113 * 1024 - 1024;  // of one of two CTAs
+constexpr int kQmmSmemMax = 227 * 1024 - 1024;  // dynamic shared memory of a CTA alone on its SM
+constexpr int kQmmSmemHalf = 113 * 1024;         // of one of two CTAs (a CTA takes 1 KB more for itself)
 
 enum QmmOrder : int { kOrdK45 = 0, kOrd32 = 1, kOrdQ6 = 2, kOrdQ6N = 3 };
 
@@ -330,11 +330,13 @@ template <> struct QmmFmt<NSQ_TYPE_Q6_K> { static constexpr int CB = 210, PA = 2
 template <> struct QmmFmt<NSQ_TYPE_Q4_0> { static constexpr int CB = 144, PA = 144, PG = 176, MT = 2; };
 template <> struct QmmFmt<NSQ_TYPE_Q8_0> { static constexpr int CB = 272, PA = 272, PG = 304, MT = 1; };
 
-// Row tiles of a warp for groups of up to TS tokens: one beyond 4 tokens, whose
-// sums take the registers.
+// Row tiles of a warp for groups of up to TS tokens: one beyond 4 tokens for
+// the 32-weight formats and beyond 8 for all.  Two of them share a unit's
+// bookkeeping, some 100 of 470 instructions (16 tokens, 8 experts of
+// [14336 x 4096] Q4_K and Q6_K: 342 -> 313 us).
 template <int TYPE>
 __host__ __device__ constexpr int qmm_tiles(int TS) {
-  return TS > 4 ? 1 : QmmFmt<TYPE>::MT;
+  return TS > 8 || (TS > 4 && Fmt<TYPE>::QK == 32) ? 1 : QmmFmt<TYPE>::MT;
 }
 
 // All shared memory is addressed as an offset from this array, so that loads
@@ -874,17 +876,21 @@ __device__ __forceinline__ void qmm_build_lists(const QmmParams& p, int32_t* mem
   if (lane == 0) *p.ngroups = groups;
 }
 
+// The most groups of P picks: a partly filled one per expert, the others full.
+__host__ __device__ inline int qmm_most_groups(int P, int E, int TS) { return min(P, min(P, E) + P / TS); }
+
 __device__ __forceinline__ QmmLists qmm_load_lists(const QmmParams& p, uint8_t* mem) {
   const int P = p.M * p.top_k;
   QmmLists L;
   L.groups = reinterpret_cast<QmmGroup*>(mem);
-  L.plist = reinterpret_cast<int32_t*>(L.groups + P);
+  const int most = qmm_most_groups(P, p.E, p.TS);
+  L.plist = reinterpret_cast<int32_t*>(L.groups + most);
   L.pwts = reinterpret_cast<float*>(L.plist + P);
   L.ptok = reinterpret_cast<int32_t*>(L.pwts + P);
   // from L2: kQmmDown reads them while the kernel before it still runs
   L.ngroups = __ldcg(p.ngroups);
   for (int q = threadIdx.x; q < P; q += kQmmThreads) {  // entries past the lists' ends are not used
-    reinterpret_cast<int4*>(L.groups)[q] = __ldcg(reinterpret_cast<const int4*>(p.groups) + q);
+    if (q < most) reinterpret_cast<int4*>(L.groups)[q] = __ldcg(reinterpret_cast<const int4*>(p.groups) + q);
     L.plist[q] = __ldcg(p.plist + q);
     L.ptok[q] = __ldcg(p.ptok + q);
     L.pwts[q] = __ldcg(p.pwts + q);
@@ -898,7 +904,9 @@ __host__ __device__ inline uint32_t qmm_slot_bytes(int row_tiles, int pitch, int
   const int tokens = TS <= 2 ? 2 : TS <= 4 ? 4 : TS <= 8 ? 8 : 16;
   return (uint32_t)(row_tiles * 16 * pitch + (tokens * kQmmRecPitch + 127) / 128 * 128);
 }
-inline size_t qmm_lists_bytes(int P) { return (size_t)P * (sizeof(QmmGroup) + 12); }
+inline size_t qmm_lists_bytes(int P, int E, int TS) {
+  return (size_t)qmm_most_groups(P, E, TS) * sizeof(QmmGroup) + (size_t)P * 12;
+}
 
 // Bias, activation and residual (kQmmLinear), or the residual alone
 // (kQmmDown), for one finished sum.
@@ -927,6 +935,18 @@ static __device__ __noinline__ void qmm_store(const QmmParams& p, int col, int r
     static_cast<float*>(p.y)[at] = v;
   } else {
     static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+  }
+}
+
+// One or four (aligned) floats; FRESH: written by another CTA of this kernel.
+template <bool FRESH = false, int V>
+__device__ __forceinline__ void qmm_load(float (&v)[V], const float* from) {
+  if constexpr (V == 4) {
+    const float4* q = reinterpret_cast<const float4*>(from);
+    const float4 f = FRESH ? __ldcg(q) : *q;
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else {
+    v[0] = FRESH ? __ldcg(from) : *from;
   }
 }
 
@@ -1393,24 +1413,55 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       __syncwarp();
     }
     const float* y0 = ys + buf * ys_buf + rw * KW * ys_warp;
-    auto joined = [&](int at) {
-      float v = y0[at];
-      for (int k = 1; k < KW; ++k) v += y0[k * ys_warp + at];
-      return v;
+    // V places [token][row ..] at once: four, or one where that takes the warp
+    // two turns at most (a lane makes its outputs one after the other: a token
+    // alone loses 1.5 us by four; 7 tokens win 5 us by it)
+    const bool wide = OR * cnt > 64;
+    auto joined = [&](auto& v, int at) {
+      constexpr int V = sizeof(v) / 4;
+      qmm_load(v, y0 + at);
+      for (int k = 1; k < KW; ++k) {
+        float f[V];
+        qmm_load(f, y0 + k * ys_warp + at);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += f[e];
+      }
     };
     const int row0 = tile * tile_rows + rw * OR;
-    // writes the outputs of this row tile, sum(at) being the sum of place [token][row]
-    auto emit = [&](auto&& sum) {
-      for (int i = lane; i < OR * cnt; i += 32) {
-        const int col = i / OR, r = i % OR;
+    // writes the outputs of this row tile, sum(v, at) being the sums of V places
+    auto emit_by = [&](auto width, auto&& sum) {
+      constexpr int V = decltype(width)::value;
+      for (int i = lane; i < OR / V * cnt; i += 32) {
+        const int col = i / (OR / V), r = i % (OR / V) * V;
         if (row0 + r >= p.n) continue;
+        float v[V];
+        sum(v, col * WR + r);
         if constexpr (MODE == kQmmUp) {
-          const float gate = sum(col * WR + r), up = sum(col * WR + r + OR);
-          p.h[(int64_t)L.plist[L.groups[task_g].start + col] * p.n + row0 + r] = qmm_act(gate, p.act) * up;
+          float up[V];
+          sum(up, col * WR + r + OR);
+          float* h = p.h + (int64_t)L.plist[L.groups[task_g].start + col] * p.n + row0 + r;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            if (row0 + r + e < p.n) h[e] = qmm_act(v[e], p.act) * up[e];
+          }
         } else {
-          const QmmAdd add = qmm_adds(p, col, row0 + r);
-          qmm_store(p, col, row0 + r, sum(col * WR + r), add);
+          QmmAdd add[V] = {};
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            if (row0 + r + e < p.n) add[e] = qmm_adds(p, col, row0 + r + e);
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            if (row0 + r + e < p.n) qmm_store(p, col, row0 + r + e, v[e], add[e]);
+          }
         }
+      }
+    };
+    auto emit = [&](auto&& sum) {
+      if (wide) {
+        emit_by(std::integral_constant<int, 4>{}, sum);
+      } else {
+        emit_by(std::integral_constant<int, 1>{}, sum);
       }
     };
     // the buffer is free as soon as it was read: the reports below take 1 to 2 us
@@ -1430,15 +1481,33 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         return p.parts + ((int64_t)(cta * 2 + (cta == c_lo ? 1 : 0)) * kQmmWarps + rw) * ys_warp;
       };
       float* mine = part_of((int)blockIdx.x);
-      for (int i = lane; i < WR * cnt; i += 32) mine[i] = joined(i);
+      for (int i = 4 * lane; i < WR * cnt; i += 128) {
+        float v[4];
+        joined(v, i);
+        *reinterpret_cast<float4*>(mine + i) = make_float4(v[0], v[1], v[2], v[3]);
+      }
       release_ys();
       int last = 0;
       if (lane == 0) last = qmm_add_acq_rel(p.tickets + c_lo * kQmmWarps + rw, n_steps) + n_steps == st;
       if (__shfl_sync(0xffffffffu, last, 0)) {
-        emit([&](int at) {
-          float v = 0.0f;
-          for (int q = c_lo; q <= c_hi; ++q) v += __ldcg(part_of(q) + at);
-          return v;
+        // eight parts' loads at a time: one after the other their latencies
+        // were 50 us of 32 tokens' and 64 experts' 207
+        emit([&](auto& v, int at) {
+          constexpr int V = sizeof(v) / 4;
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] = 0.0f;
+          for (int q = c_lo; q <= c_hi; q += 8) {
+            float f[8][V] = {};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              if (q + k <= c_hi) qmm_load<true>(f[k], part_of(q + k) + at);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) v[e] += f[k][e];
+            }
+          }
         });
         if constexpr (MODE == kQmmUp) report_rows(task_g, row0, OR, 1);
       }

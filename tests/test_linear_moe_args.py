@@ -47,9 +47,9 @@ def test_linear_refusals(lib, want, kw):
 
 def test_linear_workspace_size(lib):
     # one record of 880 bytes per token and 256 of K (rounded up to 256), 8 tickets
-    # and two parts of 8 row tiles of 32 (16 beyond 4 tokens) rows for 320 CTAs
+    # and two parts of 8 row tiles of 32 (16 beyond 8 tokens) rows for 320 CTAs
     def size(m, k):
-        return -(-m * -(-k // 256) * 880 // 256) * 256 + 320 * 8 * 4 + 320 * 2 * 8 * (16 if m > 4 else 32) * m * 4
+        return -(-m * -(-k // 256) * 880 // 256) * 256 + 320 * 8 * 4 + 320 * 2 * 8 * (16 if m > 8 else 32) * m * 4
     for m, k in ((1, 256), (4, 896), (5, 896), (16, 14336)):
         assert lib.nsq_linear_workspace_size(m, k) == size(m, k)
     assert lib.nsq_linear_workspace_size(17, 256) == 0
