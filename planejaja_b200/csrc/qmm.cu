@@ -21,6 +21,7 @@ int run_gemm_epi(const uint8_t* w, int type, int layout, const void* x, const fl
 constexpr int kPrepThreads = 32 * kQmmWarps;
 constexpr int kRouteTok = 8;  // tokens of one CTA's logits
 constexpr int kQmmMaxCtas = 320;  // of a product: two per SM
+constexpr int kOwnRecords = 8;   // records that a CTA of nsq_linear's product makes itself
 constexpr size_t kTicketBytes = (size_t)kQmmMaxCtas * kQmmWarps * 4;
 
 // Activation records of rows x nsb units, one warp each.
@@ -213,7 +214,11 @@ static bool encode_rows(CUtensorMap* map, const uint8_t* w, int64_t rows, int64_
 }
 
 // Plans and launches one product.  groups: the most groups there can be.
-static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream_t st, int num_sms) {
+struct QmmPlan {
+  size_t smem;
+  int64_t grid;
+};
+static int plan_qmm(QmmParams& p, int type, int64_t groups, int num_sms, QmmPlan* plan) {
   const QmmShape f = qmm_shape(type, p.TS);
   const int64_t most_units = p.mode == kQmmDown ? groups * p.nsb : p.nsb;
   const int64_t slots = 2 * (int64_t)num_sms < kQmmMaxCtas ? 2 * (int64_t)num_sms : kQmmMaxCtas;
@@ -274,6 +279,14 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
     }
   }
   if (smem == 0) return NSQ_ERR_SHAPE;
+  *plan = QmmPlan{smem, grid};
+  return NSQ_OK;
+}
+
+static int launch_qmm(QmmParams& p, const QmmPlan& plan, int type, int layout, cudaStream_t st) {
+  const QmmShape f = qmm_shape(type, p.TS);
+  const size_t smem = plan.smem;
+  const int64_t grid = plan.grid;
   // TMA boxes where every row starts 16-byte aligned (experts and tensors then do too)
   alignas(64) CUtensorMap maps[2] = {};
   const int64_t rows = p.wbytes / p.rb;
@@ -292,6 +305,12 @@ static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream
     case NSQ_TYPE_Q8_0: return launch_qmm_q80(layout, p, maps, (int)grid, smem, st);
     default: return NSQ_ERR_TYPE;
   }
+}
+
+static int run_qmm(QmmParams p, int type, int layout, int64_t groups, cudaStream_t st, int num_sms) {
+  QmmPlan plan{};
+  const int rc = plan_qmm(p, type, groups, num_sms, &plan);
+  return rc ? rc : launch_qmm(p, plan, type, layout, st);
 }
 
 static int64_t units_of(int64_t K) { return (K + 255) / 256; }
@@ -470,10 +489,6 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   QmmParams p{};
   p.tickets = reinterpret_cast<int32_t*>(recs + linear_records(M, K));
   p.parts = reinterpret_cast<float*>(recs + linear_records(M, K) + kTicketBytes);
-  rc = dtype == NSQ_OUT_F32
-           ? launch_prep(static_cast<const float*>(x), M, K, order, recs, p.tickets, st)
-           : launch_prep(static_cast<const __nv_bfloat16*>(x), M, K, order, recs, p.tickets, st);
-  if (rc) return rc;
   p.mode = kQmmLinear;
   p.M = p.TS = p.YC = (int)M;
   p.top_k = 1;
@@ -490,7 +505,25 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   p.bias = bias;
   p.residual = residual;
   p.y = y;
-  return run_qmm(p, ggml_type, q6k_layout, 1, st, num_sms);
+  QmmPlan plan{};
+  if ((rc = plan_qmm(p, ggml_type, 1, num_sms, &plan))) return rc;
+  // One record per warp at most: every CTA makes them itself, which takes less
+  // than a kernel before it (1 token, Q8_0 1152 x 896: 5.5 against 6.7 us, and
+  // 2.4 us less on the host; two per warp, Q4_K 4096 x 4096: 8.1 against 7.8).
+  // Divided tasks need that kernel for their tickets.
+  const size_t own = (size_t)p.nsb * qmm_recs_bytes(p.TS);
+  if (p.whole && M * p.nsb <= kOwnRecords &&
+      plan.smem + own <= (size_t)(plan.smem <= (size_t)kQmmSmemHalf ? kQmmSmemHalf : kQmmSmemMax)) {
+    p.x = x;
+    p.order = order;
+    plan.smem += own;
+  } else {
+    rc = dtype == NSQ_OUT_F32
+             ? launch_prep(static_cast<const float*>(x), M, K, order, recs, p.tickets, st)
+             : launch_prep(static_cast<const __nv_bfloat16*>(x), M, K, order, recs, p.tickets, st);
+    if (rc) return rc;
+  }
+  return launch_qmm(p, plan, ggml_type, q6k_layout, st);
 }
 
 size_t nsq_moe_workspace_size(const nsq_moe* moe, int64_t M, int64_t top_k) {

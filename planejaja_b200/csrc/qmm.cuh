@@ -223,6 +223,8 @@ struct QmmParams {
   int64_t wbytes;            // bytes of all experts' rows
   const uint8_t* recs;       // activation records [row][nsb]
   // kQmmLinear
+  const void* x;             // [M][K]: every CTA makes all records itself, there are few (else NULL: see recs)
+  int order;                 // of their values
   const float* bias;
   // kQmmLinear, kQmmDown
   const void* residual;
@@ -899,10 +901,13 @@ __device__ __forceinline__ QmmLists qmm_load_lists(const QmmParams& p, uint8_t* 
 }
 
 // Bytes of a slot: RW tiles of rows at this pitch, then TS records.
-__host__ __device__ inline uint32_t qmm_slot_bytes(int row_tiles, int pitch, int TS) {
+__host__ __device__ inline uint32_t qmm_recs_bytes(int TS) {
   // whole n-tiles of tokens: absent ones are read too
   const int tokens = TS <= 2 ? 2 : TS <= 4 ? 4 : TS <= 8 ? 8 : 16;
-  return (uint32_t)(row_tiles * 16 * pitch + (tokens * kQmmRecPitch + 127) / 128 * 128);
+  return (uint32_t)((tokens * kQmmRecPitch + 127) / 128 * 128);
+}
+__host__ __device__ inline uint32_t qmm_slot_bytes(int row_tiles, int pitch, int TS) {
+  return (uint32_t)(row_tiles * 16 * pitch) + qmm_recs_bytes(TS);
 }
 inline size_t qmm_lists_bytes(int P, int E, int TS) {
   return (size_t)qmm_most_groups(P, E, TS) * sizeof(QmmGroup) + (size_t)P * 12;
@@ -992,6 +997,9 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   // partial sums [buffer][warp][YC][WR]
   float* const ys = reinterpret_cast<float*>(smem + kQmmCtl + ring_bytes);
   const int ys_warp = YC * WR, ys_buf = kQmmWarps * ys_warp;
+  // records of all units, where the CTA makes them itself
+  const bool own_recs = MODE == kQmmLinear && p.x != nullptr;
+  const uint32_t own_at = kQmmCtl + ring_bytes + p.PB * ys_buf * 4;
   const int tile_rows = OR * RW;
   const int tiles = (int)((p.n + tile_rows - 1) / tile_rows);
 
@@ -1013,7 +1021,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
     for (int i = 0; i < KW; ++i) {
       for (int k = 0; k < S; ++k) {
         // rows of every warp (one arrival per warp, or per lane), records (one warp: with the rows)
-        mbar_init(&full[i][k], (p.rows_aligned ? RW : 32 * RW) + (RW > 1));
+        mbar_init(&full[i][k], (p.rows_aligned ? RW : 32 * RW) + (RW > 1 && !own_recs));
         mbar_init(&used[i][k], RW);
       }
     }
@@ -1178,7 +1186,25 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
   // about 500 cycles (always the same one: the others wait 750 cycles a unit).
   int rec_unit = kw;  // units of the column whose records were refilled, from kw on
   auto my_turn = [&] { return rw == (rec_unit++ & (RW - 1)); };
-  if constexpr (MODE != kQmmUp) {
+  if (own_recs) {
+    qmm_dep_wait();
+    qmm_dep_launch();
+    for (int k = 0; k < S && pc.left > 0; ++k) {
+      fill_rows(k, 0);
+      advance();
+    }
+    for (int j = warp; j < p.M * p.nsb; j += kQmmWarps) {
+      const int row = j / p.nsb, sb = j - row * p.nsb, valid = (int)min((int64_t)256, p.K - 256 * sb);
+      uint8_t* rec = smem + own_at + sb * qmm_recs_bytes(TS) + row * kQmmRecPitch;
+      const int64_t at = row * p.K + 256 * sb;
+      if (p.dtype == NSQ_OUT_F32) {
+        qmm_make_record(static_cast<const float*>(p.x) + at, valid, p.order, rec, lane);
+      } else {
+        qmm_make_record(static_cast<const __nv_bfloat16*>(p.x) + at, valid, p.order, rec, lane);
+      }
+    }
+    __syncthreads();
+  } else if constexpr (MODE != kQmmUp) {
     // the weights do not depend on the kernel before; records, residual and
     // outputs do
     const QmmCursor start = pc;
@@ -1300,7 +1326,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
         __syncwarp();
         const int count = MODE == kQmmDown ? count_of(c) : task_count;
         const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes;
-        const uint32_t recs = slot + recs_at;
+        const uint32_t recs = own_recs ? own_at + c.sb * qmm_recs_bytes(TS) : slot + recs_at;
         const int nv = min(8, p.nblk - 8 * c.sb);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -1371,9 +1397,12 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
           }
         }
         __syncwarp();
-        if (RW > 1 && lane == 0) mbar_arrive(&used[kw][stage]);
+        if (RW > 1 && !own_recs && lane == 0) mbar_arrive(&used[kw][stage]);
         if (pc.left > 0) {
-          if (RW == 1) {
+          if (own_recs) {
+            fill_rows(stage, 0);
+            advance();
+          } else if (RW == 1) {
             fill_rows(stage, count_of(pc) * kQmmRec);
             fill_records(stage);
             advance();

@@ -259,9 +259,9 @@ class CudaEngine:
             raise NsqError(_lib.ERR_SHAPE, f"{what}: {t.numel()} elements, not {numel}")
         return t if t.is_contiguous() else t.contiguous()
 
-    def _out(self, out: Optional[torch.Tensor], shape, dtype: torch.dtype, what: str) -> torch.Tensor:
+    def _out(self, out: Optional[torch.Tensor], shape, dtype: torch.dtype, what: str, like: torch.Tensor) -> torch.Tensor:
         if out is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return like.new_empty(shape)
         if not out.is_contiguous():
             raise NsqError(_lib.ERR_SHAPE, f"{what}: the output has to be contiguous")
         return self._tensor(out, shape[0] * shape[1], dtype, what)
@@ -314,7 +314,7 @@ class CudaEngine:
         x = self._tensor(x, size, dtype, "linear: x")
         bias = self._tensor(bias, n, torch.float32, "linear: bias")
         residual = self._tensor(residual, m * n, dtype, "linear: residual")
-        y = self._out(out, (m, n), dtype, "linear: out")
+        y = self._out(out, (m, n), dtype, "linear: out", x)
         self._call(self.lib.nsq_linear, "nsq_linear", lambda: self.lib.nsq_linear_workspace_size(m, k), workspace,
                    (_ptr(w), ggml_type, q6k_layout, _ptr(x), _ptr(bias), _lib.ACTS[act], _ptr(residual), _ptr(y),
                     _lib.OUT_F32 if dtype is torch.float32 else _lib.OUT_BF16, m, n, k), sync)
@@ -339,7 +339,7 @@ class CudaEngine:
         ids = self._tensor(ids, m * top_k, torch.int32, "moe_ffn: ids")
         weights = self._tensor(weights, m * top_k, torch.float32, "moe_ffn: weights")
         residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_ffn: residual")
-        y = self._out(out, (m, moe.n_embd), torch.float32, "moe_ffn: out")
+        y = self._out(out, (m, moe.n_embd), torch.float32, "moe_ffn: out", x)
         self._call(self.lib.nsq_moe_ffn, "nsq_moe_ffn", lambda: self.lib.nsq_moe_workspace_size(moe._ref, m, top_k),
                    workspace, (moe._ref, _ptr(x), _ptr(ids), _ptr(weights), _ptr(residual), _ptr(y), m, top_k), sync)
         return y
@@ -361,7 +361,7 @@ class CudaEngine:
         w_router = self._tensor(w_router, moe.n_expert * moe.n_embd, torch.float32, "moe_layer: w_router")
         sel_bias = self._tensor(sel_bias, moe.n_expert, torch.float32, "moe_layer: sel_bias")
         residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_layer: residual")
-        y = self._out(out, (m, moe.n_embd), torch.float32, "moe_layer: out")
+        y = self._out(out, (m, moe.n_embd), torch.float32, "moe_layer: out", x)
         ids = torch.empty((m, max(top_k, 0)), dtype=torch.int32, device=self.device)
         weights = torch.empty((m, max(top_k, 0)), dtype=torch.float32, device=self.device)
         self._call(self.lib.nsq_moe_layer, "nsq_moe_layer",
