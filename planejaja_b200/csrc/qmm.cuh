@@ -1302,6 +1302,17 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       for (int i = lane; i < ys_warp; i += 32) my_ys[i] = 0.0f;
       __syncwarp();
     }
+    // kQmmDown: the sums of a group so far go to its tokens' places, weighted
+    // (once per group: once per unit took 40 of its 370 instructions)
+    [[maybe_unused]] int acc_g = -1;
+    auto spread = [&](int g) {
+      if (g < 0) return;
+      const int count = L.groups[g].count, start = L.groups[g].start;
+      each_sum(count, [&](int tk, int r, float v) {
+        if (tk < count) my_ys[L.ptok[start + tk] * WR + r] += L.pwts[start + tk] * v;
+      });
+      __syncwarp();
+    };
     [[maybe_unused]] int task_count = 0;
     if constexpr (MODE != kQmmDown) task_count = count_of(c);
     for (int i = 0; i < n_steps && ok; ++i) {
@@ -1324,6 +1335,12 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
           break;
         }
         __syncwarp();
+        if constexpr (MODE == kQmmDown) {
+          if (c.g != acc_g) {
+            spread(acc_g);
+            acc_g = c.g;
+          }
+        }
         const int count = MODE == kQmmDown ? count_of(c) : task_count;
         const uint32_t slot = kQmmCtl + (stage * KW + kw) * slot_bytes;
         const uint32_t recs = own_recs ? own_at + c.sb * qmm_recs_bytes(TS) : slot + recs_at;
@@ -1357,24 +1374,8 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
               const int tk = first + (limbs ? 2 * lc + q : 2 * q + (lc >> 1));
               float s = tk < count ? qmm_lds<float>(recs + tk * kQmmRecPitch + kQmmRecS) : 0.0f;
               if (!limbs && (lc & 1)) s *= 65536.0f;  // limb 2 of the token
-              float y0 = s * v[q][0], y1 = s * v[q][1];
-              if constexpr (MODE == kQmmDown) {
-                if constexpr (!limbs) {  // the pair of lanes takes a row half each
-                  y0 += __shfl_xor_sync(0xffffffffu, y0, 1);
-                  y1 += __shfl_xor_sync(0xffffffffu, y1, 1);
-                }
-                if (tk < count) {
-                  const int pick = L.groups[c.g].start + tk;
-                  const float w = L.pwts[pick];
-                  float* to = my_ys + L.ptok[pick] * WR + 16 * t + lr;
-                  if constexpr (limbs) {
-                    to[0] += w * y0;
-                    to[8] += w * y1;
-                  } else {
-                    to[8 * (lc & 1)] += w * (lc & 1 ? y1 : y0);
-                  }
-                }
-              } else if (NQ <= 2 || first == 0) {
+              const float y0 = s * v[q][0], y1 = s * v[q][1];
+              if (NQ <= 2 || first == 0) {
                 tot[t][q][0] += y0;
                 tot[t][q][1] += y1;
               } else {
@@ -1419,6 +1420,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       next_step(c);
     }
     if (!ok) break;
+    if constexpr (MODE == kQmmDown) spread(acc_g);
     c.left -= n_steps;
     c.s = s_first + n_steps;  // (columns without a unit in the last step count it too)
     const bool ends = c.s == st;
