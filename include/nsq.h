@@ -307,12 +307,14 @@ int nsq_gemv_multi_xchg(const nsq_xsegment *segs, int nseg, const float *x, int6
  *   dtype     element type of x, residual and y: NSQ_OUT_F32 or NSQ_OUT_BF16
  *   bias      N f32, or NULL;  act: NSQ_ACT_*
  *   residual  [M x N] of dtype, or NULL; may be y itself
+ * y overlaps neither a part of residual nor bias (NSQ_ERR_SHAPE).
  * M = 1..16: 24-bit activations per 256 of K, exact integer products, f32
  * sums: f32 results are off by about 3e-7 of their norm, bf16 ones rounded
  * once.  A token with an infinity or a NaN gives NaN throughout.  K is a
  * multiple of the type's block.  `workspace` (nsq_linear_workspace_size(M, K)
- * bytes, 16-byte aligned) is used by one call at a time.
- * M > 16: bf16 only, K % 256 == 0, x and y 16-byte aligned; the product of
+ * bytes, 16-byte aligned) is used by one call at a time and holds none of the
+ * tensors.  y may lie on x.
+ * M > 16: bf16 only, K % 256 == 0, x and y 16-byte aligned and apart; the product of
  * nsq_gemm_bf16 (weights rounded to bf16, f32 sums), the epilogue in f32
  * before the one rounding of the result.  No workspace. */
 #define NSQ_ACT_NONE 0
@@ -332,7 +334,8 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
  *   h_j  = act(x . W_gate[e_j]^T) * (x . W_up[e_j]^T)        [n_ff]
  *   y[m] = residual[m] + sum_j weight[m, j] * (h_j . W_down[e_j]^T)
  * over the top_k picks e_j = ids[m, j] of token m.  All tensors but the
- * experts are f32; residual may be NULL or y itself.  Accuracy as
+ * experts are f32; residual may be NULL or y itself, y may lie on x; no other
+ * tensor and nothing in the workspace overlaps (NSQ_ERR_SHAPE).  Accuracy as
  * nsq_linear's f32.  A reference routing shader exists but is never built
  * (crates/nodestor-vulkan/build.rs:24, moe_routing). */
 typedef struct nsq_moe {

@@ -318,6 +318,11 @@ static int64_t units_of(int64_t K) { return (K + 255) / 256; }
 static size_t parts_bytes(int64_t tokens, int64_t TS) {
   return (size_t)kQmmMaxCtas * 2 * kQmmWarps * (TS > 8 ? 16 : 32) * tokens * 4;
 }
+// Whether two ranges of memory share a byte (NULL shares none).
+static bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x && y && x < y + bn && y < x + an;
+}
 static bool act_ok(int act) { return act >= NSQ_ACT_NONE && act <= NSQ_ACT_RELU; }
 
 // Workspace of a mixture-of-experts call, in this order.
@@ -382,6 +387,13 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   const MoeSpace s = moe_space(E, D, F, M, top_k);
   if (!workspace || workspace_bytes < s.total) return NSQ_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NSQ_ERR_ALIGN;
+  // (x is read by the first kernel alone, y written by the last)
+  const size_t xb = (size_t)(M * D) * 4, pb = (size_t)(M * top_k) * 4;
+  if ((residual != y && overlap(residual, xb, y, xb)) || overlap(ids, pb, weights, pb) || overlap(ids, pb, y, xb) ||
+      overlap(weights, pb, y, xb) || overlap(workspace, s.total, x, xb) || overlap(workspace, s.total, y, xb) ||
+      overlap(workspace, s.total, residual, xb) || overlap(workspace, s.total, ids, pb) ||
+      overlap(workspace, s.total, weights, pb))
+    return NSQ_ERR_SHAPE;
   int num_sms = 0;
   if ((rc = device_check(&num_sms))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -472,8 +484,12 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & mask)
     return NSQ_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(bias) & 3) return NSQ_ERR_ALIGN;
+  const size_t es = dtype == NSQ_OUT_F32 ? 4 : 2, xb = (size_t)(M * K) * es, yb = (size_t)(M * N) * es;
+  const bool y_on_x = overlap(x, xb, y, yb);
+  const bool y_on_others = (residual != y && overlap(residual, yb, y, yb)) || overlap(bias, (size_t)N * 4, y, yb);
   if (prompt) {
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) return NSQ_ERR_ALIGN;
+    if (y_on_x || y_on_others) return NSQ_ERR_SHAPE;
     int sms = 0;
     if ((rc = device_check(&sms))) return rc;
     return run_gemm_epi(static_cast<const uint8_t*>(w), ggml_type, q6k_layout, x, bias, act, residual, y, M, N, K,
@@ -481,6 +497,10 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   }
   if (!workspace || workspace_bytes < nsq_linear_workspace_size(M, K)) return NSQ_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NSQ_ERR_ALIGN;
+  const size_t wb = nsq_linear_workspace_size(M, K);
+  if (y_on_others || overlap(workspace, wb, x, xb) || overlap(workspace, wb, y, yb) ||
+      overlap(workspace, wb, residual, yb) || overlap(workspace, wb, bias, (size_t)N * 4))
+    return NSQ_ERR_SHAPE;
   int num_sms = 0;
   if ((rc = device_check(&num_sms))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -510,9 +530,10 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   // One record per warp at most: every CTA makes them itself, which takes less
   // than a kernel before it (1 token, Q8_0 1152 x 896: 5.5 against 6.7 us, and
   // 2.4 us less on the host; two per warp, Q4_K 4096 x 4096: 8.1 against 7.8).
-  // Divided tasks need that kernel for their tickets.
+  // Divided tasks need that kernel for their tickets, and an output over x
+  // needs every record made before it.
   const size_t own = (size_t)p.nsb * qmm_recs_bytes(p.TS);
-  if (p.whole && M * p.nsb <= kOwnRecords &&
+  if (p.whole && !y_on_x && M * p.nsb <= kOwnRecords &&
       plan.smem + own <= (size_t)(plan.smem <= (size_t)kQmmSmemHalf ? kQmmSmemHalf : kQmmSmemMax)) {
     p.x = x;
     p.order = order;

@@ -8,9 +8,9 @@
 // 256 of K); X is three signed bytes ("limbs", X = sum 256^l X_l, each
 // -128..127).  The formats' integers meet the limbs in mma.sync m16n8k32 / k16
 // (u8 x s8, exact s32 sums): 16 weight rows as A and eight columns as B,
-// which are two tokens of four limbs (the fourth is zero) or, from five tokens
-// on, one limb of eight tokens.  The integer scale of a group multiplies its
-// sum in s32 too, so the first rounding comes after 256 weights:
+// which are two tokens of four limbs (the fourth a copy, not used) or, from
+// five tokens on, one limb of eight tokens.  The integer scale of a group
+// multiplies its sum in s32 too, so the first rounding comes after 256 weights:
 //   Q4_K, Q5_K  sum sc_j (sum q X_l): |sum| < 2^29;  d times it in f32.  The
 //               mins enter through the limb sums T of 16 activations (at most
 //               2048, exact in fp16):  - dmin * sum m T  by one fp16 MMA
@@ -25,20 +25,26 @@
 // fp16) needs a multiply or subtract per pair of weights beside the mask, 290
 // cycles a tile of 16 x 256; this one masks four weights at a time, about 170.
 //
-// What bounds it: HBM for the weights as long as a tile's cycles stay under
-// its bytes' time (Q4_K: 390 cycles of a scheduler at 6.5 TB/s).
+// What bounds it.  Up to 4 tokens HBM and the start and end of a kernel: two
+// experts' [14336 x 4096] Q4_K in 61 us are 3.2 TB/s with 10 us of routing and
+// starts; Q5_K [28672 x 8192], 3 tokens, 47 us = 3.4 TB/s, its fifth bits' logic.
+// From five tokens on instructions: 400 a tile of 16 x 256 at 0.6 a cycle and
+// scheduler, 16 tokens over 8 experts 301 us = 3.0 TB/s.
 //
 // Layout.  A CTA is 8 warps = RW row tiles of 16 MT weight rows x KW columns.
 // A task is a tile of 16 MT RW rows; its units of 256 weights of K are dealt
 // to the columns in turn.  A column has its own ring of shared-memory slots
 // (the weight bytes of its RW tiles and the activation records of the unit)
 // behind full mbarriers.  Every warp refills its own rows as soon as it has
-// used them, by TMA: one 2-D box where rows start 16-byte aligned, else one
-// bulk copy per row; one warp of the column refills the records.  (A producer
-// warp would cost a ninth warp's registers, 96 instead of 128 a thread, and
-// ties the columns together.)  The partial sums of the KW columns meet in
-// shared memory, those of a K split over a cluster through distributed shared
-// memory, always in the same order.  Every wait is bounded.
+// used them: one 2-D TMA box where rows start 16-byte aligned, else 16-byte
+// asynchronous copies; the column's warps refill the records in turn.  (A
+// producer warp would cost a ninth warp's registers, 96 instead of 128 a
+// thread, and ties the columns together.)  The partial sums of the KW columns
+// meet in shared memory.  The CTAs share all tasks' steps evenly (a CTA may
+// hold parts of two tasks; with a task's steps never divided 16 tokens over 8
+// experts take 575 us instead of 301), and a divided task's parts meet in the
+// workspace, where the last to arrive adds them up in the CTAs' order.  No CTA
+// waits for another; every other wait is bounded.
 #pragma once
 
 #include <cuda.h>
@@ -323,8 +329,8 @@ static __device__ __noinline__ float qmm_act(float v, int act) {
 // pitches of a slot's rows: with 16-byte aligned rows (PA, the TMA box) and
 // without (PG: the copies then carry up to 14 bytes before and 15 after the
 // unit).  The pitches put the reads of 8 rows x 4 lanes on distinct banks.
-// Two row tiles share their B operands and bookkeeping; the wider formats
-// have one, for the depth of the ring.
+// Two row tiles share a unit's bookkeeping; the wider formats have one, for
+// the depth of the ring.
 template <int TYPE> struct QmmFmt;
 template <> struct QmmFmt<NSQ_TYPE_Q4_K> { static constexpr int CB = 144, PA = 160, PG = 160, MT = 2; };
 template <> struct QmmFmt<NSQ_TYPE_Q5_K> { static constexpr int CB = 176, PA = 176, PG = 176, MT = 2; };

@@ -1,17 +1,21 @@
-"""GPU tests of nsq_linear (M <= 16) and the mixture-of-experts layer against
-a plain implementation in 64 bits over the oracle's dequantised weights.
+"""GPU tests of nsq_linear and the mixture-of-experts layer against a plain
+implementation in 64 bits over the oracle's dequantised weights.
 
-Tolerances.  An activation is kept as two fp16 numbers (error <= 2^-22 of it),
-so are the sums T that carry the formats' offsets (q - 8, - dmin m ...); the
-products are exact and the sums f32.  With A = sum_k |x_k| (|w_k| + 2 o_k),
-o the offset part of a weight (the weight whose quant bits are 0), a result
-has passed through at most 17 MMA accumulations, nsb units and 16 joins, each
-off by at most 2^-23 of a partial sum <= A:
+Tolerances (up to 16 tokens).  An activation is an integer below 2^23 times
+one scale per 256 of K: off by at most 2^-24 of the largest of its 256; the
+formats' integers are exact, sums are s32 and then f32.  With A = sum_k |x_k|
+(|w_k| + 2 o_k), o the offset part of a weight (the weight whose quant bits
+are 0), the f32 part passes at most 17 additions within a unit, nsb units and
+16 joins, each off by at most 2^-23 of a partial sum <= A:
   |y - r| <= (2 * 2^-22 + 2^-23 (17 + nsb + 16)) A                (element)
-The roundings are independent, so the 2-norm error is far smaller: with
-parts up to 3 times the result, 3 (2^-22 + 2^-23 sqrt(33 + nsb) / 2) <= 3e-6
-relative for nsb <= 56; 5e-6 is asked of one product, 1e-5 of the two of an
-expert.  A bf16 result adds half a step, 2^-9 of the value at most 2^-8.
+The activations' roundings are independent.  Here (normal values, one in a
+hundred 50 times as large: largest <= 200, mean size of all >= 1) they add up
+to a deviation of 2^-24 * 200 sqrt(256 / 3) = 2^-24 * 1850 of a weight per
+unit, a ninth of the bound's 2^-24 * (8 + 66) * 246 of a weight.  As a norm
+that is 2^-24 * 1850 / (16 * 5) = 1.4e-6 of the result, and the f32 part
+2^-23 sqrt(33 + nsb) / 2 <= 6e-7 of parts up to 3 times the result: 5e-6 is
+asked of one product, 1e-5 of the two of an expert.  A bf16 result adds half
+a step, at most 2^-8 of the value.
 """
 import numpy as np
 import pytest
@@ -202,6 +206,33 @@ def test_linear_repeats_bit_for_bit_and_other_streams(eng):
     assert all(torch.equal(v, y) for v in z)
 
 
+@pytest.mark.parametrize("m,n,k,t", [(1, 896, 896, Q8_0), (3, 512, 512, Q4_K), (16, 4096, 4096, Q4_K), (2, 2048, 2048, Q6_K)])
+def test_linear_output_over_its_input(eng, m, n, k, t):
+    w = eng.upload(blocks(n, k, t, 4))
+    x = torch.randn(m, k, device="cuda")
+    want = eng.linear(x, w, t, n, k, act="silu", residual=x)
+    got = eng.linear(x, w, t, n, k, act="silu", residual=x, out=x)
+    assert got.data_ptr() == x.data_ptr() and torch.equal(got, want)
+
+
+def test_linear_calls_side_by_side(eng):
+    """Four streams, their kernels on the GPU at once: small, divided and whole tasks, prompts; each its own workspace."""
+    calls = []
+    for i, (m, n, k, t) in enumerate(((1, 1152, 896, Q8_0), (1, 4096, 14336, Q6_K), (16, 2048, 4096, Q4_K), (40, 512, 1024, Q5_K))):
+        w = eng.upload(blocks(n, k, t, i))
+        x = torch.randn(m, k, device="cuda")
+        x = x.bfloat16() if m > 16 else x
+        calls.append((torch.cuda.Stream(), x, w, t, n, k, eng.linear(x, w, t, n, k, act="gelu")))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, x, w, t, n, k, want in calls:
+            with torch.cuda.stream(s):
+                got.append((eng.linear(x, w, t, n, k, act="gelu", sync=False), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y, want in got)
+
+
 def test_linear_captured_with_one_workspace(eng):
     """Two graphs that share a workspace, replayed in turn over changing inputs."""
     n, k = 512, 1024
@@ -377,6 +408,7 @@ def test_moe_ffn_every_format(eng, oracle, t, layout, m):
     (512, 6, 8, 256, 256, Q4_0, Q6_K, "silu"),    # the most experts
     (7, 33, 1, 1024, 1376, Q5_K, Q8_0, "gelu_tanh"),
     (3, 2, 2, 2048, 3840, Q6_K, Q5_K, "none"),
+    (512, 64, 16, 256, 256, Q5_K, Q4_K, "silu"),  # the most of everything
 ])
 def test_moe_ffn_sizes(eng, oracle, e, m, k, d, f, t_in, t_down, act):
     ly = Layer(eng, oracle, e, d, f, t_in, t_down, act=act)
@@ -522,6 +554,24 @@ def test_moe_layer_captured_and_on_another_stream(eng, oracle):
         z = eng.moe_layer(ly.moe, wr, x, 2, residual=res, sync=False)[0]
     torch.cuda.synchronize()
     assert torch.equal(z, y)
+
+
+def test_moe_calls_side_by_side(eng, oracle):
+    """A layer on two streams at once, each call with a workspace of its own."""
+    ly = Layer(eng, oracle, 16, 512, 1024, Q4_K, Q4_K)
+    wr = torch.randn(16, 512, device="cuda")
+    xs = [torch.randn(m, 512, device="cuda") for m in (1, 24)]
+    want = [eng.moe_layer(ly.moe, wr, x, 4) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, eng.moe_layer(ly.moe, wr, xs[i], 4, sync=False)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
 
 
 def test_a_decoder_block_of_these_operators(eng, oracle):

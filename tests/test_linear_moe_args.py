@@ -45,6 +45,26 @@ def test_linear_refusals(lib, want, kw):
     assert linear(lib, **kw) == want
 
 
+@pytest.mark.parametrize("kw", [
+    dict(res=4 * AL - 4), dict(bias=4 * AL + 60), dict(ws=4 * AL), dict(x=8 * AL, ws=8 * AL), dict(ws=2 * AL, res=2 * AL),
+    dict(m=17, dtype=1, x=4 * AL), dict(m=17, dtype=1, x=4 * AL + 512), dict(m=17, dtype=1, res=4 * AL + 2),
+])
+def test_linear_overlaps_are_refused(lib, kw):
+    """Ranges that the product reads while it writes y: y [16] at 4 AL, everything else apart."""
+    a = dict(x=AL, bias=2 * AL, res=None, y=4 * AL, ws=16 * AL, wsb=lib.nsq_linear_workspace_size(1, 256))
+    a.update(kw)
+    assert linear(lib, **a) == _lib.ERR_SHAPE
+
+
+def test_linear_allowed_overlaps_pass_the_checks(lib):
+    apart = dict(x=AL, bias=2 * AL, res=None, y=4 * AL, ws=16 * AL, wsb=lib.nsq_linear_workspace_size(1, 256))
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not the device's")
+    for kw in (dict(), dict(res=4 * AL), dict(x=4 * AL), dict(res=4 * AL + 64), dict(m=17, dtype=1, res=4 * AL)):
+        assert linear(lib, **dict(apart, **kw)) in (_lib.ERR_CUDA, _lib.ERR_DEVICE), kw
+
+
 def test_linear_workspace_size(lib):
     # one record of 880 bytes per token and 256 of K (rounded up to 256), 8 tickets
     # and two parts of 8 row tiles of 32 (16 beyond 8 tokens) rows for 320 CTAs
@@ -86,6 +106,14 @@ def ffn(lib, mo, **kw):
 ])
 def test_moe_refusals(lib, want, mo, kw):
     assert ffn(lib, moe(**mo), **kw) == want
+
+
+@pytest.mark.parametrize("kw", [dict(res=4 * AL + 4), dict(wts=2 * AL + 4), dict(ids=4 * AL), dict(wts=4 * AL + 64),
+                                dict(ws=AL), dict(ws=4 * AL), dict(ws=2 * AL), dict(ws=3 * AL), dict(res=64 * AL)])
+def test_moe_overlaps_are_refused(lib, kw):
+    a = dict(x=AL, ids=2 * AL, wts=3 * AL, res=None, y=4 * AL, ws=64 * AL)
+    a.update(kw)
+    assert ffn(lib, moe(), **a) == _lib.ERR_SHAPE
 
 
 def test_moe_null_and_layer_refusals(lib):
