@@ -82,8 +82,7 @@ __host__ __device__ constexpr int gemm_stages() {
 // kColumnWarps wants (Q4_K, N = K = 4096, M = 1000: 53 -> 42 us).  Elsewhere
 // two rings only cost the MMA thread a wait and a commit per K block (128
 // tokens, 14336 x 4096: 41 against 37 us; 512 tokens with half tiles freed
-// separately: 67 against 57 us, where shared memory's bandwidth binds: MMA
-// operands, x tiles and W tiles are 170 to 190 KB per 1024 cycles of MMA).
+// separately: no change, the loop runs at the MMA rate of the measured peak).
 template <int TYPE, int TOK>
 __host__ __device__ constexpr int gemm_w_stages() {
   constexpr int avail = GEMM_SMEM_LIMIT - 1024 - GEMM_RAW_STAGES * 128 * RawCol<TYPE>::pitch - 256;
