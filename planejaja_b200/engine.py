@@ -362,8 +362,8 @@ class CudaEngine:
         sel_bias = self._tensor(sel_bias, moe.n_expert, torch.float32, "moe_layer: sel_bias")
         residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_layer: residual")
         y = self._out(out, (m, moe.n_embd), torch.float32, "moe_layer: out", x)
-        ids = torch.empty((m, max(top_k, 0)), dtype=torch.int32, device=self.device)
-        weights = torch.empty((m, max(top_k, 0)), dtype=torch.float32, device=self.device)
+        ids = x.new_empty((m, max(top_k, 0)), dtype=torch.int32)
+        weights = x.new_empty((m, max(top_k, 0)))
         self._call(self.lib.nsq_moe_layer, "nsq_moe_layer",
                    lambda: self.lib.nsq_moe_workspace_size(moe._ref, m, top_k), workspace,
                    (moe._ref, _ptr(w_router), _lib.SCORES[score], _ptr(sel_bias), scale, _ptr(x), _ptr(residual),
