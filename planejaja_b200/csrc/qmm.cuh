@@ -9,7 +9,8 @@
 // -128..127).  The formats' integers meet the limbs in mma.sync m16n8k32 / k16
 // (u8 x s8, exact s32 sums): 16 weight rows as A and eight columns as B,
 // which are two tokens of four limbs (the fourth a copy, not used) or, from
-// five tokens on, one limb of eight tokens.  The integer scale of a group
+// five tokens on, one limb of eight tokens (six such tiles for 9 to 16 tokens,
+// over weights unpacked once: 14336 x 4096 Q4_K, 16 tokens 31 us; by eights 33).  The integer scale of a group
 // multiplies its sum in s32 too, so the first rounding comes after 256 weights:
 //   Q4_K, Q5_K  sum sc_j (sum q X_l): |sum| < 2^29;  d times it in f32.  The
 //               mins enter through the limb sums T of 16 activations (at most
@@ -362,7 +363,7 @@ __device__ __forceinline__ T qmm_lds(uint32_t off) {
 //   LIMBS == false: tile j holds tokens first + 2j and first + 2j + 1, column n
 //                   limb n % 4 of token first + 2j + n / 4 (limb 3: limb 0
 //                   again, its sums are not used)
-//   LIMBS == true:  tile j holds limb j of token first + n
+//   LIMBS == true:  tile j holds limb j % 3 of token first + 8 (j / 3) + n
 // Columns of absent tokens hold what was there; their sums are not used.
 template <bool LIMBS>
 struct QmmB {
@@ -385,17 +386,18 @@ struct QmmB {
   }
   __device__ __forceinline__ uint4 unit(int j, int i) const {
     // the middle limb's units are exchanged
-    if constexpr (LIMBS) return qmm_lds<uint4>(base[0] + 256 * j + (j == 1 ? 64 * (i ^ 1) : 64 * i));
+    if constexpr (LIMBS)
+      return qmm_lds<uint4>(base[0] + j / 3 * 8 * kQmmRecPitch + 256 * (j % 3) + (j % 3 == 1 ? 64 * (i ^ 1) : 64 * i));
     return qmm_lds<uint4>(base[i & 1] + 2 * kQmmRecPitch * j + 64 * i);
   }
   __device__ __forceinline__ uint2 sums(int j) const {
-    return qmm_lds<uint2>(t + (LIMBS ? 32 * j : 2 * kQmmRecPitch * j));
+    return qmm_lds<uint2>(t + (LIMBS ? j / 3 * 8 * kQmmRecPitch + 32 * (j % 3) : 2 * kQmmRecPitch * j));
   }
 };
 // Values of a lane per row half: one of a token's two limb pairs per tile, or
 // (LIMBS, three tiles) two whole tokens, 2c and 2c + 1.
 template <int NI, bool LIMBS>
-constexpr int kQmmVals = LIMBS ? 2 : NI;
+constexpr int kQmmVals = LIMBS ? 2 * NI / 3 : NI;
 // u += k * (the tiles' sums f as values)
 template <int NI, bool LIMBS>
 __device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], const float (&k)[2], const float (&f)[NI][4],
@@ -404,9 +406,9 @@ __device__ __forceinline__ void qmm_add(float (&u)[kQmmVals<NI, LIMBS>][2], cons
   for (int r = 0; r < 2; ++r) {
     if constexpr (LIMBS) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int e = 2 * r + q;
-        u[q][r] = fmaf(k[r], fmaf(65536.0f, f[2][e], fmaf(256.0f, f[1][e], f[0][e])), u[q][r]);
+      for (int q = 0; q < kQmmVals<NI, LIMBS>; ++q) {
+        const int e = 2 * r + (q & 1), j = 3 * (q >> 1);
+        u[q][r] = fmaf(k[r], fmaf(65536.0f, f[j + 2][e], fmaf(256.0f, f[j + 1][e], f[j][e])), u[q][r]);
       }
     } else {
 #pragma unroll
@@ -500,11 +502,11 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
 #pragma unroll
       for (int r = 0; r < 2; ++r) hg[r] = qmm_lds<uint2>(o[r] + 16 + 8 * c);
     }
-    int lo[NI][4], hi[NI][4];  // even and odd sub-blocks: Q4_K's odd ones count 16 times
+    int sum[NI][4];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) lo[j][e] = hi[j][e] = 0;
+      for (int e = 0; e < 4; ++e) sum[j][e] = 0;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // sub-blocks 2i, 2i + 1; weights 8c .. 8c + 7 of each
@@ -542,7 +544,7 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
       int se[2], so[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        se[r] = qmm_u8(sc[r][i >> 1], (2 * i) & 3);
+        se[r] = qmm_u8(sc[r][i >> 1], (2 * i) & 3) * (TYPE == NSQ_TYPE_Q4_K ? 16 : 1);  // (odd sub-blocks count 16 times)
         so[r] = qmm_u8(sc[r][i >> 1], (2 * i + 1) & 3);
       }
 #pragma unroll
@@ -551,17 +553,17 @@ __device__ __forceinline__ void qmm_unit(const uint32_t (&o)[2], int c, const Qm
         int acc[4];
         qmm_mma_k32<false>(acc, a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y, 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) lo[j][e] += acc[e] * se[e >> 1];
+        for (int e = 0; e < 4; ++e) sum[j][e] += acc[e] * se[e >> 1];
         qmm_mma_k32<false>(acc, b[0][0], b[1][0], b[0][1], b[1][1], x.z, x.w, 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) hi[j][e] += acc[e] * so[e >> 1];
+        for (int e = 0; e < 4; ++e) sum[j][e] += acc[e] * so[e >> 1];
       }
     }
     float f[NI][4];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[j][e] = (float)((TYPE == NSQ_TYPE_Q4_K ? 16 * lo[j][e] : lo[j][e]) + hi[j][e]);
+      for (int e = 0; e < 4; ++e) f[j][e] = (float)sum[j][e];
     }
     qmm_add<NI, LIMBS>(u, d, f, B.k256);
   } else if constexpr (TYPE == NSQ_TYPE_Q4_0 || TYPE == NSQ_TYPE_Q8_0) {
@@ -1368,39 +1370,34 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
             }
             o[h] = slot + my_rows + r * pitch + mis;
           }
-          auto unit = [&](auto N, auto Limbs, int first) {
+          auto unit = [&](auto N, auto Limbs) {
             constexpr int ni = decltype(N)::value;
             constexpr bool limbs = decltype(Limbs)::value;
             constexpr int nq = kQmmVals<ni, limbs>;
-            const QmmB<limbs> B(recs, first, lr, lc);
+            const QmmB<limbs> B(recs, 0, lr, lc);
             float v[nq][2];
             qmm_unit<TYPE, LAYOUT, ni, limbs>(o, lc, B, nv, v);
 #pragma unroll
             for (int q = 0; q < nq; ++q) {
-              const int tk = first + (limbs ? 2 * lc + q : 2 * q + (lc >> 1));
+              const int tk = limbs ? 8 * (q >> 1) + 2 * lc + (q & 1) : 2 * q + (lc >> 1);
               float s = tk < count ? qmm_lds<float>(recs + tk * kQmmRecPitch + kQmmRecS) : 0.0f;
               if (!limbs && (lc & 1)) s *= 65536.0f;  // limb 2 of the token
               const float y0 = s * v[q][0], y1 = s * v[q][1];
-              if (NQ <= 2 || first == 0) {
-                tot[t][q][0] += y0;
-                tot[t][q][1] += y1;
-              } else {
-                tot[t][NQ - 2 + (q & 1)][0] += y0;
-                tot[t][NQ - 2 + (q & 1)][1] += y1;
-              }
+              tot[t][q][0] += y0;
+              tot[t][q][1] += y1;
             }
           };
           using std::integral_constant;
           using std::false_type;
           using std::true_type;
           if (TC == 2 || count <= 2) {
-            unit(integral_constant<int, 1>{}, false_type{}, 0);
+            unit(integral_constant<int, 1>{}, false_type{});
           } else if (TC == 4 || count <= 4) {
-            if constexpr (TC > 2) unit(integral_constant<int, 2>{}, false_type{}, 0);
-          } else if constexpr (TC > 4) {
-            // eight tokens at a time (all sixteen at once would not fit the registers)
-#pragma unroll 1
-            for (int first = 0; first < (TC > 8 ? count : 8); first += 8) unit(integral_constant<int, 3>{}, true_type{}, first);
+            if constexpr (TC > 2) unit(integral_constant<int, 2>{}, false_type{});
+          } else if (TC == 8 || count <= 8) {
+            if constexpr (TC > 4) unit(integral_constant<int, 3>{}, true_type{});
+          } else if constexpr (TC > 8) {
+            unit(integral_constant<int, 6>{}, true_type{});
           }
         }
         __syncwarp();
