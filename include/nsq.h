@@ -312,8 +312,8 @@ int nsq_gemv_multi_xchg(const nsq_xsegment *segs, int nseg, const float *x, int6
  * sums: f32 results are off by about 3e-7 of their norm, bf16 ones rounded
  * once.  A token with an infinity or a NaN gives NaN throughout.  K is a
  * multiple of the type's block.  `workspace` (nsq_linear_workspace_size(M, K)
- * bytes, 16-byte aligned) is used by one call at a time and holds none of the
- * tensors.  y may lie on x.
+ * bytes, which serve every call of up to M and K; 16-byte aligned) is used by
+ * one call at a time and holds none of the tensors.  y may lie on x.
  * M > 16: bf16 only, K % 256 == 0, x and y 16-byte aligned and apart; the product of
  * nsq_gemm_bf16 (weights rounded to bf16, f32 sums), the epilogue in f32
  * before the one rounding of the result.  No workspace. */

@@ -467,7 +467,9 @@ static size_t linear_records(int64_t M, int64_t K) { return ((size_t)(M * units_
 
 size_t nsq_linear_workspace_size(int64_t M, int64_t K) {
   if (M < 1 || M > NSQ_GEMV_MAX_M || K < 1) return 0;
-  return linear_records(M, K) + kTicketBytes + parts_bytes(M, M);
+  // never less than a smaller call's: 8 tokens have row tiles twice as high as 9 to 15
+  const size_t parts = parts_bytes(M, M), of8 = parts_bytes(M < 8 ? M : 8, 8);
+  return linear_records(M, K) + kTicketBytes + (parts > of8 ? parts : of8);
 }
 
 int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, const float* bias, int act,

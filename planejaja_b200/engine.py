@@ -289,8 +289,10 @@ class CudaEngine:
             torch.cuda.synchronize(self.device)
 
     def linear_workspace(self, m: int, n: int, k: int) -> torch.Tensor:
-        """Workspace of `linear` calls of up to this size; one call at a time may use it."""
-        return torch.empty(self.lib.nsq_linear_workspace_size(m, k) or 16, dtype=torch.uint8, device=self.device)
+        """Workspace of `linear` calls of up to this size; one call at a time may use it.  (Calls of more than 16
+        tokens use none: one made for them serves those of up to 16.)"""
+        size = self.lib.nsq_linear_workspace_size(min(m, _lib.GEMV_MAX_M), k)
+        return torch.empty(size or 16, dtype=torch.uint8, device=self.device)
 
     def linear(self, x: torch.Tensor, w: torch.Tensor, ggml_type: int, n: int, k: int,
                bias: Optional[torch.Tensor] = None, act: str = "none", residual: Optional[torch.Tensor] = None,
