@@ -351,6 +351,8 @@ typedef struct nsq_moe {
 #define NSQ_MOE_MAX_EXPERTS 512
 #define NSQ_MOE_MAX_TOP_K 16
 
+/* Bytes that serve every call of up to M tokens and top_k picks with these
+ * experts (16-byte aligned, used by one call at a time). */
 size_t nsq_moe_workspace_size(const nsq_moe* moe, int64_t M, int64_t top_k);
 
 /* The experts' products for given picks: ids [M x top_k], weights [M x

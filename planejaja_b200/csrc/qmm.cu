@@ -354,7 +354,11 @@ static MoeSpace moe_space(int64_t E, int64_t D, int64_t F, int64_t M, int64_t to
   s.ngroups = take(4);
   s.done = take((size_t)(P * units_of(F)) * 4);
   s.tickets = take(2 * kTicketBytes);  // of both products
-  s.parts = take(parts_bytes(M, moe_group(E, M, top_k)));
+  // never less than a smaller call's: one of few tokens or picks may have
+  // groups of 8, whose row tiles are twice as high as those of 9 to 16
+  const int64_t of8 = 4 * E > 8 ? 4 * E : 8;  // tokens that have, with one pick
+  const size_t parts = parts_bytes(M, moe_group(E, M, top_k)), parts8 = parts_bytes(M < of8 ? M : of8, 8);
+  s.parts = take(parts > parts8 ? parts : parts8);
   s.total = at;
   return s;
 }

@@ -323,7 +323,7 @@ class CudaEngine:
         return y
 
     def moe_workspace(self, moe: MoeExperts, m: int, top_k: int) -> torch.Tensor:
-        """Workspace of `moe_ffn` / `moe_layer` calls of this size; one call at a time may use it."""
+        """Workspace of `moe_ffn` / `moe_layer` calls of up to this size; one call at a time may use it."""
         return torch.empty(self.lib.nsq_moe_workspace_size(moe._ref, m, top_k) or 16, dtype=torch.uint8,
                            device=self.device)
 

@@ -40,3 +40,20 @@ def test_linear_workspace_of_a_prompt_serves_decode_calls(lib):
         assert eng.linear_workspace(m, 64, 1024).numel() >= lib.nsq_linear_workspace_size(16, 1024)
     for m in range(1, 17):
         assert eng.linear_workspace(m, 64, 1024).numel() == lib.nsq_linear_workspace_size(m, 1024)
+
+
+def moe_size(lib, m, top_k, e=8, d=512, f=512):
+    import ctypes
+    mo = _lib.Moe(0x10000, 0x10000, 0x10000, 12, 0, 12, 0, 1, e, d, f)
+    return lib.nsq_moe_workspace_size(ctypes.addressof(mo), m, top_k)
+
+
+@pytest.mark.parametrize("e", [1, 2, 7, 8, 60, 512])
+def test_moe_workspace_never_shrinks(lib, e):
+    """With the tokens and with the picks of each: one made for the largest call serves the others."""
+    for top_k in range(1, _lib.MOE_MAX_TOP_K + 1):
+        sizes = [moe_size(lib, m, top_k, e) for m in range(1, _lib.MOE_MAX_TOKENS + 1)]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:])), (top_k, sizes)
+    for m in range(1, _lib.MOE_MAX_TOKENS + 1):
+        sizes = [moe_size(lib, m, top_k, e) for top_k in range(1, _lib.MOE_MAX_TOP_K + 1)]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:])), (m, sizes)
