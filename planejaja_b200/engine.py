@@ -56,7 +56,7 @@ def _stream_handle(device: torch.device) -> int:
 
 
 class MoeExperts:
-    """The experts of a mixture-of-experts layer: three GGUF tensors on the
+    """The experts of a mixture-of-experts layer: three GGUF tensors on one
     device, as they lie in the file (ffn_gate_exps and ffn_up_exps
     [n_expert x n_ff rows of n_embd], ffn_down_exps [n_expert x n_embd rows of
     n_ff])."""
@@ -70,19 +70,22 @@ class MoeExperts:
                 raise NsqError(_lib.ERR_TYPE, f"MoeExperts: {name} has ggml type {t}")
             if min(n_expert, n, k) < 1 or k % FORMATS[t].block_weights:
                 raise NsqError(_lib.ERR_SHAPE, f"MoeExperts: {name} [{n_expert} x {n} x {k}]")
-            _check_bytes(w, n_expert * FORMATS[t].tensor_bytes(n, k), f"MoeExperts: {name}")
+            _check_bytes(w, n_expert * FORMATS[t].tensor_bytes(n, k), f"MoeExperts: {name}", w_gate.get_device())
         if act not in _lib.ACTS:
             raise NsqError(_lib.ERR_TYPE, f"MoeExperts: activation {act!r}")
         self.w_gate, self.w_up, self.w_down = w_gate, w_up, w_down
         self.n_expert, self.n_embd, self.n_ff = n_expert, n_embd, n_ff
+        self.device_index = w_gate.get_device()
         self._c = _lib.Moe(_ptr(w_gate), _ptr(w_up), _ptr(w_down), type_in, layout_in, type_down, layout_down,
                            _lib.ACTS[act], n_expert, n_embd, n_ff)
         self._ref = ctypes.addressof(self._c)
 
 
-def _check_bytes(w: torch.Tensor, nbytes: int, what: str) -> None:
+def _check_bytes(w: torch.Tensor, nbytes: int, what: str, device: int) -> None:
     if w.dtype != torch.uint8 or not w.is_cuda or not w.is_contiguous():
         raise NsqError(_lib.ERR_TYPE, f"{what}: GGUF bytes are a contiguous uint8 CUDA tensor")
+    if w.get_device() != device:  # the kernels would read memory that the GPU need not have mapped
+        raise NsqError(_lib.ERR_DEVICE, f"{what}: on {w.device}, cuda:{device} is wanted")
     if w.numel() < nbytes:
         raise NsqError(_lib.ERR_SHAPE, f"{what}: {w.numel()} bytes, {nbytes} needed")
 
@@ -245,6 +248,16 @@ class CudaEngine:
         return self.gemm_bf16(w, ggml_type, xb, n, k, q6k_layout, sync=sync).float()
 
     # ---- products with an epilogue, and mixture-of-experts layers -----------
+    def _index(self) -> int:
+        """The device that calls run on: the engine's, or the current one where the engine names none."""
+        index = self.device.index
+        return torch._C._cuda_getDevice() if index is None else index
+
+    def _check_experts(self, moe: MoeExperts, what: str) -> None:
+        if moe.device_index != self._index():
+            raise NsqError(_lib.ERR_DEVICE, f"{what}: the experts are on cuda:{moe.device_index}, the engine is on "
+                                            f"{self.device}")
+
     def _tensor(self, t: Optional[torch.Tensor], numel: int, dtype: torch.dtype, what: str) -> Optional[torch.Tensor]:
         """`t` as the library reads it: contiguous, of this dtype and size, on the engine's device."""
         if t is None:
@@ -253,7 +266,7 @@ class CudaEngine:
             return t  # small calls are bound by the host: the usual case first
         if t.dtype != dtype or not t.is_cuda:
             raise NsqError(_lib.ERR_TYPE, f"{what}: a {dtype} CUDA tensor is wanted, not {t.dtype} on {t.device}")
-        if self.device.index is not None and t.device.index != self.device.index:
+        if t.device.index != self._index():
             raise NsqError(_lib.ERR_DEVICE, f"{what}: on {t.device}, the engine is on {self.device}")
         if t.numel() != numel:
             raise NsqError(_lib.ERR_SHAPE, f"{what}: {t.numel()} elements, not {numel}")
@@ -312,7 +325,7 @@ class CudaEngine:
         if k < 1 or n < 1 or size % k or k % f.block_weights:
             raise NsqError(_lib.ERR_SHAPE, f"linear: {size} activations, n = {n}, k = {k}")
         m = size // k
-        _check_bytes(w, n * k // f.block_weights * f.block_bytes, "linear: w")
+        _check_bytes(w, n * k // f.block_weights * f.block_bytes, "linear: w", self._index())
         x = self._tensor(x, size, dtype, "linear: x")
         bias = self._tensor(bias, n, torch.float32, "linear: bias")
         residual = self._tensor(residual, m * n, dtype, "linear: residual")
@@ -324,6 +337,7 @@ class CudaEngine:
 
     def moe_workspace(self, moe: MoeExperts, m: int, top_k: int) -> torch.Tensor:
         """Workspace of `moe_ffn` / `moe_layer` calls of up to this size; one call at a time may use it."""
+        self._check_experts(moe, "moe_workspace")
         return torch.empty(self.lib.nsq_moe_workspace_size(moe._ref, m, top_k) or 16, dtype=torch.uint8,
                            device=self.device)
 
@@ -334,6 +348,7 @@ class CudaEngine:
 
         x [m, n_embd] f32; ids [m, top_k] int32, -1 for an unused slot; weights [m, top_k] f32.  `out` may be
         `residual`."""
+        self._check_experts(moe, "moe_ffn")
         if ids.dim() != 2:
             raise NsqError(_lib.ERR_SHAPE, "moe_ffn: ids are [tokens, top_k]")
         m, top_k = ids.shape
@@ -354,6 +369,7 @@ class CudaEngine:
 
         w_router [n_expert, n_embd] f32 (GGUF ffn_gate_inp); score one of "softmax", "softmax_norm",
         "sigmoid_norm"; sel_bias [n_expert] enters the choice alone."""
+        self._check_experts(moe, "moe_layer")
         if score not in _lib.SCORES:
             raise NsqError(_lib.ERR_TYPE, f"moe_layer: score {score!r}")
         if x.numel() % moe.n_embd:
