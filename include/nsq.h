@@ -334,9 +334,10 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
  *   h_j  = act(x . W_gate[e_j]^T) * (x . W_up[e_j]^T)        [n_ff]
  *   y[m] = residual[m] + sum_j weight[m, j] * (h_j . W_down[e_j]^T)
  * over the top_k picks e_j = ids[m, j] of token m.  All tensors but the
- * experts are f32; residual may be NULL or y itself, y may lie on x; no other
- * tensor and nothing in the workspace overlaps (NSQ_ERR_SHAPE).  Accuracy as
- * nsq_linear's f32.  A reference routing shader exists but is never built
+ * experts are f32; residual may be NULL or y itself, y may lie on x; else
+ * nothing that a call writes (y, the workspace, nsq_moe_layer's ids and
+ * weights) overlaps another tensor, nor ids weights (NSQ_ERR_SHAPE).  Accuracy
+ * as nsq_linear's f32.  A reference routing shader exists but is never built
  * (crates/nodestor-vulkan/build.rs:24, moe_routing). */
 typedef struct nsq_moe {
   const void *w_gate; /* [E x n_ff rows of n_embd], type_in, 16-byte aligned */

@@ -391,12 +391,30 @@ static int run_moe(const nsq_moe* moe, const float* w_router, int score, const f
   const MoeSpace s = moe_space(E, D, F, M, top_k);
   if (!workspace || workspace_bytes < s.total) return NSQ_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NSQ_ERR_ALIGN;
-  // (x is read by the first kernel alone, y written by the last)
+  // What the call writes (y, the workspace, the router's picks) lies apart from
+  // what it reads and from one another; but y may lie on x, which the first
+  // kernel alone reads, and on residual, element on element.
   const size_t xb = (size_t)(M * D) * 4, pb = (size_t)(M * top_k) * 4;
-  if ((residual != y && overlap(residual, xb, y, xb)) || overlap(ids, pb, weights, pb) || overlap(ids, pb, y, xb) ||
-      overlap(weights, pb, y, xb) || overlap(workspace, s.total, x, xb) || overlap(workspace, s.total, y, xb) ||
-      overlap(workspace, s.total, residual, xb) || overlap(workspace, s.total, ids, pb) ||
-      overlap(workspace, s.total, weights, pb))
+  struct Range {
+    const void* at;
+    size_t bytes;
+  };
+  const Range ws_r{workspace, s.total}, y_r{y, xb}, ids_r{ids, pb}, wts_r{weights, pb}, x_r{x, xb}, res_r{residual, xb};
+  const Range only_read[] = {
+      {w_router, (size_t)(E * D) * 4},
+      {sel_bias, (size_t)E * 4},
+      {moe->w_gate, (size_t)(E * F * (D / nsq_block_weights(moe->type_in)) * nsq_block_bytes(moe->type_in))},
+      {moe->w_up, (size_t)(E * F * (D / nsq_block_weights(moe->type_in)) * nsq_block_bytes(moe->type_in))},
+      {moe->w_down, (size_t)(E * D * (F / nsq_block_weights(moe->type_down)) * nsq_block_bytes(moe->type_down))}};
+  auto meet = [](const Range& a, const Range& b) { return overlap(a.at, a.bytes, b.at, b.bytes); };
+  for (const Range& r : only_read) {
+    if (meet(r, ws_r) || meet(r, y_r) || (w_router && (meet(r, ids_r) || meet(r, wts_r)))) return NSQ_ERR_SHAPE;
+  }
+  for (const Range& r : {x_r, res_r}) {
+    if (meet(r, ws_r) || (w_router && (meet(r, ids_r) || meet(r, wts_r)))) return NSQ_ERR_SHAPE;
+  }
+  if ((residual != y && meet(res_r, y_r)) || meet(ids_r, wts_r) || meet(y_r, ids_r) || meet(y_r, wts_r) ||
+      meet(ws_r, y_r) || meet(ws_r, ids_r) || meet(ws_r, wts_r))
     return NSQ_ERR_SHAPE;
   int num_sms = 0;
   if ((rc = device_check(&num_sms))) return rc;

@@ -137,3 +137,69 @@ def test_experts_of_another_device_are_refused(lib):
         assert status_of(call, there) == _lib.ERR_DEVICE
         assert status_of(call, here) == _lib.ERR_TYPE  # x is no CUDA tensor
     assert status_of(eng.moe_workspace, there, 2, 1) == _lib.ERR_DEVICE
+
+
+# ---------------------------------------------------------------- overlapping ranges
+# Addresses that are never dereferenced: a range of A bytes for each tensor.
+A = 1 << 32
+NAMES = ["gate", "up", "down", "router", "bias", "x", "res", "y", "ids", "wts", "ws"]
+PLACES = {n: (i + 1) * A for i, n in enumerate(NAMES)}
+M, K, E, D, F = 3, 2, 8, 512, 256
+ROW_IN, ROW_DOWN = 2 * 144, 210  # bytes of a row: Q4_K of 512, Q6_K of 256
+SIZES = dict(gate=E * F * ROW_IN, up=E * F * ROW_IN, down=E * D * ROW_DOWN, router=E * D * 4, bias=E * 4, x=M * D * 4,
+             res=M * D * 4, y=M * D * 4, ids=M * K * 4, wts=M * K * 4)
+
+
+def moe_call(lib, given=False, **at):
+    import ctypes
+    a = dict(PLACES, **at)
+    mo = _lib.Moe(a["gate"], a["up"], a["down"], 12, 0, 14, 0, 1, E, D, F)
+    ref = ctypes.addressof(mo)
+    size = lib.nsq_moe_workspace_size(ref, M, K)
+    if given:
+        return lib.nsq_moe_ffn(ref, a["x"], a["ids"], a["wts"], a["res"], a["y"], M, K, a["ws"], size, None)
+    return lib.nsq_moe_layer(ref, a["router"], 0, a["bias"], 1.0, a["x"], a["res"], a["y"], a["ids"], a["wts"], M, K,
+                             a["ws"], size, None)
+
+
+def ends(lib, name):
+    import ctypes
+    mo = _lib.Moe(A, A, A, 12, 0, 14, 0, 1, E, D, F)
+    size = SIZES.get(name) or lib.nsq_moe_workspace_size(ctypes.addressof(mo), M, K)
+    return PLACES[name], PLACES[name] + (size - 1) // 16 * 16
+
+
+# what a call writes, against everything else that it has: y may lie on x and on all of residual
+PAIRS = [(w, o) for w in ("y", "ids", "wts", "ws") for o in NAMES if o != w and (w, o) != ("y", "x")]
+
+
+@pytest.mark.parametrize("written,other", PAIRS)
+def test_moe_layer_refuses_outputs_over_other_tensors(lib, written, other):
+    """On the first and on the last 16 bytes of the other tensor."""
+    first, last = ends(lib, other)
+    for at in ((last,) if (written, other) == ("y", "res") else (first, last)):
+        assert moe_call(lib, **{written: at}) == _lib.ERR_SHAPE, (written, other, at)
+
+
+@pytest.mark.parametrize("other", [n for n in NAMES if n not in ("ws", "router", "bias")])
+def test_moe_ffn_refuses_its_workspace_and_output_over_other_tensors(lib, other):
+    for at in ends(lib, other):
+        assert moe_call(lib, given=True, ws=at) == _lib.ERR_SHAPE, other
+        if other not in ("x", "y") and (other, at) != ("res", PLACES["res"]):
+            assert moe_call(lib, given=True, y=at) == _lib.ERR_SHAPE, other
+
+
+def passes(status):
+    return status in (_lib.ERR_CUDA, _lib.ERR_DEVICE)
+
+
+def test_moe_allowed_overlaps_pass_the_checks(lib):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not the device's")
+    p = PLACES
+    for kw in (dict(), dict(y=p["x"]), dict(y=p["x"] + 16), dict(y=p["res"]), dict(res=p["x"], y=p["x"]), dict(res=None),
+               dict(res=p["x"]), dict(bias=None), dict(bias=p["router"]), dict(gate=p["up"]), dict(x=p["router"])):
+        assert passes(moe_call(lib, **kw)), kw
+    for kw in (dict(), dict(y=p["x"]), dict(y=p["res"]), dict(ids=p["x"]), dict(wts=p["x"]), dict(wts=p["res"])):
+        assert passes(moe_call(lib, given=True, **kw)), kw
