@@ -307,7 +307,7 @@ int nsq_gemv_multi_xchg(const nsq_xsegment *segs, int nseg, const float *x, int6
  *   dtype     element type of x, residual and y: NSQ_OUT_F32 or NSQ_OUT_BF16
  *   bias      N f32, or NULL;  act: NSQ_ACT_*
  *   residual  [M x N] of dtype, or NULL; may be y itself
- * y overlaps neither a part of residual nor bias (NSQ_ERR_SHAPE).
+ * y overlaps neither a part of residual nor bias nor w (NSQ_ERR_SHAPE).
  * M = 1..16: 24-bit activations per 256 of K, exact integer products, f32
  * sums: f32 results are off by about 3e-7 of their norm, bf16 ones rounded
  * once.  A token with an infinity or a NaN gives NaN throughout.  K is a

@@ -510,7 +510,9 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   if (reinterpret_cast<uintptr_t>(bias) & 3) return NSQ_ERR_ALIGN;
   const size_t es = dtype == NSQ_OUT_F32 ? 4 : 2, xb = (size_t)(M * K) * es, yb = (size_t)(M * N) * es;
   const bool y_on_x = overlap(x, xb, y, yb);
-  const bool y_on_others = (residual != y && overlap(residual, yb, y, yb)) || overlap(bias, (size_t)N * 4, y, yb);
+  const size_t w_bytes = (size_t)(N * (K / nsq_block_weights(ggml_type)) * nsq_block_bytes(ggml_type));
+  const bool y_on_others = (residual != y && overlap(residual, yb, y, yb)) || overlap(bias, (size_t)N * 4, y, yb) ||
+                           overlap(w, w_bytes, y, yb);
   if (prompt) {
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) return NSQ_ERR_ALIGN;
     if (y_on_x || y_on_others) return NSQ_ERR_SHAPE;
@@ -523,7 +525,8 @@ int nsq_linear(const void* w, int ggml_type, int q6k_layout, const void* x, cons
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NSQ_ERR_ALIGN;
   const size_t wb = nsq_linear_workspace_size(M, K);
   if (y_on_others || overlap(workspace, wb, x, xb) || overlap(workspace, wb, y, yb) ||
-      overlap(workspace, wb, residual, yb) || overlap(workspace, wb, bias, (size_t)N * 4))
+      overlap(workspace, wb, residual, yb) || overlap(workspace, wb, bias, (size_t)N * 4) ||
+      overlap(workspace, wb, w, w_bytes))
     return NSQ_ERR_SHAPE;
   int num_sms = 0;
   if ((rc = device_check(&num_sms))) return rc;

@@ -203,3 +203,22 @@ def test_moe_allowed_overlaps_pass_the_checks(lib):
         assert passes(moe_call(lib, **kw)), kw
     for kw in (dict(), dict(y=p["x"]), dict(y=p["res"]), dict(ids=p["x"]), dict(wts=p["x"]), dict(wts=p["res"])):
         assert passes(moe_call(lib, given=True, **kw)), kw
+
+
+def linear_call(lib, m=1, n=512, k=512, t=12, dtype=0, **at):
+    a = dict(w=A, x=2 * A, bias=3 * A, res=4 * A, y=5 * A, ws=6 * A)
+    a.update(at)
+    return lib.nsq_linear(a["w"], t, 0, a["x"], a["bias"], 0, a["res"], a["y"], dtype, m, n, k, a["ws"],
+                          lib.nsq_linear_workspace_size(min(m, 16), k), None)
+
+
+def test_linear_refuses_outputs_over_its_weights(lib):
+    import torch
+    last = A + 512 * ROW_IN - 16
+    for at in (A, last):
+        assert linear_call(lib, ws=at) == _lib.ERR_SHAPE
+        for m, dtype in ((1, 0), (16, 1), (17, 1)):
+            assert linear_call(lib, m, dtype=dtype, y=at) == _lib.ERR_SHAPE, (m, at)
+    if not torch.cuda.is_available():
+        assert passes(linear_call(lib)) and passes(linear_call(lib, ws=last + 16)) and passes(linear_call(lib, y=last + 16))
+        assert passes(linear_call(lib, 17, dtype=1, ws=A))  # no workspace is used
