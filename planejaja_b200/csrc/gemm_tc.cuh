@@ -716,7 +716,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
     }
     // ---- epilogue: warp w reads TMEM lanes 32*(w%4).. (its W rows) for a
     // quarter of the TOK accumulator columns
-    have = ok && mbar_wait_bounded(accum, 0);
+    // (the same in every lane: what follows are instructions of whole warps)
+    have = __all_sync(0xffffffffu, ok && mbar_wait_bounded(accum, 0));
     if (have) tc_fence_after();
     if (split == 1) {
       if (have) {
@@ -742,6 +743,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
               if (m < p.M) p.y[m * p.N + n] = __float2bfloat16_rn(__uint_as_float(v[j]));
             }
           }
+          __syncwarp();  // lanes behind the last row meet the others before the next load of the whole warp
         }
       }
     }
@@ -785,6 +787,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
                              v[4 * g + 3]);
         }
       }
+      __syncwarp();
       gemm_cluster_sync();  // partials of this round have landed
       if (epi_warp && have) {
         const int64_t n = n0 + 32 * qd + lane;
@@ -809,6 +812,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
           }
         }
       }
+      __syncwarp();  // (the barrier is one of whole warps, and lanes behind the last row were apart)
       gemm_cluster_sync();  // the owners are done with the slots of this round
     }
   }

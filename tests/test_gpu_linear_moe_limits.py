@@ -8,6 +8,7 @@ import torch
 from planejaja_b200 import _lib
 from planejaja_b200 import quantize as Q
 from planejaja_b200.formats import Q4_0, Q4_K, Q5_K, Q6_K, Q8_0
+from test_gpu_linear_moe import act64, bf16
 
 pytestmark = pytest.mark.gpu
 
@@ -32,6 +33,43 @@ def test_linear_kept_workspace_serves_smaller_calls(eng, t):
             for m in range(1, min(made_for, 16) + 1):
                 y = eng.linear(x[:m].contiguous(), w, t, n, k, workspace=ws)
                 assert torch.equal(y, want[m - 1]), (made_for, m)
+
+
+
+def prompt_reference(oracle, raw, t, n, k, x, bias, act, residual, parts):
+    """nsq_linear for prompts in 64 bits over weights rounded to bf16, and what a bf16 result may be off by.
+
+    The f32 sums truncate at most once per 16 products and once per joined part, 2^-23 of at most A = |x| . |w|
+    each; the activations' slopes are at most 1.13 and their own errors below 2^-20 of the sum; the result is
+    rounded once, by at most 2^-8 of itself."""
+    w = bf16(oracle.dequant(raw, t, 0).reshape(n, k))
+    v = x @ w.T + bias
+    e = 1.13 * 2.0 ** -23 * (k / 16 + parts) * (np.abs(x) @ np.abs(w).T + np.abs(bias)) + 2.0 ** -20 * np.abs(v)
+    v = act64(v, act) + residual
+    return v, e + 2.0 ** -8 * (np.abs(v) + e)
+
+
+@pytest.mark.parametrize("tok", [128, 256, 512])
+@pytest.mark.parametrize("split", [1, 2, 3, 5, 8])
+def test_prompts_with_lanes_behind_the_last_row(eng, oracle, tuning, tok, split):
+    """N that ends inside a warp's 32 rows, every activation: warps meet again before each load and barrier of theirs."""
+    tuning.set("NSQ_GEMM_TOK", tok)
+    tuning.set("NSQ_GEMM_SPLIT", split)
+    m, k = 70, 2048
+    for n in (1, 45, 129, 1003):
+        r = np.random.default_rng(n + split)
+        raw = Q.synthetic_weights(n, k, Q4_K, seed=n)
+        w = eng.upload(raw)
+        x, b, s = bf16(r.standard_normal((m, k))), bf16(r.standard_normal(n)), bf16(r.standard_normal((m, n)))
+        xd, sd = torch.from_numpy(x).cuda().bfloat16(), torch.from_numpy(s).cuda().bfloat16()
+        bd = torch.from_numpy(b).cuda().float()
+        for act in sorted(_lib.ACTS):
+            y = eng.linear(xd, w, Q4_K, n, k, bias=bd, act=act, residual=sd).double().cpu().numpy()
+            v, tol = prompt_reference(oracle, raw, Q4_K, n, k, x, b, act, s, split)
+            assert np.all(np.abs(y - v) <= tol), (n, act, float((np.abs(y - v) / tol).max()))
+        y = eng.gemm_bf16(w, Q4_K, xd, n, k).double().cpu().numpy()
+        v, tol = prompt_reference(oracle, raw, Q4_K, n, k, x, 0 * b, "none", 0 * s, split)
+        assert np.all(np.abs(y - v) <= tol), n
 
 
 # ---------------------------------------------------------------- mixture of experts
