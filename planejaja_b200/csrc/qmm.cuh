@@ -1287,6 +1287,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       if (mine) last = qmm_add_acq_rel(p.done + (int64_t)g * nsb + sb, rows) + rows == valid;
     }
     if (!__shfl_sync(0xffffffffu, last, 0)) return;
+    __syncwarp();  // what lane 0 acquired is the other lanes' too (a shuffle orders no memory)
     const int count = L.groups[g].count, start = L.groups[g].start;
     for (int t = 0; t < count; ++t) {
       const int64_t pick = L.plist[start + t];
@@ -1524,6 +1525,7 @@ __global__ void __launch_bounds__(kQmmThreads, 2)
       int last = 0;
       if (lane == 0) last = qmm_add_acq_rel(p.tickets + c_lo * kQmmWarps + rw, n_steps) + n_steps == st;
       if (__shfl_sync(0xffffffffu, last, 0)) {
+        __syncwarp();  // (as in report_rows)
         // eight parts' loads at a time: one after the other their latencies
         // were 50 us of 32 tokens' and 64 experts' 207
         emit([&](auto& v, int at) {

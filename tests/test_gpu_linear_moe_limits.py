@@ -90,3 +90,23 @@ def test_moe_kept_workspace_serves_smaller_calls(eng):
         want = eng.moe_layer(moe, wr, x[:m].contiguous(), k)
         got = eng.moe_layer(moe, wr, x[:m].contiguous(), k, workspace=ws)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), (m, k)
+
+
+def test_divided_tasks_joined_by_many_ctas_repeat(eng, tuning):
+    """Every task divided, its parts and rows of h read by the last CTA to arrive: the same bits each time."""
+    tuning.set("NSQ_QMM_SPLIT", 1)
+    for t, m, e, d, f in ((Q4_K, 24, 8, 512, 2048), (Q8_0, 5, 4, 1056, 992), (Q6_K, 2, 16, 768, 1280)):
+        moe = experts(eng, e, d, f, t, Q8_0 if t == Q8_0 else Q4_K)
+        x, wr = torch.randn(m, d, device="cuda"), torch.randn(e, d, device="cuda")
+        ws = eng.moe_workspace(moe, m, 3)
+        want = eng.moe_layer(moe, wr, x, 3, workspace=ws)
+        got = [eng.moe_layer(moe, wr, x, 3, workspace=ws, sync=False)[0] for _ in range(50)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[0]) for y in got), t
+        n = 640
+        w = eng.upload(Q.synthetic_weights(n, d, t, seed=9))
+        x = x[:16].contiguous()
+        want = eng.linear(x, w, t, n, d)
+        got = [eng.linear(x, w, t, n, d, sync=False) for _ in range(50)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in got), t
