@@ -90,6 +90,18 @@ def _check_bytes(w: torch.Tensor, nbytes: int, what: str, device: int) -> None:
         raise NsqError(_lib.ERR_SHAPE, f"{what}: {w.numel()} bytes, {nbytes} needed")
 
 
+def _has_rows(shape, row: int) -> bool:
+    """Whether a tensor of this shape is a list of rows of `row` elements: its last dimensions make one up
+    ([tokens, heads, size] holds rows of heads x size), or it is one run of elements."""
+    dims = [s for s in shape if s != 1]
+    size = 1
+    for s in reversed(dims):
+        if size == row:
+            return True
+        size *= s
+    return size == row or len(dims) <= 1
+
+
 class CudaEngine:
     """Engine facade over libnsq for one CUDA device."""
 
@@ -258,11 +270,14 @@ class CudaEngine:
             raise NsqError(_lib.ERR_DEVICE, f"{what}: the experts are on cuda:{moe.device_index}, the engine is on "
                                             f"{self.device}")
 
-    def _tensor(self, t: Optional[torch.Tensor], numel: int, dtype: torch.dtype, what: str) -> Optional[torch.Tensor]:
-        """`t` as the library reads it: contiguous, of this dtype and size, on the engine's device."""
+    def _tensor(self, t: Optional[torch.Tensor], numel: int, dtype: torch.dtype, what: str,
+                row: int = 0) -> Optional[torch.Tensor]:
+        """`t` as the library reads it: contiguous, of this dtype and size, on the engine's device, its last
+        dimensions making up rows of `row` elements (where it has rows)."""
         if t is None:
             return None
-        if t.dtype is dtype and t.device == self.device and t.numel() == numel and t.is_contiguous():
+        if (t.dtype is dtype and t.device == self.device and t.numel() == numel
+                and (not row or numel == row or t.shape[-1] == row) and t.is_contiguous()):
             return t  # small calls are bound by the host: the usual case first
         if t.dtype != dtype or not t.is_cuda:
             raise NsqError(_lib.ERR_TYPE, f"{what}: a {dtype} CUDA tensor is wanted, not {t.dtype} on {t.device}")
@@ -270,6 +285,8 @@ class CudaEngine:
             raise NsqError(_lib.ERR_DEVICE, f"{what}: on {t.device}, the engine is on {self.device}")
         if t.numel() != numel:
             raise NsqError(_lib.ERR_SHAPE, f"{what}: {t.numel()} elements, not {numel}")
+        if row and not _has_rows(t.shape, row):
+            raise NsqError(_lib.ERR_SHAPE, f"{what}: {list(t.shape)} has no rows of {row}")
         return t if t.is_contiguous() else t.contiguous()
 
     def _out(self, out: Optional[torch.Tensor], shape, dtype: torch.dtype, what: str, like: torch.Tensor) -> torch.Tensor:
@@ -277,7 +294,7 @@ class CudaEngine:
             return like.new_empty(shape)
         if not out.is_contiguous():
             raise NsqError(_lib.ERR_SHAPE, f"{what}: the output has to be contiguous")
-        return self._tensor(out, shape[0] * shape[1], dtype, what)
+        return self._tensor(out, shape[0] * shape[1], dtype, what, shape[1])
 
     def _call(self, fn, what: str, nbytes, workspace: Optional[torch.Tensor], args, sync: bool) -> None:
         """fn(*args, workspace, bytes, stream) with the engine's device current.  Without a workspace of the
@@ -326,9 +343,9 @@ class CudaEngine:
             raise NsqError(_lib.ERR_SHAPE, f"linear: {size} activations, n = {n}, k = {k}")
         m = size // k
         _check_bytes(w, n * k // f.block_weights * f.block_bytes, "linear: w", self._index())
-        x = self._tensor(x, size, dtype, "linear: x")
+        x = self._tensor(x, size, dtype, "linear: x", k)
         bias = self._tensor(bias, n, torch.float32, "linear: bias")
-        residual = self._tensor(residual, m * n, dtype, "linear: residual")
+        residual = self._tensor(residual, m * n, dtype, "linear: residual", n)
         y = self._out(out, (m, n), dtype, "linear: out", x)
         self._call(self.lib.nsq_linear, "nsq_linear", lambda: self.lib.nsq_linear_workspace_size(m, k), workspace,
                    (_ptr(w), ggml_type, q6k_layout, _ptr(x), _ptr(bias), _lib.ACTS[act], _ptr(residual), _ptr(y),
@@ -352,10 +369,10 @@ class CudaEngine:
         if ids.dim() != 2:
             raise NsqError(_lib.ERR_SHAPE, "moe_ffn: ids are [tokens, top_k]")
         m, top_k = ids.shape
-        x = self._tensor(x, m * moe.n_embd, torch.float32, "moe_ffn: x")
+        x = self._tensor(x, m * moe.n_embd, torch.float32, "moe_ffn: x", moe.n_embd)
         ids = self._tensor(ids, m * top_k, torch.int32, "moe_ffn: ids")
-        weights = self._tensor(weights, m * top_k, torch.float32, "moe_ffn: weights")
-        residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_ffn: residual")
+        weights = self._tensor(weights, m * top_k, torch.float32, "moe_ffn: weights", top_k)
+        residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_ffn: residual", moe.n_embd)
         y = self._out(out, (m, moe.n_embd), torch.float32, "moe_ffn: out", x)
         self._call(self.lib.nsq_moe_ffn, "nsq_moe_ffn", lambda: self.lib.nsq_moe_workspace_size(moe._ref, m, top_k),
                    workspace, (moe._ref, _ptr(x), _ptr(ids), _ptr(weights), _ptr(residual), _ptr(y), m, top_k), sync)
@@ -375,10 +392,10 @@ class CudaEngine:
         if x.numel() % moe.n_embd:
             raise NsqError(_lib.ERR_SHAPE, f"moe_layer: {x.numel()} activations, n_embd = {moe.n_embd}")
         m = x.numel() // moe.n_embd
-        x = self._tensor(x, m * moe.n_embd, torch.float32, "moe_layer: x")
-        w_router = self._tensor(w_router, moe.n_expert * moe.n_embd, torch.float32, "moe_layer: w_router")
+        x = self._tensor(x, m * moe.n_embd, torch.float32, "moe_layer: x", moe.n_embd)
+        w_router = self._tensor(w_router, moe.n_expert * moe.n_embd, torch.float32, "moe_layer: w_router", moe.n_embd)
         sel_bias = self._tensor(sel_bias, moe.n_expert, torch.float32, "moe_layer: sel_bias")
-        residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_layer: residual")
+        residual = self._tensor(residual, m * moe.n_embd, torch.float32, "moe_layer: residual", moe.n_embd)
         y = self._out(out, (m, moe.n_embd), torch.float32, "moe_layer: out", x)
         ids = x.new_empty((m, max(top_k, 0)), dtype=torch.int32)
         weights = x.new_empty((m, max(top_k, 0)))

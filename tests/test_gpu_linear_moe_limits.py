@@ -110,3 +110,21 @@ def test_divided_tasks_joined_by_many_ctas_repeat(eng, tuning):
         got = [eng.linear(x, w, t, n, d, sync=False) for _ in range(50)]
         torch.cuda.synchronize()
         assert all(torch.equal(y, want) for y in got), t
+
+
+def test_shapes_that_hold_the_rows_otherwise(eng):
+    """Flat tensors, heads x size for a row, and the refusals of transposed ones, on the GPU's own tensors."""
+    n, k = 48, 512
+    w = eng.upload(Q.synthetic_weights(n, k, Q4_K, seed=2))
+    x, res = torch.randn(6, k, device="cuda"), torch.randn(6, n, device="cuda")
+    want = eng.linear(x, w, Q4_K, n, k, residual=res)
+    for a, b in ((x.reshape(-1), res.reshape(-1)), (x.reshape(6, 4, 128), res.reshape(6, 3, 16)),
+                 (x.reshape(2, 3, k), res.reshape(2, 3, n))):
+        assert torch.equal(eng.linear(a, w, Q4_K, n, k, residual=b), want)
+    heads = torch.randn(4, 6, 128, device="cuda").transpose(0, 1)  # not contiguous
+    assert torch.equal(eng.linear(heads, w, Q4_K, n, k), eng.linear(heads.reshape(6, k), w, Q4_K, n, k))
+    for bad in (dict(x=x.t().contiguous()), dict(residual=res.t().contiguous()), dict(residual=res.t()),
+                dict(out=torch.empty(n, 6, device="cuda"))):
+        with pytest.raises(_lib.NsqError) as e:
+            eng.linear(**dict(dict(x=x, w=w, ggml_type=Q4_K, n=n, k=k), **bad))
+        assert e.value.status == _lib.ERR_SHAPE, list(bad)

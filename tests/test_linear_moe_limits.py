@@ -222,3 +222,77 @@ def test_linear_refuses_outputs_over_its_weights(lib):
     if not torch.cuda.is_available():
         assert passes(linear_call(lib)) and passes(linear_call(lib, ws=last + 16)) and passes(linear_call(lib, y=last + 16))
         assert passes(linear_call(lib, 17, dtype=1, ws=A))  # no workspace is used
+
+
+# ---------------------------------------------------------------- shapes
+class Dev(Bytes):
+    """A tensor on a GPU as the host checks see it."""
+
+    def __init__(self, *shape, dtype=None):
+        import torch
+        n = 1
+        for s in shape:
+            n *= s
+        super().__init__(0, n)
+        self.shape, self.dtype = torch.Size(shape), dtype or torch.float32
+
+    def dim(self):
+        return len(self.shape)
+
+    def new_empty(self, shape, dtype=None):
+        return Dev(*shape, dtype=dtype or self.dtype)
+
+
+class Calls:
+    """libnsq that takes every call and does nothing."""
+
+    def __getattr__(self, name):
+        return lambda *a: 0
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    import torch
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    return engine_on("cuda:0", Calls()), dict(workspace=Dev(1 << 20, dtype=torch.uint8), sync=False)
+
+
+def test_linear_refuses_transposed_tensors(fake):
+    eng, kw = fake
+    w, k, n = Bytes(0), 256, 16
+
+    def call(x=Dev(3, 256), residual=None, out=None, n=n):
+        return eng.linear(x, w, 12, n, k, residual=residual, out=out, **kw)
+    for bad in (dict(x=Dev(256, 3)), dict(x=Dev(2, 256, 3)), dict(residual=Dev(16, 3)), dict(out=Dev(16, 3)),
+                dict(residual=Dev(4, 3, 4)), dict(x=Dev(6, 128))):
+        assert status_of(call, **bad) == _lib.ERR_SHAPE, list(bad.values())[0].shape
+    for good in (dict(), dict(x=Dev(768)), dict(x=Dev(3, 1, 256)), dict(x=Dev(3, 2, 128)), dict(residual=Dev(3, 16)),
+                 dict(residual=Dev(3, 4, 4)), dict(residual=Dev(1, 48)), dict(residual=Dev(48)),
+                 dict(residual=Dev(1, 3, 16), out=Dev(48)), dict(x=Dev(256)), dict(x=Dev(256, 1), residual=Dev(16, 1)),
+                 dict(x=Dev(1, 256), residual=Dev(1, 16)), dict(n=1, residual=Dev(1, 3)), dict(x=Dev(256), n=1, residual=Dev())):
+        call(**good)
+
+
+def test_moe_refuses_transposed_tensors(fake):
+    import torch
+    eng, kw = fake
+    moe = experts_of()
+    ids = Dev(4, 2, dtype=torch.int32)
+
+    def ffn(x=Dev(4, 256), weights=Dev(4, 2), residual=None, out=None, ids=ids):
+        return eng.moe_ffn(moe, x, ids, weights, residual=residual, out=out, **kw)
+
+    def layer(x=Dev(4, 256), router=Dev(2, 256), residual=None, out=None):
+        return eng.moe_layer(moe, router, x, 2, residual=residual, out=out, **kw)
+    for call in (ffn, layer):
+        for bad in (dict(x=Dev(256, 4)), dict(residual=Dev(256, 4)), dict(out=Dev(256, 4)), dict(out=Dev(2, 512))):
+            assert status_of(call, **bad) == _lib.ERR_SHAPE, bad
+        for good in (dict(), dict(x=Dev(2, 2, 256)), dict(x=Dev(1024)), dict(residual=Dev(1024), out=Dev(4, 1, 256))):
+            call(**good)
+    assert status_of(ffn, weights=Dev(2, 4)) == _lib.ERR_SHAPE
+    assert status_of(layer, router=Dev(256, 2)) == _lib.ERR_SHAPE
+    ffn(weights=Dev(8))
+    ffn(weights=Dev(4, 2, dtype=torch.float32))
+    layer(router=Dev(512))
+    ffn(x=Dev(256), ids=Dev(1, 2, dtype=torch.int32), weights=Dev(2))
