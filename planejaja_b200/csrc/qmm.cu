@@ -238,9 +238,6 @@ static int plan_qmm(QmmParams& p, int type, int64_t groups, int num_sms, QmmPlan
   int64_t grid = 0;
   for (int KW = 1; KW <= kQmmWarps; KW *= 2) {
     if (KW > 1 && KW / 2 >= most_units) break;
-    if (const int only = tune(kTuneQmmKW, 0)) {
-      if (KW < only && KW < kQmmWarps && KW < most_units) continue;
-    }
     QmmParams t = p;
     t.KW = KW;
     t.RW = kQmmWarps / KW;
@@ -251,6 +248,7 @@ static int plan_qmm(QmmParams& p, int type, int64_t groups, int num_sms, QmmPlan
     while (t.stages > 2 && fixed + t.PB * ys + t.stages * KW * slot > (size_t)kQmmSmemHalf) --t.stages;
     const size_t need = fixed + t.PB * ys + t.stages * KW * slot;
     if (need > (size_t)kQmmSmemMax) continue;
+    if (KW > 1 && KW / 2 < tune(kTuneQmmKW, 0)) smem = 0;  // fewer columns than asked for: only where more do not fit
     const int64_t here = need > (size_t)kQmmSmemHalf ? slots / 2 : slots;  // CTAs at a time
     const int64_t rows = (int64_t)(p.mode == kQmmUp ? 8 : 16) * f.MT * t.RW;
     // (an expert's share of the picks usually is one group)

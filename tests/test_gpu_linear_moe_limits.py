@@ -128,3 +128,38 @@ def test_shapes_that_hold_the_rows_otherwise(eng):
         with pytest.raises(_lib.NsqError) as e:
             eng.linear(**dict(dict(x=x, w=w, ggml_type=Q4_K, n=n, k=k), **bad))
         assert e.value.status == _lib.ERR_SHAPE, list(bad)
+
+
+# ---------------------------------------------------------------- launch-planning switches
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("kw", [1, 2, 4, 8])
+def test_switches_change_the_plan_and_not_the_result(eng, oracle, tuning, kw, split):
+    """Columns of K and the division of tasks set by hand, where the rings of 8 columns fit and where they do not
+    (9 to 16 tokens).  5e-6 and 1e-5 of the norm, as for the planner's own choices: the sums only meet in another
+    order, at most 8 columns and one part per unit."""
+    tuning.set("NSQ_QMM_KW", kw)
+    tuning.set("NSQ_QMM_SPLIT", split)
+    for t, k in ((Q4_K, 2048), (Q5_K, 1280), (Q6_K, 768), (Q4_0, 992), (Q8_0, 4096)):
+        n = 150
+        raw = Q.synthetic_weights(n, k, t, seed=k)
+        w, w64 = eng.upload(raw), oracle.dequant(raw, t, 0).reshape(n, k).astype(np.float64)
+        for m in (1, 3, 8, 16):
+            x = np.random.default_rng(m).standard_normal((m, k)).astype(np.float32)
+            y = eng.linear(torch.from_numpy(x).cuda(), w, t, n, k).double().cpu().numpy()
+            r = x.astype(np.float64) @ w64.T
+            assert np.linalg.norm(y - r) <= 5e-6 * np.linalg.norm(r), (t, m)
+    for m, e, d, f, t in ((2, 4, 512, 768, Q4_K), (40, 4, 256, 1024, Q8_0), (11, 6, 1056, 352, Q4_0)):
+        moe = experts(eng, e, d, f, t, t)
+        g, u, dn = (oracle.dequant(v.cpu().numpy()[:], t, 0).astype(np.float64) for v in (moe.w_gate, moe.w_up, moe.w_down))
+        g, u, dn = g.reshape(e, f, d), u.reshape(e, f, d), dn.reshape(e, d, f)
+        r = np.random.default_rng(m)
+        x = r.standard_normal((m, d)).astype(np.float32)
+        ids = np.stack([r.permutation(e)[:2] for _ in range(m)]).astype(np.int32)
+        wts = r.random((m, 2)).astype(np.float32)
+        y = eng.moe_ffn(moe, *(torch.from_numpy(v).cuda() for v in (x, ids, wts))).double().cpu().numpy()
+        want = np.zeros((m, d))
+        for i in range(m):
+            for j in range(2):
+                xe, c = x[i].astype(np.float64), ids[i, j]
+                want[i] += float(wts[i, j]) * (dn[c] @ (act64(g[c] @ xe, "silu") * (u[c] @ xe)))
+        assert np.linalg.norm(y - want) <= 1e-5 * np.linalg.norm(want), (t, m)
