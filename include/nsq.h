@@ -370,7 +370,10 @@ int nsq_moe_ffn(const nsq_moe* moe, const float* x, const int32_t* ids, const fl
  *   NSQ_SCORE_SIGMOID_NORM  s = sigmoid(logits), divided likewise
  * The picks are the top_k largest of s (+ sel_bias[E], which may be NULL and
  * does not enter the weights), largest first, of equal ones the lowest id;
- * a NaN score comes last.  ids and weights [M x top_k] are written. */
+ * a NaN score comes last.  Without sel_bias the softmax scores' order is taken
+ * from the logits: scores that would round to one value (0, far below the
+ * largest) keep it, and a NaN logit spoils no other expert's place.  ids and
+ * weights [M x top_k] are written. */
 #define NSQ_SCORE_SOFTMAX 0
 #define NSQ_SCORE_SOFTMAX_NORM 1
 #define NSQ_SCORE_SIGMOID_NORM 2

@@ -8,7 +8,7 @@ import torch
 from planejaja_b200 import _lib
 from planejaja_b200 import quantize as Q
 from planejaja_b200.formats import Q4_0, Q4_K, Q5_K, Q6_K, Q8_0
-from test_gpu_linear_moe import act64, bf16
+from test_gpu_linear_moe import act64, bf16, reference_route
 
 pytestmark = pytest.mark.gpu
 
@@ -163,3 +163,73 @@ def test_switches_change_the_plan_and_not_the_result(eng, oracle, tuning, kw, sp
                 xe, c = x[i].astype(np.float64), ids[i, j]
                 want[i] += float(wts[i, j]) * (dn[c] @ (act64(g[c] @ xe, "silu") * (u[c] @ xe)))
         assert np.linalg.norm(y - want) <= 1e-5 * np.linalg.norm(want), (t, m)
+
+
+# ---------------------------------------------------------------- routers
+def cuda(v):
+    return None if v is None else torch.from_numpy(v).cuda()
+
+
+def check_route(eng, moe, x, wr, k, score, bias, scale=1.5):
+    y, ids, wts = eng.moe_layer(moe, cuda(wr), cuda(x), k, score=score, sel_bias=cuda(bias), scale=scale)
+    ri, rw = reference_route(x, wr, score, bias, scale, k)
+    assert np.array_equal(ids.cpu().numpy(), ri)
+    assert np.all(np.abs(wts.double().cpu().numpy() - rw) <= 2.0 ** -23 * rw)  # f64 inside, rounded once
+    assert torch.equal(y, eng.moe_ffn(moe, cuda(x), ids, wts))
+
+
+@pytest.mark.parametrize("score", sorted(_lib.SCORES))
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("e", [33, 128, 129, 300, 512])
+def test_routers_of_many_experts(eng, e, with_bias, score):
+    """Up to 16 experts of a lane, with the last lanes' part filled and empty."""
+    moe = experts(eng, e, 256, 32, Q4_K, Q8_0)
+    r = np.random.default_rng(e)
+    wr = (r.standard_normal((e, 256)) / 16).astype(np.float32)
+    bias = (0.1 * r.standard_normal(e)).astype(np.float32) if with_bias else None
+    for m, k in ((1, 8), (21, 16), (64, 1)):
+        x = r.standard_normal((m, 256)).astype(np.float32)
+        check_route(eng, moe, x, wr, k, score, bias)
+    wr[:] = 0  # ties over all lanes: the lowest ids, or the order of the bias
+    check_route(eng, moe, x[:2].copy(), wr, 16, score, bias)
+    x, wr = np.ones((1, 256), np.float32), np.zeros((e, 256), np.float32)
+    wr[[e - 1, e // 2], 0] = 1.0
+    check_route(eng, moe, x, wr, 3, score, None)
+
+
+@pytest.mark.parametrize("d", [4064, 4096, 4128, 8192, 12320])
+@pytest.mark.parametrize("off", [0, 1])
+def test_routers_over_wide_rows(eng, d, off):
+    """Rows of one, two and four turns of the logits' CTA, whole and begun, with and without 16-byte alignment."""
+    moe = experts(eng, 5, d, 32, Q8_0, Q8_0)
+    r = np.random.default_rng(d)
+    wr = (r.standard_normal((5, d)) / np.sqrt(d)).astype(np.float32)
+    for m in (1, 11):
+        x = r.standard_normal((m, d)).astype(np.float32)
+        xd, wd = (torch.empty(v.size + 1, device="cuda")[off:off + v.size].copy_(cuda(v.reshape(-1))).reshape(v.shape)
+                  for v in (x, wr))
+        assert (xd.data_ptr() % 16 != 0) == bool(off)
+        y, ids, wts = eng.moe_layer(moe, wd, xd, 2)
+        ri, rw = reference_route(x, wr, "softmax_norm", None, 1.0, 2)
+        assert np.array_equal(ids.cpu().numpy(), ri)
+        assert np.all(np.abs(wts.double().cpu().numpy() - rw) <= 2.0 ** -23 * rw)
+        assert torch.equal(y, eng.moe_layer(moe, cuda(wr), cuda(x), 2)[0])
+
+
+def test_softmax_picks_go_by_the_logits(eng):
+    """Scores far below the largest round to 0 and keep their logits' order; a NaN logit comes last, alone."""
+    e = 40
+    moe = experts(eng, e, 256, 32, Q4_K, Q8_0)
+    x = np.zeros((1, 256), np.float32)
+    x[0, 0] = 1.0
+    wr = np.zeros((e, 256), np.float32)
+    wr[:, 0] = -2000.0 - np.arange(e)[::-1]
+    wr[7, 0] = 0.0
+    for score in ("softmax", "softmax_norm"):
+        _, ids, wts = eng.moe_layer(moe, cuda(wr), cuda(x), 4, score=score)
+        assert ids.tolist() == [[7, 39, 38, 37]] and wts.tolist() == [[1.0, 0.0, 0.0, 0.0]]
+    wr[39, 0] = np.nan
+    _, ids, wts = eng.moe_layer(moe, cuda(wr), cuda(x), 4, score="softmax_norm")
+    assert ids.tolist() == [[7, 38, 37, 36]] and wts.tolist() == [[1.0, 0.0, 0.0, 0.0]]
+    _, ids, _ = eng.moe_layer(moe, cuda(wr), cuda(x), 16, score="sigmoid_norm")
+    assert 39 not in ids.tolist()[0]
