@@ -7,7 +7,7 @@ import torch
 
 from planejaja_b200 import _lib
 from planejaja_b200 import quantize as Q
-from planejaja_b200.formats import Q4_0, Q4_K, Q5_K, Q6_K, Q8_0
+from planejaja_b200.formats import FORMATS, Q4_0, Q4_K, Q5_K, Q6_K, Q8_0
 from test_gpu_linear_moe import act64, bf16, reference_route
 
 pytestmark = pytest.mark.gpu
@@ -233,3 +233,84 @@ def test_softmax_picks_go_by_the_logits(eng):
     assert ids.tolist() == [[7, 38, 37, 36]] and wts.tolist() == [[1.0, 0.0, 0.0, 0.0]]
     _, ids, _ = eng.moe_layer(moe, cuda(wr), cuda(x), 16, score="sigmoid_norm")
     assert 39 not in ids.tolist()[0]
+
+
+# ---------------------------------------------------------------- tensors beyond 32-bit offsets, long and short shapes
+def device_blocks(rows, k, t, seed):
+    """Random GGUF blocks made on the GPU, their f16 scales small and finite."""
+    f = FORMATS[t]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    n = rows * k // f.block_weights
+    b = torch.randint(0, 256, (n, f.block_bytes), generator=g, device="cuda", dtype=torch.uint8)
+    places = {Q6_K: (208,), Q4_K: (0, 2), Q5_K: (0, 2)}.get(t, (0,))
+    for at in places:
+        scale = (torch.rand(n, generator=g, device="cuda") * 1e-3 + 1e-4).to(torch.float16)
+        b[:, at:at + 2] = scale.view(torch.uint8).reshape(n, 2)
+    return b.reshape(-1)
+
+
+@pytest.mark.parametrize("t,k", [(Q8_0, 8192), (Q6_K, 7936), (Q4_0, 8224)], ids=["aligned", "unaligned_q6k", "unaligned_q40"])
+def test_linear_rows_beyond_4_gb(eng, t, k):
+    """The last rows of a tensor of more than 4 GB against the same rows as a tensor of their own."""
+    rb = FORMATS[t].row_bytes(k)
+    n, last = (4 << 30) // rb + 3000, 259
+    w = device_blocks(n, k, t, 1)
+    tail = w[(n - last) * rb:].clone()
+    for m in (1, 6, 16):
+        x = torch.randn(m, k, device="cuda")
+        y = eng.linear(x, w, t, n, k)[:, -last:].double()
+        r = eng.linear(x, tail, t, last, k).double()
+        assert torch.linalg.norm(y - r) <= 1e-5 * torch.linalg.norm(r), m  # two results, each 5e-6 off
+    if k % 256 == 0:
+        x = torch.randn(40, k, device="cuda").bfloat16()
+        y, r = eng.linear(x, w, t, n, k)[:, -last:].double(), eng.linear(x, tail, t, last, k).double()
+        assert torch.linalg.norm(y - r) <= 2.0 ** -7 * torch.linalg.norm(r)  # both rounded to bf16
+
+
+@pytest.mark.parametrize("t,d,f", [(Q4_K, 4096, 4096), (Q6_K, 3584, 4352), (Q4_0, 4128, 4064)])
+def test_moe_experts_beyond_4_gb(eng, t, d, f):
+    """The last of many experts against a layer that has it alone (gate and up are one tensor here)."""
+    from planejaja_b200.engine import MoeExperts
+    up, down = f * FORMATS[t].row_bytes(d), d * FORMATS[t].row_bytes(f)
+    e = (33 << 27) // min(up, down) + 1
+    assert e <= 512
+    wu, wd = device_blocks(e * f, d, t, 2), device_blocks(e * d, f, t, 3)
+    assert min(wu.numel(), wd.numel()) > (4 << 30) + min(up, down)
+    many = MoeExperts(wu, wu, wd, e, d, f, t, t)
+    g, dn = wu[(e - 1) * up:].clone(), wd[(e - 1) * down:].clone()
+    one = MoeExperts(g, g, dn, 1, d, f, t, t)
+    for m in (1, 7, 33):
+        x = torch.randn(m, d, device="cuda")
+        wts = torch.rand(m, 1, device="cuda")
+        ids = torch.full((m, 1), e - 1, dtype=torch.int32, device="cuda")
+        y, r = eng.moe_ffn(many, x, ids, wts).double(), eng.moe_ffn(one, x, ids * 0, wts).double()
+        assert torch.linalg.norm(y - r) <= 2e-5 * torch.linalg.norm(r), m  # two results, each 1e-5 off
+
+
+def test_prompt_outputs_beyond_2_to_31_elements(eng):
+    m, n, k = 65600, 33000, 256
+    w = eng.upload(Q.synthetic_weights(n, k, Q4_K, seed=4))
+    x = torch.randn(m, k, device="cuda").bfloat16()
+    b = torch.randn(n, device="cuda")
+    y = eng.linear(x, w, Q4_K, n, k, bias=b, act="silu")
+    assert y.numel() > 2 ** 31
+    for rows in (slice(0, 200), slice(m - 200, m), slice(m // 2, m // 2 + 200)):
+        r = eng.linear(x[rows], w, Q4_K, n, k, bias=b, act="silu").double()
+        assert torch.linalg.norm(y[rows].double() - r) <= 2.0 ** -7 * torch.linalg.norm(r)
+
+
+@pytest.mark.parametrize("m", [1, 4, 9])
+@pytest.mark.parametrize("n,k,t", [(1, 1 << 20, Q8_0), (3, 1 << 20, Q6_K), (1 << 20, 32, Q4_0), (1 << 18, 256, Q5_K)])
+def test_linear_long_and_flat(eng, oracle, m, n, k, t):
+    """One row of a million, a million rows of one block.  With independent roundings (2^-24 of the partial sums, up
+    to 3 times the result, at each of nsb units and 33 joins; 1.4e-6 for the activations) an output is off by
+    3 * 2^-24 sqrt(33 + nsb) + 1.4e-6 of its terms' root sum of squares; 5e-6 at least is allowed."""
+    w = device_blocks(n, k, t, n + k)
+    x = torch.randn(m, k, device="cuda")
+    y = eng.linear(x, w, t, n, k).double()
+    w64 = torch.from_numpy(oracle.dequant(w.cpu().numpy(), t, 0).reshape(n, k)).cuda().double()
+    r = x.double() @ w64.t()
+    size = torch.sqrt((x.double() ** 2) @ (w64 ** 2).t())
+    tol = max(5e-6, 1.4e-6 + 3 * 2.0 ** -24 * (33 + -(-k // 256)) ** 0.5)
+    assert torch.linalg.norm(y - r) <= tol * torch.linalg.norm(size)
