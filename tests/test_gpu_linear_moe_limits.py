@@ -314,3 +314,35 @@ def test_linear_long_and_flat(eng, oracle, m, n, k, t):
     size = torch.sqrt((x.double() ** 2) @ (w64 ** 2).t())
     tol = max(5e-6, 1.4e-6 + 3 * 2.0 ** -24 * (33 + -(-k // 256)) ** 0.5)
     assert torch.linalg.norm(y - r) <= tol * torch.linalg.norm(size)
+
+
+@pytest.mark.parametrize("act", sorted(_lib.ACTS))
+@pytest.mark.parametrize("m,dtype", [(2, torch.float32), (2, torch.bfloat16), (17, torch.bfloat16)])
+def test_activations_over_all_values(eng, m, dtype, act):
+    """x = 0, so that bias is what the activation gets: small, large, infinite and NaN values against the formula in
+    64 bits, written without the cancellation of 1 + erf and 1 + tanh far below 0.
+
+    In half steps of f32 (2^-24): gelu's argument v / sqrt 2 has 2 roundings, and erfc falls by 2 x^2 of itself per
+    relative change of x, x^2 <= 88; the argument of gelu_tanh's exponential, up to 88, has 7 (4 of them in the
+    cube); the functions and what follows them at most 12.  A bf16 result adds its rounding (2^-8 here, twice the
+    half step, which leaves room for the fast exponential of prompts: 2 + 1.16 * 88 steps of f32).  An exponential
+    below 1e-30 may be lost."""
+    v = np.concatenate([s * np.float32(10.0) ** np.arange(-30, 31, 3) for s in (-1, 1)] + [np.linspace(-100, 100, 401)])
+    v = np.concatenate([v, [0.0, -0.0, np.inf, -np.inf, np.nan, 3e38, -3e38]]).astype(np.float32)
+    n, k = v.size, 256
+    w = eng.upload(Q.synthetic_weights(n, k, Q4_K, seed=0))
+    x = torch.zeros(m, k, device="cuda", dtype=dtype)
+    y = eng.linear(x, w, Q4_K, n, k, bias=torch.from_numpy(v).cuda(), act=act).double().cpu()
+    d = torch.from_numpy(v).double()
+    r = {"none": d, "silu": d * torch.sigmoid(d), "gelu": 0.5 * d * torch.erfc(-d / 2 ** 0.5),
+         "gelu_tanh": d * torch.sigmoid(2 * (2 / np.pi) ** 0.5 * (d + 0.044715 * d ** 3)),
+         "relu": torch.where(d < 0, 0.0, d)}[act]  # (-inf * 0 is NaN)
+    eps = 2.0 ** -24 * (12 + 88 * {"gelu": 4, "gelu_tanh": 7}.get(act, 0)) + (2.0 ** -8 if dtype is torch.bfloat16 else 0)
+    for i in range(m):
+        assert torch.equal(y[i].isnan(), r.isnan())
+        # (in bf16 3e38 may round to infinity)
+        ok = r.isfinite() if dtype is torch.float32 else r.abs() < 3e38
+        over = (y[i][ok] - r[ok]).abs() / (eps * r[ok].abs() + 1e-30)
+        worst = int(over.argmax())
+        assert float(over[worst]) <= 1, (float(d[ok][worst]), float(y[i][ok][worst]), float(r[ok][worst]))
+        assert torch.equal(y[i][r.isinf()], r[r.isinf()])
