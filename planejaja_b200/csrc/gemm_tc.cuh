@@ -14,18 +14,22 @@
 // against 582 with 256.  K advances in blocks of 64 (one 128-byte swizzle
 // atom of bf16).
 //
-// Warp roles (384 threads):
+// Warp roles (640 threads):
 //   warp 0      : TMA producer -- one thread loads the x tile [TOK x 64]
 //                 (2-D tiled bulk tensor copies, 128B swizzle) per K block.
 //   warp 1      : allocates TMEM; one lane issues 4 tcgen05.mma
 //                 (kind::f16, bf16 inputs, fp32 accumulate, K = 16 each)
 //                 per K block and 256 tokens and commits them to the
 //                 stage's "empty" barrier, and finally to the accumulator's.
-//   warps 4..11 : dequant producers -- 2 threads per W row turn the GGUF
-//                 blocks of the K block into bf16 and store them in the
-//                 same 128B-swizzled K-major layout TMA uses; then the
-//                 epilogue: tcgen05.ld of the accumulator, bf16 convert,
-//                 store to y.
+//   warp 2      : raw GGUF bytes of the CTA's 128 rows, 256 of K at a time.
+//   warp 3      : nsq_linear's residuals of the tile into L2.
+//   warps 4..19 : dequant producers -- they turn the GGUF blocks into bf16
+//                 and store them in the same 128B-swizzled K-major layout
+//                 TMA uses: where the ring holds four K blocks a warp takes
+//                 one of them for 32 rows, 64 weights a thread, else all 16
+//                 share each K block, 16 weights a thread; then the
+//                 epilogue: tcgen05.ld of the accumulator, for nsq_linear
+//                 bias, activation and residual, bf16 convert, store to y.
 // W and x tiles go round in rings guarded by mbarriers.  Every wait is bounded
 // (%globaltimer); a wait that gives up records NSQ_ERR_TIMEOUT and the
 // kernel winds down instead of hanging.
@@ -325,7 +329,9 @@ struct GemmParams {
 // v (1 + erf(v / sqrt 2)) / 2 = v Phi(v), with h = Phi(-|v|) = erfc(u) / 2 at
 // u = |v| / sqrt 2 written as e^(-u^2) P(t), t = 1 / (1 + u / 2); P is the
 // polynomial of degree 7 without a constant term fitted to e^(u^2) erfc(u) / 2
-// over u = 0..10 for the least largest relative error, 1.4e-6.  With the f32
+// over u = 0..10 for the least largest relative error, 1.4e-6 (least squares
+// of the relative error at 20001 points, the weights multiplied by the error
+// after each turn until it is level).  With the f32
 // roundings h is off by at most 8e-6 of itself for |v| <= 13 and 8e-7
 // absolutely: far inside the result's rounding to bf16, and a third of the
 // instructions of erfcf.
@@ -884,9 +890,11 @@ static int launch_gemm_t(const void* x, const CUtensorMap& wmap, const GemmParam
   GemmParams p = p0;
   const int64_t tiles_n = (p.N + GEMM_BM - 1) / GEMM_BM, tiles_m = (p.M + TOK - 1) / TOK;
   if (tiles_m > 65535) return NSQ_ERR_SHAPE;
-  // Split-K (nsq_gemm_bf16; the order of its sums hangs on it) when the tiles leave most SMs idle: S CTAs per tile (cluster),
-  // as many as the SMs allow, at most 4, each with >= 2 K columns, and no
-  // more partial-sum slots than the leader's stage buffers hold.
+  // Split-K, S CTAs per tile (a cluster).  nsq_linear: as gemm_consider chose.
+  // nsq_gemm_bf16: when the tiles leave most SMs idle, as many as the SMs
+  // allow, at most 4, each with >= 2 K columns, and by a bound on the stage
+  // buffers (slots for S - 1 ranks' whole sums) that the join below no longer
+  // needs; it stays, as the order of that call's sums hangs on S.
   constexpr size_t region = (size_t)gemm_stages<TYPE, TOK>() * (GEMM_BM * 128 + TOK * 128) +
                             (size_t)GEMM_RAW_STAGES * GEMM_BM * RawCol<TYPE>::pitch;
   int S = 1;
@@ -951,7 +959,10 @@ static int gemm_clusters(int S, int num_sms) {
 // 2.5, 6 and 11 us.  M = 333, N = 1003, K = 2816 (Q8_0): 128 tokens, S = 4
 // 14 us; 256 tokens, S = 4 18 us; 128 tokens, S = 8 (24 clusters, 2 waves)
 // 25 us.  M = 1000, N = K = 4096: 256 tokens, S = 1 42 us; 512, S = 2 46 us;
-// 128, S = 1 74 us.
+// 128, S = 1 74 us.  These costs were taken before the MMA warp went round
+// together.  Since then a column costs 1.8 us with 128 or 256 tokens and 2.7 to
+// 3.7 us with 512, and the same choices in one run take 15.5, 19.7 and 25.9 us
+// and 41, 48 and 71 us: the order, and so the choice, is the same.
 template <int TYPE, int LAYOUT, int TOK>
 static void gemm_consider(const GemmParams& p, int num_sms, int64_t* best, int* tok, int* split) {
   constexpr int64_t kColumn = TOK == 128 ? 10 : TOK == 512 ? 19 : gemm_w_stages<TYPE, TOK>() >= 4 ? 13 : 17;

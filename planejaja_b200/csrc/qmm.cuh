@@ -17,20 +17,28 @@
 //               2048, exact in fp16):  - dmin * sum m T  by one fp16 MMA
 //   Q6_K        the same with 16-weight groups; q - 32 through T
 //   Q4_0, Q8_0  one f32 scale per 32 weights; q - 8 through T
-// An activation is off by at most max / 2^24 of its 256, a limb's f32 value by
+// With max the largest of its 256 an activation v is off by at most max / 2^22:
+// 1 / s and s are each off by 2^-24 of themselves (2 |v| / 2^24), the product
+// v / s, below 2^23, by a quarter and its rounding to X by a half of a step s =
+// max / 8355710 (1.51 max / 2^24); small v lose little more than the half step,
+// max / 2^24.  (max below 2^-63: s is a power of two, the half step at most
+// max / 2^22, and below 2^-120 it is 2^-142.)  So values far below an outlier
+// of their 256 keep fewer bits than f32 has.  A limb's f32 value is off by
 // 2^-24 of the limb's sum: norm errors of a product are about 2e-7.
 //
 // Measured on B200: the byte MMA (4096 products), the fp16 MMA (2048), take 8
 // cycles of a scheduler each; logic, permutes, IMAD and fp16x2 take 2.  A
 // first form with fp16 operands (x as hi + lo, two columns a token, q * sc in
-// fp16) needs a multiply or subtract per pair of weights beside the mask, 290
-// cycles a tile of 16 x 256; this one masks four weights at a time, about 170.
+// fp16) needs a multiply or subtract per pair of weights beside the mask; this
+// one masks four weights at a time.  Counted for Q4_K and one n-tile of tokens,
+// 290 against about 170 cycles per 16 x 256 weights.
 //
 // What bounds it.  Up to 4 tokens HBM and the start and end of a kernel: two
 // experts' [14336 x 4096] Q4_K in 61 us are 3.2 TB/s with 10 us of routing and
 // starts; Q5_K [28672 x 8192], 3 tokens, 47 us = 3.4 TB/s, its fifth bits' logic.
-// From five tokens on instructions: 400 a tile of 16 x 256 at 0.6 a cycle and
-// scheduler, 16 tokens over 8 experts 301 us = 3.0 TB/s.
+// From five tokens on instructions: with groups of up to 8 tokens (three
+// n-tiles) 400 per 16 x 256 weights, loads and bookkeeping included, at 0.6 a
+// cycle and scheduler; 16 tokens over 8 experts 301 us = 3.0 TB/s.
 //
 // Layout.  A CTA is 8 warps = RW row tiles of 16 MT weight rows x KW columns.
 // A task is a tile of 16 MT RW rows; its units of 256 weights of K are dealt
