@@ -346,3 +346,41 @@ def test_activations_over_all_values(eng, m, dtype, act):
         worst = int(over.argmax())
         assert float(over[worst]) <= 1, (float(d[ok][worst]), float(y[i][ok][worst]), float(r[ok][worst]))
         assert torch.equal(y[i][r.isinf()], r[r.isinf()])
+
+
+# ---------------------------------------------------------------- captures
+def test_captured_behind_copies_and_between_streams(eng):
+    """One graph: inputs copied from the host, two branches of products that meet in a layer, its output copied back."""
+    d, e, f = 512, 8, 768
+    moe = experts(eng, e, d, f, Q4_K, Q6_K)
+    w = [eng.upload(Q.synthetic_weights(d, d, t, seed=t)) for t in (Q4_K, Q8_0)]
+    wr = torch.randn(e, d, device="cuda")
+    host, back = torch.empty(3, d).pin_memory(), torch.empty(3, d).pin_memory()
+    x = torch.empty(3, d, device="cuda")
+    ws = [eng.linear_workspace(3, d, d), eng.linear_workspace(3, d, d), eng.moe_workspace(moe, 3, 2)]
+
+    def step(sync):
+        side, main = torch.cuda.Stream(), torch.cuda.current_stream()
+        x.copy_(host, non_blocking=True)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b = eng.linear(x, w[1], Q8_0, d, d, act="silu", workspace=ws[1], sync=sync)
+        a = eng.linear(x, w[0], Q4_K, d, d, workspace=ws[0], sync=sync)
+        main.wait_stream(side)
+        y, _, _ = eng.moe_layer(moe, wr, a, 2, residual=b, workspace=ws[2], sync=sync)
+        z = eng.linear(y, w[0], Q4_K, d, d, residual=a, workspace=ws[0], sync=sync)
+        back.copy_(z, non_blocking=True)
+        b.record_stream(main)
+        return z
+    host.normal_()
+    step(True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        z = step(False)
+    for _ in range(5):
+        host.normal_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = z.clone()
+        assert torch.equal(back, got.cpu())
+        assert torch.equal(step(True), got)
